@@ -34,15 +34,23 @@ def nvcc() -> str:
     raise RuntimeError("nvcc not found: the CUDA toolkit is required to build linattn_b200")
 
 
-def _deps_mtime() -> float:
-    return max(p.stat().st_mtime for p in [*CSRC.glob("*.cuh"), *INCLUDE.glob("*.h")])
+def _deps_mtime(obj: Path) -> float:
+    """Newest of the project headers that the object was compiled from (nvcc's dependency
+    file); every header where there is no such file yet."""
+    headers = [*CSRC.glob("*.cuh"), *INCLUDE.glob("*.h")]
+    dep = obj.with_suffix(".d")
+    if dep.exists():
+        used = {Path(w).resolve() for w in dep.read_text().replace("\\\n", " ").split()}
+        headers = [h for h in headers if h.resolve() in used]
+    return max((h.stat().st_mtime for h in headers), default=0.0)
 
 
 def _compile(src: Path, force: bool) -> Path:
     obj = OBJ_DIR / (src.stem + ".o")
-    if not force and obj.exists() and obj.stat().st_mtime >= max(src.stat().st_mtime, _deps_mtime()):
+    if not force and obj.exists() and obj.stat().st_mtime >= max(src.stat().st_mtime, _deps_mtime(obj)):
         return obj
-    cmd = [nvcc(), *NVFLAGS, f"-I{INCLUDE}", f"-I{CSRC}", "-c", str(src), "-o", str(obj)]
+    cmd = [nvcc(), *NVFLAGS, "-MMD", "-MF", str(obj.with_suffix(".d")), f"-I{INCLUDE}", f"-I{CSRC}", "-c", str(src),
+           "-o", str(obj)]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"nvcc failed on {src.name}:\n{res.stderr}")
