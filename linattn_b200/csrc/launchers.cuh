@@ -70,6 +70,9 @@ bool indexer_scores_mma(const void* q, int q_dtype, const int64_t* qs, const voi
 // and 128-byte swizzle, from a process-wide cache.  False if encoding fails.
 bool tensor_map_2d(CUtensorMap* out, const void* base, CUtensorMapDataType cu_dtype, int64_t inner, int64_t rows,
                    int64_t stride_bytes, int box_inner, int box_rows);
+// 3-D TMA tensor map {inner, middle, outer} with 128-byte swizzle (encoded on every call).
+bool tensor_map_3d(CUtensorMap* out, const void* base, CUtensorMapDataType cu_dtype, const int64_t dims[3],
+                   const int64_t stride_bytes[2], const int box[3]);
 int tile_rows_f32(int D);
 int tile_rows_f16(int D);
 int tile_rows_bf16(int D);

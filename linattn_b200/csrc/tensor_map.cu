@@ -75,4 +75,19 @@ bool tensor_map_2d(CUtensorMap* out, const void* base, CUtensorMapDataType cu_dt
   return true;
 }
 
+bool tensor_map_3d(CUtensorMap* out, const void* base, CUtensorMapDataType cu_dtype, const int64_t dims[3],
+                   const int64_t stride_bytes[2], const int box[3]) {
+  PFN_cuTensorMapEncodeTiled_v12000 fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t d[3] = {static_cast<cuuint64_t>(dims[0]), static_cast<cuuint64_t>(dims[1]),
+                           static_cast<cuuint64_t>(dims[2])};
+  const cuuint64_t s[2] = {static_cast<cuuint64_t>(stride_bytes[0]), static_cast<cuuint64_t>(stride_bytes[1])};
+  const cuuint32_t b[3] = {static_cast<cuuint32_t>(box[0]), static_cast<cuuint32_t>(box[1]),
+                           static_cast<cuuint32_t>(box[2])};
+  const cuuint32_t elem_strides[3] = {1u, 1u, 1u};
+  return fn(out, cu_dtype, 3, const_cast<void*>(base), d, s, b, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 }  // namespace linattn
