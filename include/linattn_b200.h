@@ -525,6 +525,100 @@ int linattn_shard_merge(const float* scores, const int32_t* ids, int64_t R, int6
                         int64_t max_union, const int32_t* seq_lens, int64_t page_size, int32_t* union_tokens,
                         void* stream);
 
+/*
+ * Causal attention over packed sequences with grouped heads.  q (N_q, H_q, D) and
+ * k, v (N_k, H_kv, D) hold S sequences one after the other: sequence s owns the query
+ * rows [cu_q[s], cu_q[s + 1]) and the key rows [cu_k[s], cu_k[s + 1]) (int32, device,
+ * ascending from 0).  Its last query stands at its last key: query i reads the keys
+ * j <= i + len_k - len_q (every key with causal = 0); a query that reads nothing gets
+ * o = 0 and lse = -inf.  bf16 or f16 (one type), D 64 or 128, at most 128 query heads to
+ * a kv head.  Strides in elements {token, head}, channels contiguous, rows and strides
+ * multiples of 16 bytes.  lse (N_q, H_q) contiguous, or NULL.  max_q / max_k: at least the
+ * longest sequence's query / key rows (they size the grid; rows beyond them are not
+ * written).  n_splits > 1 cuts every key range and merges the parts through
+ * `workspace` (linattn_packed_attention_workspace bytes, 16-byte aligned);
+ * linattn_packed_attention_splits proposes a number.  Offsets that are not ascending or
+ * leave the buffers are clamped and reported (LINATTN_DEV_BAD_ID).  No reference
+ * counterpart in one operator: dense_attention over each sequence
+ * (src/linattn/core.py:148-181).
+ */
+int linattn_packed_attention(const void* q, const void* k, const void* v, int32_t dtype, int64_t N_q, int64_t N_k,
+                             int64_t Hq, int64_t Hkv, int64_t D, const int64_t* q_strides /*[2]*/,
+                             const int64_t* k_strides /*[2]*/, const int64_t* v_strides /*[2]*/, const int32_t* cu_q,
+                             const int32_t* cu_k, int64_t S, int64_t max_q, int64_t max_k, int32_t causal, float scale,
+                             void* out, const int64_t* out_strides /*[2]*/, float* lse, int32_t n_splits,
+                             void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
+int32_t linattn_packed_attention_splits(int64_t N_q, int64_t Hq, int64_t Hkv, int64_t S, int64_t max_q, int64_t max_k);
+int64_t linattn_packed_attention_workspace(int64_t N_q, int64_t Hq, int64_t D, int32_t n_splits);
+
+/*
+ * Attention weight that each key has received: mass[h, j] = sum over the queries i of
+ * j's sequence (its last `window` ones; 0 = all) that read key j, and over the query heads
+ * of kv head h, of exp(scale * q_i . k_j - lse[i, head]).  Arguments as
+ * linattn_packed_attention, lse as it writes it (a row with lse = -inf adds nothing); mass
+ * (H_kv, N_k) fp32 with row stride mass_stride, every key of a sequence written.
+ * n_splits > 1 cuts the queries and sums the parts in a fixed order through `workspace`.
+ */
+int linattn_attention_mass(const void* q, const void* k, int32_t dtype, int64_t N_q, int64_t N_k, int64_t Hq,
+                           int64_t Hkv, int64_t D, const int64_t* q_strides /*[2]*/, const int64_t* k_strides /*[2]*/,
+                           const float* lse, const int32_t* cu_q, const int32_t* cu_k, int64_t S, int64_t max_q,
+                           int64_t max_k, int32_t causal, int64_t window, float scale, float* mass, int64_t mass_stride,
+                           int32_t n_splits, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
+int32_t linattn_attention_mass_splits(int64_t Hq, int64_t Hkv, int64_t S, int64_t max_q, int64_t max_k, int64_t window);
+int64_t linattn_attention_mass_workspace(int64_t N_k, int64_t Hkv, int32_t n_splits);
+
+/*
+ * Heavy-hitter cache: `budget` slots per (sequence, kv head).  k, v (batch, n_kv_heads,
+ * budget, head_dim), mass fp32 and pos int32 (batch, n_kv_heads, budget), seen int32
+ * (batch): tokens taken so far, min(seen, budget) slots in use.  All contiguous, 16-byte
+ * aligned.  sinks + recent <= budget, recent >= 1.  The eviction rule keeps what the
+ * reference's eviction variants call heavy hitters (src/linattn/variants/eviction.py),
+ * as a cache that holds nothing else.
+ */
+typedef struct {
+  void* k;
+  void* v;
+  float* mass;
+  int32_t* pos;
+  int32_t* seen;
+  int32_t dtype, batch, n_kv_heads, budget, head_dim, sinks, recent;
+} linattn_heavy_t;
+
+/*
+ * Packed prompts into the cache: sequence s of k, v (N, H_kv, head_dim) (strides {token,
+ * head} in elements) fills cache row rows[s] (rows NULL: row s).  A sequence of at most
+ * `budget` tokens is kept whole; of a longer one the first `sinks`, the last `recent` and
+ * those of most mass among the rest (lowest position on ties, NaN above all), in ascending
+ * position.  mass (H_kv, N), row stride mass_stride.  The row's masses, positions and
+ * `seen` are replaced.
+ */
+int linattn_heavy_load(const linattn_heavy_t* cache, const void* k, const void* v, const int64_t* k_strides /*[2]*/,
+                       const int64_t* v_strides /*[2]*/, int64_t N, const float* mass, int64_t mass_stride,
+                       const int32_t* cu, const int32_t* rows, int64_t S, int32_t* status, void* stream);
+
+/*
+ * T_new tokens of every sequence, one after the other: k_new, v_new (batch, n_kv_heads,
+ * T_new, head_dim) in the cache's dtype, strides {sequence, head, token} in elements.  A
+ * token takes the next empty slot, or in a full cache the slot of least mass (lowest slot
+ * on ties) among those with sinks <= pos <= position - recent; its mass starts at 0.
+ * ticket: `batch` int32 of scratch that holds zeros before and after every call.
+ */
+int linattn_heavy_append(const linattn_heavy_t* cache, const void* k_new, const void* v_new,
+                         const int64_t* k_strides /*[3]*/, const int64_t* v_strides /*[3]*/, int64_t T_new,
+                         int32_t* ticket, int32_t* status, void* stream);
+
+/*
+ * One query token per sequence over the slots in use: o = softmax(scale q . K) V, and with
+ * accumulate != 0 each slot's mass grows by its weights summed over the group's query
+ * heads.  q, out (batch, H_q, head_dim) in the cache's dtype, strides {sequence, head} in
+ * elements.  f16 / bf16, head_dim 64 or 128.  A sequence without slots gets o = 0.
+ * workspace: linattn_heavy_attend_workspace bytes (0 for most sizes), 16-byte aligned.
+ */
+int linattn_heavy_attend(const linattn_heavy_t* cache, const void* q, int64_t Hq, const int64_t* q_strides /*[2]*/,
+                         float scale, int32_t accumulate, void* out, const int64_t* out_strides /*[2]*/,
+                         void* workspace, int64_t workspace_bytes, void* stream);
+int64_t linattn_heavy_attend_workspace(int64_t batch, int64_t Hq, int64_t Hkv, int64_t budget);
+
 
 #ifdef __cplusplus
 }

@@ -49,6 +49,14 @@ class KV(ctypes.Structure):
     ]
 
 
+class Heavy(ctypes.Structure):
+    _fields_ = [
+        ("k", c_vp), ("v", c_vp), ("mass", c_vp), ("pos", c_vp), ("seen", c_vp),
+        ("dtype", c_i32), ("batch", c_i32), ("n_kv_heads", c_i32), ("budget", c_i32), ("head_dim", c_i32),
+        ("sinks", c_i32), ("recent", c_i32),
+    ]
+
+
 def rows_addressable(t: torch.Tensor, head_dim: int) -> int:
     """D-element rows reachable from ``t.data_ptr()`` to the end of its storage."""
     nbytes = t.untyped_storage().nbytes() - t.storage_offset() * t.element_size()
@@ -134,6 +142,30 @@ def _declare(lib: ctypes.CDLL) -> None:
                                                     c_i64, c_vp, c_i64, c_i32, c_i32, c_i64, c_vp, c_vp, c_vp, c_i64,
                                                     c_vp, c_vp, c_vp]
     lib.linattn_lse_combine_strided.argtypes = [c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_i64, c_vp, c_i32, c_vp, c_vp]
+    lib.linattn_packed_attention.argtypes = [c_vp, c_vp, c_vp, c_i32, c_i64, c_i64, c_i64, c_i64, c_i64, P(c_i64),
+                                             P(c_i64), P(c_i64), c_vp, c_vp, c_i64, c_i64, c_i64, c_i32,
+                                             ctypes.c_float, c_vp, P(c_i64), c_vp, c_i32, c_vp, c_i64, c_vp, c_vp]
+    lib.linattn_packed_attention_splits.argtypes = [c_i64] * 6
+    lib.linattn_packed_attention_splits.restype = c_i32
+    lib.linattn_packed_attention_workspace.argtypes = [c_i64, c_i64, c_i64, c_i32]
+    lib.linattn_packed_attention_workspace.restype = c_i64
+    lib.linattn_attention_mass.argtypes = [c_vp, c_vp, c_i32, c_i64, c_i64, c_i64, c_i64, c_i64, P(c_i64), P(c_i64),
+                                           c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i32, c_i64, ctypes.c_float, c_vp,
+                                           c_i64, c_i32, c_vp, c_i64, c_vp, c_vp]
+    lib.linattn_attention_mass_splits.argtypes = [c_i64] * 6
+    lib.linattn_attention_mass_splits.restype = c_i32
+    lib.linattn_attention_mass_workspace.argtypes = [c_i64, c_i64, c_i32]
+    lib.linattn_attention_mass_workspace.restype = c_i64
+    lib.linattn_heavy_load.argtypes = [P(Heavy), c_vp, c_vp, P(c_i64), P(c_i64), c_i64, c_vp, c_i64, c_vp, c_vp, c_i64,
+                                       c_vp, c_vp]
+    lib.linattn_heavy_append.argtypes = [P(Heavy), c_vp, c_vp, P(c_i64), P(c_i64), c_i64, c_vp, c_vp, c_vp]
+    lib.linattn_heavy_attend.argtypes = [P(Heavy), c_vp, c_i64, P(c_i64), ctypes.c_float, c_i32, c_vp, P(c_i64), c_vp,
+                                         c_i64, c_vp]
+    lib.linattn_heavy_attend_workspace.argtypes = [c_i64] * 4
+    lib.linattn_heavy_attend_workspace.restype = c_i64
+    for name in ("linattn_packed_attention", "linattn_attention_mass", "linattn_heavy_load", "linattn_heavy_append",
+                 "linattn_heavy_attend"):
+        getattr(lib, name).restype = ctypes.c_int
     for name in ("linattn_read_bandwidth", "linattn_block_score_topk", "linattn_shard_merge", "linattn_quest_decode_candidates", "linattn_lse_combine_strided", "linattn_block_sparse_prefill", "linattn_prefill_v_to_f16", "linattn_block_mean", "linattn_csa2_pool_quant", "linattn_merge_block_lists", "linattn_token_attention", "linattn_indexer_scores", "linattn_row_topk", "linattn_page_bounds", "linattn_paged_page_bounds", "linattn_paged_append", "linattn_quest_scores", "linattn_page_topk",
                  "linattn_sparse_attention", "linattn_lse_combine", "linattn_lse_combine_strided"):
         getattr(lib, name).restype = ctypes.c_int
@@ -179,6 +211,14 @@ def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 def strides4(t: torch.Tensor):
     return (c_i64 * 4)(*t.stride())
+
+
+def strides3(t: torch.Tensor):
+    return (c_i64 * 3)(*t.stride()[:3])
+
+
+def strides2(t: torch.Tensor):
+    return (c_i64 * 2)(*t.stride()[:2])
 
 
 def stream_of(t: torch.Tensor) -> int:

@@ -1,0 +1,49 @@
+// Tiles of packed sequences: which rows of which sequence a CTA works on, found on the
+// device from the offsets, so that no call needs them on the host.
+#pragma once
+
+#include "common.cuh"
+
+namespace linattn {
+
+// Rows [first, first + n) of sequence s.  Offsets that are not ascending or leave [0, N]
+// are clamped; false if they had to be.
+__device__ __forceinline__ bool packed_range(const int32_t* cu, int s, int64_t N, int* first, int* n) {
+  const int64_t a = cu[s], b = cu[s + 1];
+  const int64_t lo = lmin(lmax(a, 0), N), hi = lmin(lmax(b, lo), N);
+  *first = static_cast<int>(lo);
+  *n = static_cast<int>(hi - lo);
+  return a == lo && b == hi;
+}
+
+// Sequence and tile of the `idx`-th tile of `rows` rows, sequence after sequence; all
+// lanes of a warp call it and get the same answer.  False past the last tile.
+__device__ __forceinline__ bool packed_tile(const int32_t* cu, int S, int64_t N, int rows, int64_t idx, int* seq,
+                                            int* tile) {
+  const int lane = threadIdx.x & 31;
+  int64_t base = 0;
+  for (int s0 = 0; s0 < S; s0 += 32) {
+    int first, n = 0;
+    if (s0 + lane < S) (void)packed_range(cu, s0 + lane, N, &first, &n);
+    const int mine = (n + rows - 1) / rows;
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    const int total = __shfl_sync(0xffffffffu, incl, 31);
+    if (idx < base + total) {
+      const int off = static_cast<int>(idx - base);
+      const unsigned owner = __ballot_sync(0xffffffffu, off >= incl - mine && off < incl);
+      const int l = __ffs(owner) - 1;
+      *seq = s0 + l;
+      *tile = off - __shfl_sync(0xffffffffu, incl - mine, l);
+      return true;
+    }
+    base += total;
+  }
+  return false;
+}
+
+}  // namespace linattn

@@ -1,0 +1,152 @@
+"""A cache of fixed size that keeps the heavy hitters: attention-weight eviction.
+
+Where the paged cache keeps every token and selects what a query reads, this one keeps, per
+sequence and kv head, ``budget`` tokens: the first ``sinks``, the last ``recent`` and, of the
+rest, the ones that have received the most attention weight (the eviction family of
+``src/linattn/variants/eviction.py``, as a physical cache that holds nothing else).
+
+    o, lse = packed_attention(q, k, v, cu)              # the prompts
+    mass = attention_mass(q, k, lse, cu)                # what each key received
+    cache.load(k, v, mass, cu)                          # cut to the budget
+    while decoding:
+        o = cache.step(q, k_new, v_new)                 # replace the least slot, attend, add up
+
+``k, v (B, H_kv, budget, D)``: a (sequence, kv head) is one contiguous block of rows, so
+decoding streams it; slots are not ordered by position (attention does not depend on the
+order of its keys), ``pos`` says which token a slot holds.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Optional
+
+import torch
+
+from linattn_b200 import _lib as L
+
+__all__ = ["HeavyCache"]
+
+
+class HeavyCache:
+    """``budget`` slots per (sequence, kv head) with accumulated attention weights.
+
+    Every update runs on the device and on the current stream: no host copy of the lengths,
+    no allocation, so a decode step can be captured in a CUDA graph.  ``seen (B,)`` counts
+    the tokens of each sequence; ``min(seen, budget)`` slots are in use."""
+
+    def __init__(self, batch: int, n_kv_heads: int, head_dim: int, budget: int, *, sinks: int = 0, recent: int = 1,
+                 dtype: torch.dtype = torch.bfloat16, device="cuda"):
+        self.device = torch.device(device)
+        if self.device.type != "cuda":
+            raise ValueError("HeavyCache lives in device memory (cuda)")
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise NotImplementedError(f"HeavyCache holds bf16 or f16, not {dtype}")
+        if head_dim not in (64, 128):
+            raise NotImplementedError(f"head_dim must be 64 or 128, got {head_dim}")
+        if batch < 1 or n_kv_heads < 1 or budget < 1:
+            raise ValueError("batch, n_kv_heads and budget must be positive")
+        if sinks < 0 or recent < 1 or sinks + recent > budget:
+            raise ValueError(f"sinks >= 0, recent >= 1 and sinks + recent <= budget, got {sinks}, {recent}, {budget}")
+        self.batch, self.n_kv_heads, self.head_dim, self.budget = batch, n_kv_heads, head_dim, budget
+        self.sinks, self.recent, self.dtype = sinks, recent, dtype
+        shape = (batch, n_kv_heads, budget)
+        self.k = torch.zeros(*shape, head_dim, dtype=dtype, device=self.device)
+        self.v = torch.zeros(*shape, head_dim, dtype=dtype, device=self.device)
+        self.mass = torch.zeros(shape, dtype=torch.float32, device=self.device)
+        self.pos = torch.zeros(shape, dtype=torch.int32, device=self.device)
+        self.seen = torch.zeros(batch, dtype=torch.int32, device=self.device)
+        self._ticket = torch.zeros(batch, dtype=torch.int32, device=self.device)
+        self.device = self.k.device
+        self._scores: Optional[torch.Tensor] = None  # attend()'s workspace, when it needs one
+        self._desc = L.Heavy(self.k.data_ptr(), self.v.data_ptr(), self.mass.data_ptr(), self.pos.data_ptr(),
+                             self.seen.data_ptr(), L.dtype_code(self.k), batch, n_kv_heads, budget, head_dim, sinks, recent)
+
+    def reset(self) -> None:
+        """Forget every token."""
+        self.seen.zero_()
+
+    def load(self, k: torch.Tensor, v: torch.Tensor, mass: torch.Tensor, cu: torch.Tensor,
+             rows: Optional[torch.Tensor] = None) -> None:
+        """Take packed prompts ``k, v (N, H_kv, D)`` with offsets ``cu (S + 1,)`` and masses
+        ``(H_kv, N)`` fp32: prompt ``s`` replaces row ``rows[s]`` (int32; default ``s``) of the
+        cache.  One of at most ``budget`` tokens is kept whole; of a longer one the sinks, the
+        recent tokens and those of most mass (lowest position on ties), by ascending position."""
+        dev = L.require_cuda(k, v, mass, cu, rows, self.k)
+        if k.dim() != 3 or k.shape[1:] != (self.n_kv_heads, self.head_dim) or v.shape != k.shape:
+            raise ValueError(f"k and v must be (N, {self.n_kv_heads}, {self.head_dim})")
+        if k.dtype != self.dtype or v.dtype != self.dtype:
+            raise ValueError(f"k and v must be {self.dtype} as the cache")
+        if mass.shape != (self.n_kv_heads, k.shape[0]) or mass.dtype != torch.float32:
+            raise ValueError("mass must be fp32 (H_kv, N)")
+        if cu.dtype != torch.int32 or cu.dim() != 1 or cu.numel() < 1 or not cu.is_contiguous():
+            raise ValueError("cu must be a contiguous int32 vector of sequence offsets (S + 1)")
+        s = cu.numel() - 1
+        if rows is not None and (rows.dtype != torch.int32 or rows.shape != (s,) or not rows.is_contiguous()):
+            raise ValueError("rows must be a contiguous int32 vector of one cache row per sequence")
+        k, v = _rows16(k), _rows16(v)
+        if mass.stride(1) != 1:
+            mass = mass.contiguous()
+        status = L.status_word(dev)
+        L.check(L.lib().linattn_heavy_load(
+            self._desc, k.data_ptr(), v.data_ptr(), L.strides2(k), L.strides2(v), k.shape[0], mass.data_ptr(),
+            mass.stride(0), cu.data_ptr(), L.ptr(rows), s, status.data_ptr(), L.stream_of(self.k)))
+        if L.strict():
+            L.check_status(dev)
+
+    def append(self, k: torch.Tensor, v: torch.Tensor) -> None:
+        """Take ``(B, H_kv, T_new, D)`` keys / values, one token after the other: each fills the
+        next empty slot or, in a full cache, replaces the slot of least mass (lowest slot on
+        ties) outside the sinks and the last ``recent`` tokens (itself among them)."""
+        shape = k.shape
+        if len(shape) != 4 or shape[0] != self.batch or shape[1] != self.n_kv_heads or shape[3] != self.head_dim or v.shape != shape:
+            raise ValueError(f"k and v must be ({self.batch}, {self.n_kv_heads}, T_new, {self.head_dim})")
+        if k.dtype != self.dtype or v.dtype != self.dtype:
+            raise ValueError(f"k and v must be {self.dtype} as the cache")
+        dev = L.require_cuda(k, v, self.k)
+        k, v = _rows16(k), _rows16(v)
+        status = L.status_word(dev)
+        L.check(L.lib().linattn_heavy_append(self._desc, k.data_ptr(), v.data_ptr(), L.strides3(k), L.strides3(v), shape[2],
+                                             self._ticket.data_ptr(), status.data_ptr(), L.stream_of(self.k)))
+        if L.strict():
+            L.check_status(dev)
+
+    def attend(self, q: torch.Tensor, *, scale: Optional[float] = None, accumulate: bool = True,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """``o (B, H_q, 1, D)`` of one query token per sequence over the slots in use; with
+        ``accumulate`` each slot's mass grows by its weights, summed over its group's heads."""
+        shape = q.shape
+        if len(shape) != 4 or shape[0] != self.batch or shape[1] % self.n_kv_heads or shape[1] < 1 or shape[2] != 1 or shape[3] != self.head_dim:
+            raise ValueError(f"q must be ({self.batch}, a multiple of {self.n_kv_heads}, 1, {self.head_dim}), got {tuple(shape)}")
+        if q.dtype != self.dtype:
+            raise ValueError(f"q must be {self.dtype} as the cache")
+        dev = L.require_cuda(q, self.k, out)
+        q = _rows16(q)
+        if out is None:
+            out = torch.empty(shape, dtype=q.dtype, device=dev)
+        elif out.shape != shape or out.dtype != q.dtype or out.stride(3) != 1:
+            raise ValueError("out must have q's shape and dtype with contiguous channels")
+        lib = L.lib()
+        need = lib.linattn_heavy_attend_workspace(self.batch, shape[1], self.n_kv_heads, self.budget) if accumulate else 0
+        if need and (self._scores is None or self._scores.numel() < need):
+            self._scores = torch.empty(need, dtype=torch.uint8, device=dev)
+        sq, so = q.stride(), out.stride()
+        L.check(lib.linattn_heavy_attend(
+            self._desc, q.data_ptr(), shape[1], (L.c_i64 * 2)(sq[0], sq[1]),
+            1.0 / math.sqrt(self.head_dim) if scale is None else float(scale), int(accumulate), out.data_ptr(),
+            (L.c_i64 * 2)(so[0], so[1]), L.ptr(self._scores) if need else None, need, L.stream_of(self.k)))
+        return out
+
+    def step(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: Optional[float] = None,
+             out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """One decode step: :meth:`append` the new token, then :meth:`attend` with its query."""
+        self.append(k, v)
+        return self.attend(q, scale=scale, out=out)
+
+
+def _rows16(x: torch.Tensor) -> torch.Tensor:
+    """x with contiguous channels and rows on 16 bytes."""
+    st = x.stride()
+    if st[-1] != 1 or x.data_ptr() & 15 or any(s & 7 for s in st[:-1]):
+        x = x.contiguous()
+    return x
