@@ -10,6 +10,7 @@ to ``NotImplementedError`` and CUDA failures to ``RuntimeError``.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import threading
 from pathlib import Path
@@ -213,12 +214,23 @@ def strides4(t: torch.Tensor):
     return (c_i64 * 4)(*t.stride())
 
 
+@functools.lru_cache(maxsize=4096)
+def i64_array(values: tuple):
+    """A constant ``int64_t[]`` argument (the library only reads it)."""
+    return (c_i64 * len(values))(*values)
+
+
 def strides3(t: torch.Tensor):
-    return (c_i64 * 3)(*t.stride()[:3])
+    return i64_array(t.stride()[:3])
 
 
 def strides2(t: torch.Tensor):
-    return (c_i64 * 2)(*t.stride()[:2])
+    return i64_array(t.stride()[:2])
+
+
+def raw_stream(device_index: int) -> int:
+    """The current stream of a device as the library takes it (no Stream object)."""
+    return torch._C._cuda_getCurrentRawStream(device_index)
 
 
 def stream_of(t: torch.Tensor) -> int:

@@ -281,7 +281,8 @@ int mass_fail(int code, const char* what) {
 template <typename T, int D>
 cudaError_t launch_mass(const MassArgs& p, const CUtensorMap& q, const CUtensorMap& k, dim3 grid, cudaStream_t st) {
   auto kern = attention_mass_kernel<T, D>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, MassSmem<D>::BYTES);
+  static int allowed[64] = {};
+  const cudaError_t e = allow_smem(kern, MassSmem<D>::BYTES, allowed);
   if (e != cudaSuccess) return e;
   kern<<<grid, MT_THREADS, MassSmem<D>::BYTES, st>>>(p, q, k);
   return cudaGetLastError();

@@ -317,7 +317,8 @@ AttendPlan attend_plan(int64_t units, int64_t G, int64_t M, int D) {
 template <typename T, int D, int NT>
 cudaError_t launch_attend(const HeavyAttendArgs& a, const AttendPlan& p, int64_t units, cudaStream_t st) {
   auto kern = heavy_attend_kernel<T, D, NT>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem);
+  static int allowed[64] = {};
+  cudaError_t e = allow_smem(kern, p.smem, allowed);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];

@@ -120,14 +120,22 @@ __global__ void __launch_bounds__(APPEND_THREADS) heavy_append_kernel(const Heav
 // ---------------------------------------------------------------------------------
 // load
 // ---------------------------------------------------------------------------------
-// Selection: a cluster per (sequence, kv head), each CTA a contiguous part of the prompt.
-// The R-th largest mass of the candidates is found digit by digit (11 + 11 + 10 bits) from
-// histograms in shared memory that the CTAs read from one another; then every CTA knows how
-// many kept tokens lie before its part and writes the positions and masses of its own in
-// order.  The rows are moved by a second kernel, spread evenly over the GPU: what is kept
-// is not spread evenly over the prompt (`recent` tokens all lie at its end).
+// Selection: a cluster per (sequence, kv head), each CTA a contiguous part of the prompt, each
+// thread 16 tokens next to one another, whose keys stay in registers (parts of more than
+// 8192 tokens are read again for every pass).  The R-th largest mass of the candidates is found
+// digit by digit (11 + 11 + 10 bits: the first digit of positive floats is spread over enough
+// bins that the shared-memory atomics rarely meet).  The CTAs read one another's histograms
+// over distributed shared memory in two steps, the sums of 64 groups of bins and then the 32
+// bins of the group that holds the R-th: one remote load a thread and step, where reading
+// all 2048 bins of 8 CTAs took most of the time (16 ragged prompts, 8 heads: 247 us).  Then every
+// CTA knows how many kept tokens lie before its part and writes the positions and masses of
+// its own in order.  The rows are moved by a second kernel, spread evenly over the GPU: what is
+// kept is not spread evenly over the prompt (`recent` tokens all lie at its end).
 constexpr int SEL_THREADS = 512;
+constexpr int SEL_PER = 16;                        // tokens of a thread in one round
+constexpr int SEL_ROUND = SEL_THREADS * SEL_PER;   // tokens of a CTA in one round
 constexpr int SEL_BINS = 2048;
+constexpr int SEL_GROUPS = 64;                     // groups of 32 bins
 
 struct HeavyLoadArgs {
   const float* mass;   // (H, N)
@@ -146,13 +154,27 @@ __device__ __forceinline__ bool sequence_range(const int32_t* cu, int s, int64_t
   return a == lo && b == hi;
 }
 
+// Inclusive sums over a warp from the highest lane down.
+__device__ __forceinline__ uint32_t sum_from_above(uint32_t x) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t y = __shfl_down_sync(0xffffffffu, x, o);
+    if (lane + o < 32) x += y;
+  }
+  return x;
+}
+
 __global__ void __launch_bounds__(SEL_THREADS) heavy_select_kernel(const HeavyCacheArgs c, const HeavyLoadArgs a) {
   cg::cluster_group cluster = cg::this_cluster();
-  __shared__ uint32_t hist[SEL_BINS];
+  __shared__ __align__(16) uint32_t hist[SEL_BINS];
+  __shared__ uint32_t groups[SEL_GROUPS];   // sums of this CTA's bins
+  __shared__ uint32_t totals[SEL_GROUPS];   // of all CTAs: groups, then the bins of one group
   __shared__ uint32_t scan[SEL_THREADS / 32 + 1];
-  __shared__ uint32_t picked[2];      // the digit that holds the R-th largest, and how many lie above it
-  __shared__ uint32_t above[2];       // this CTA's candidates over the threshold / equal to it
-  const int tid = threadIdx.x, cl = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  __shared__ uint32_t picked[2];            // group or bin that holds the R-th largest, how many lie above it
+  __shared__ uint32_t above[2];             // this CTA's candidates over the threshold / equal to it
+  const int tid = threadIdx.x, lane = tid & 31, cl = static_cast<int>(cluster.num_blocks()),
+            rank = static_cast<int>(cluster.block_rank());
   const int unit_in = blockIdx.x / cl;
   const int h = unit_in % c.H, s = unit_in / c.H;
   int64_t first;
@@ -180,7 +202,19 @@ __global__ void __launch_bounds__(SEL_THREADS) heavy_select_kernel(const HeavyCa
   const int c_lo = c.sinks, c_hi = n - c.recent;  // candidates [c_lo, c_hi): c_hi - c_lo > M - sinks - recent
   const int want = c.M - c.sinks - c.recent;
   uint32_t prefix = 0, left = static_cast<uint32_t>(want);
-  const int a_lo = max(lo, c_lo), a_hi = min(hi, c_hi);
+  // the masses of this thread's tokens of one round: with a few tokens to a thread they sit
+  // close together, so that every thread has some
+  const int rounds = (part + SEL_ROUND - 1) / SEL_ROUND;
+  const int per = rounds <= 1 ? (part + SEL_THREADS - 1) / SEL_THREADS : SEL_PER;
+  float m[SEL_PER];
+  int base = 0;
+  auto fetch = [&](int r) {
+    base = lo + r * SEL_ROUND + tid * per;
+#pragma unroll
+    for (int e = 0; e < SEL_PER; ++e) m[e] = e < per && base + e < hi ? __ldg(mass + base + e) : 0.f;
+  };
+  auto candidate = [&](int e) { return e < per && base + e < hi && base + e >= c_lo && base + e < c_hi; };
+  if (rounds == 1) fetch(0);
   if (want > 0) {
 #pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
@@ -188,30 +222,63 @@ __global__ void __launch_bounds__(SEL_THREADS) heavy_select_kernel(const HeavyCa
       const uint32_t digits = pass == 2 ? 1023u : 2047u;
       for (int i = tid; i < SEL_BINS; i += SEL_THREADS) hist[i] = 0;
       __syncthreads();
-      for (int i = a_lo + tid; i < a_hi; i += SEL_THREADS) {
-        const uint32_t key = mass_key(mass[i]);
-        if (pass == 0 || (key >> (pass == 1 ? 21 : 10)) == prefix) atomicAdd(&hist[(key >> shift) & digits], 1u);
+      for (int r = 0; r < rounds; ++r) {
+        if (rounds > 1) fetch(r);
+#pragma unroll
+        for (int e = 0; e < SEL_PER; ++e) {
+          const uint32_t key = mass_key(m[e]);
+          if (candidate(e) && (pass == 0 || (key >> (pass == 1 ? 21 : 10)) == prefix))
+            atomicAdd(&hist[(key >> shift) & digits], 1u);
+        }
+      }
+      __syncthreads();
+      {  // 8 threads a group, 4 bins a thread
+        const uint4 x = reinterpret_cast<const uint4*>(hist)[tid];
+        uint32_t t = x.x + x.y + x.z + x.w;
+        t += __shfl_xor_sync(0xffffffffu, t, 1);
+        t += __shfl_xor_sync(0xffffffffu, t, 2);
+        t += __shfl_xor_sync(0xffffffffu, t, 4);
+        if ((tid & 7) == 0) groups[tid >> 3] = t;
       }
       cluster.sync();
-      // bins of this thread, from the largest down: 4 each, summed over the CTAs
-      uint32_t cnt[SEL_BINS / SEL_THREADS], sum = 0;
-#pragma unroll
-      for (int e = 0; e < SEL_BINS / SEL_THREADS; ++e) {
-        const int bin = SEL_BINS - 1 - (tid * (SEL_BINS / SEL_THREADS) + e);
-        cnt[e] = 0;
-        for (int r = 0; r < cl; ++r) cnt[e] += cluster.map_shared_rank(hist, r)[bin];
-        sum += cnt[e];
+      {  // thread (group, CTA)
+        uint32_t t = (tid & 7) < cl ? cluster.map_shared_rank(groups, tid & 7)[tid >> 3] : 0u;
+        t += __shfl_xor_sync(0xffffffffu, t, 1);
+        t += __shfl_xor_sync(0xffffffffu, t, 2);
+        t += __shfl_xor_sync(0xffffffffu, t, 4);
+        if ((tid & 7) == 0) totals[tid >> 3] = t;
       }
-      uint32_t before = block_exclusive_scan<SEL_THREADS>(sum, scan, nullptr);
-#pragma unroll
-      for (int e = 0; e < SEL_BINS / SEL_THREADS; ++e) {
-        if (before < left && left <= before + cnt[e]) {
-          picked[0] = static_cast<uint32_t>(SEL_BINS - 1 - (tid * (SEL_BINS / SEL_THREADS) + e));
-          picked[1] = before;
+      __syncthreads();
+      if (tid < 32) {  // two groups a lane
+        const uint32_t t0 = totals[2 * lane], t1 = totals[2 * lane + 1];
+        const uint32_t over = sum_from_above(t0 + t1) - t0 - t1;
+        if (over < left && left <= over + t1) {
+          picked[0] = 2 * lane + 1;
+          picked[1] = over;
+        } else if (over + t1 < left && left <= over + t1 + t0) {
+          picked[0] = 2 * lane;
+          picked[1] = over + t1;
         }
-        before += cnt[e];
       }
-      cluster.sync();  // every CTA has read the histograms; picked[] is there
+      __syncthreads();
+      const uint32_t group = picked[0];
+      left -= picked[1];
+      if (tid < 256) {  // thread (bin of the group, CTA)
+        uint32_t t = (tid & 7) < cl ? cluster.map_shared_rank(hist, tid & 7)[group * 32 + (tid >> 3)] : 0u;
+        t += __shfl_xor_sync(0xffffffffu, t, 1);
+        t += __shfl_xor_sync(0xffffffffu, t, 2);
+        t += __shfl_xor_sync(0xffffffffu, t, 4);
+        if ((tid & 7) == 0) totals[tid >> 3] = t;
+      }
+      __syncthreads();
+      if (tid < 32) {
+        const uint32_t t = totals[lane], over = sum_from_above(t) - t;
+        if (over < left && left <= over + t) {
+          picked[0] = group * 32 + lane;
+          picked[1] = over;
+        }
+      }
+      cluster.sync();  // picked[] is there, and every CTA has read the histograms
       prefix = pass == 0 ? picked[0] : (prefix << (pass == 1 ? 11 : 10)) | picked[0];
       left -= picked[1];
     }
@@ -222,17 +289,21 @@ __global__ void __launch_bounds__(SEL_THREADS) heavy_select_kernel(const HeavyCa
   __syncthreads();
   if (want > 0) {
     uint32_t gt = 0, eq = 0;
-    for (int i = a_lo + tid; i < a_hi; i += SEL_THREADS) {
-      const uint32_t key = mass_key(mass[i]);
-      gt += key > thr;
-      eq += key == thr;
+    for (int r = 0; r < rounds; ++r) {
+      if (rounds > 1) fetch(r);
+#pragma unroll
+      for (int e = 0; e < SEL_PER; ++e) {
+        const uint32_t key = mass_key(m[e]);
+        gt += candidate(e) && key > thr;
+        eq += candidate(e) && key == thr;
+      }
     }
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) {
       gt += __shfl_xor_sync(0xffffffffu, gt, o);
       eq += __shfl_xor_sync(0xffffffffu, eq, o);
     }
-    if ((tid & 31) == 0) {
+    if (lane == 0) {
       atomicAdd(&above[0], gt);
       atomicAdd(&above[1], eq);
     }
@@ -246,32 +317,35 @@ __global__ void __launch_bounds__(SEL_THREADS) heavy_select_kernel(const HeavyCa
   }
   // kept tokens before this part: sinks, candidates, and those `recent` ones that lie before it
   uint32_t at = static_cast<uint32_t>(min(lo, c_lo)) + gt_before + min(eq_before, ties) +
-                static_cast<uint32_t>(max(0, lo - max(c_hi, 0)));
+                static_cast<uint32_t>(max(0, lo - c_hi));
   uint32_t eq_at = eq_before;
-  for (int i0 = lo; i0 < hi; i0 += SEL_THREADS) {
-    const int i = i0 + tid;
-    float m = 0.f;
-    uint32_t keep = 0, eq = 0;
-    if (i < hi) {
-      m = mass[i];
-      if (i < c_lo || i >= c_hi) {
-        keep = 1;
-      } else if (want > 0) {
-        const uint32_t key = mass_key(m);
-        keep = key > thr;
-        eq = key == thr;
-      }
+  for (int r = 0; r < rounds; ++r) {
+    if (rounds > 1) fetch(r);
+    uint32_t keep = 0, eq = 0;  // one bit a token
+#pragma unroll
+    for (int e = 0; e < SEL_PER; ++e) {
+      const int i = base + e;
+      const uint32_t key = mass_key(m[e]);
+      const bool in = e < per && i < hi, cand = candidate(e) && want > 0;
+      keep |= static_cast<uint32_t>(in && (i < c_lo || i >= c_hi || (cand && key > thr))) << e;
+      eq |= static_cast<uint32_t>(cand && key == thr) << e;
     }
-    // ties before this thread decide whether its own stays; one scan carries both counts
+    // the ties before a token decide whether it stays; one scan carries both counts
     uint32_t total;
-    uint32_t x = block_exclusive_scan<SEL_THREADS>(keep | (eq << 16), scan, &total);
-    const uint32_t eq_here = eq_at + (x >> 16);
-    const uint32_t slot = at + (x & 0xffffu) + (min(eq_here, ties) - min(eq_at, ties));
-    if (keep || (eq && eq_here < ties)) {
-      if (slot < static_cast<uint32_t>(c.M)) {
-        out_mass[slot] = m;
-        out_pos[slot] = i;
+    const uint32_t x = block_exclusive_scan<SEL_THREADS>(__popc(keep) | (__popc(eq) << 16), scan, &total);
+    uint32_t eq_here = eq_at + (x >> 16);
+    uint32_t slot = at + (x & 0xffffu) + (min(eq_here, ties) - min(eq_at, ties));
+#pragma unroll
+    for (int e = 0; e < SEL_PER; ++e) {
+      const bool tie = (eq >> e) & 1u;
+      if (((keep >> e) & 1u) || (tie && eq_here < ties)) {
+        if (slot < static_cast<uint32_t>(c.M)) {
+          out_mass[slot] = m[e];
+          out_pos[slot] = base + e;
+        }
+        ++slot;
       }
+      eq_here += tie;
     }
     at += (total & 0xffffu) + (min(eq_at + (total >> 16), ties) - min(eq_at, ties));
     eq_at += total >> 16;
@@ -417,7 +491,11 @@ extern "C" int linattn_heavy_load(const linattn_heavy_t* cache, const void* k, c
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
-  const unsigned cl = 8;
+  // CTAs for the whole GPU where the units alone are too few, each with 1024 tokens or more
+  // (the longest a sequence can be is all of them)
+  const int64_t units = S * c.H;
+  unsigned cl = 1;
+  while (cl < 8 && units * cl < sm_count() && N / S > 1024 * static_cast<int64_t>(cl)) cl *= 2;
   cfg.gridDim = dim3(static_cast<unsigned>(S) * c.H * cl);
   cfg.blockDim = dim3(SEL_THREADS);
   cfg.stream = st;

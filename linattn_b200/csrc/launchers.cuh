@@ -25,6 +25,16 @@ struct TopkParams {
 };
 
 int device_index();
+// Allow `kern` its dynamic shared memory once per device (`allowed`: a static array of the
+// caller, one per kernel); later calls cost a look at it.
+template <typename K>
+cudaError_t allow_smem(K kern, int bytes, int (&allowed)[64]) {
+  const int d = device_index();
+  if (d >= 0 && d < 64 && allowed[d] >= bytes) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && d >= 0 && d < 64) allowed[d] = bytes;
+  return e;
+}
 // Record `msg` as linattn_last_error() and return `code` (host side).
 int set_error(int code, const char* msg);
 

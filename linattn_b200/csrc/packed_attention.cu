@@ -424,7 +424,8 @@ template <typename T, int D>
 cudaError_t launch_packed(const PackedArgs& p, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, dim3 grid,
                           cudaStream_t st) {
   auto kern = packed_attention_kernel<T, D>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PackedSmem<D>::BYTES);
+  static int allowed[64] = {};
+  const cudaError_t e = allow_smem(kern, PackedSmem<D>::BYTES, allowed);
   if (e != cudaSuccess) return e;
   kern<<<grid, PA_THREADS, PackedSmem<D>::BYTES, st>>>(p, q, k, v);
   return cudaGetLastError();

@@ -18,6 +18,8 @@ order of its keys), ``pos`` says which token a slot holds.
 
 from __future__ import annotations
 
+import ctypes
+import functools
 import math
 from typing import Optional
 
@@ -61,6 +63,10 @@ class HeavyCache:
         self._scores: Optional[torch.Tensor] = None  # attend()'s workspace, when it needs one
         self._desc = L.Heavy(self.k.data_ptr(), self.v.data_ptr(), self.mass.data_ptr(), self.pos.data_ptr(),
                              self.seen.data_ptr(), L.dtype_code(self.k), batch, n_kv_heads, budget, head_dim, sinks, recent)
+        # what every call passes
+        self._lib, self._ref, self._ticket_ptr = L.lib(), ctypes.byref(self._desc), self._ticket.data_ptr()
+        self._status_ptr = L.status_word(self.device).data_ptr()
+        self._scale = 1.0 / math.sqrt(head_dim)
 
     def reset(self) -> None:
         """Forget every token."""
@@ -87,10 +93,9 @@ class HeavyCache:
         k, v = _rows16(k), _rows16(v)
         if mass.stride(1) != 1:
             mass = mass.contiguous()
-        status = L.status_word(dev)
-        L.check(L.lib().linattn_heavy_load(
-            self._desc, k.data_ptr(), v.data_ptr(), L.strides2(k), L.strides2(v), k.shape[0], mass.data_ptr(),
-            mass.stride(0), cu.data_ptr(), L.ptr(rows), s, status.data_ptr(), L.stream_of(self.k)))
+        L.check(self._lib.linattn_heavy_load(
+            self._ref, k.data_ptr(), v.data_ptr(), L.strides2(k), L.strides2(v), k.shape[0], mass.data_ptr(),
+            mass.stride(0), cu.data_ptr(), L.ptr(rows), s, self._status_ptr, L.raw_stream(dev.index)))
         if L.strict():
             L.check_status(dev)
 
@@ -105,9 +110,9 @@ class HeavyCache:
             raise ValueError(f"k and v must be {self.dtype} as the cache")
         dev = L.require_cuda(k, v, self.k)
         k, v = _rows16(k), _rows16(v)
-        status = L.status_word(dev)
-        L.check(L.lib().linattn_heavy_append(self._desc, k.data_ptr(), v.data_ptr(), L.strides3(k), L.strides3(v), shape[2],
-                                             self._ticket.data_ptr(), status.data_ptr(), L.stream_of(self.k)))
+        L.check(self._lib.linattn_heavy_append(
+            self._ref, k.data_ptr(), v.data_ptr(), L.strides3(k), L.strides3(v), shape[2], self._ticket_ptr, self._status_ptr,
+            L.raw_stream(dev.index)))
         if L.strict():
             L.check_status(dev)
 
@@ -126,15 +131,12 @@ class HeavyCache:
             out = torch.empty(shape, dtype=q.dtype, device=dev)
         elif out.shape != shape or out.dtype != q.dtype or out.stride(3) != 1:
             raise ValueError("out must have q's shape and dtype with contiguous channels")
-        lib = L.lib()
-        need = lib.linattn_heavy_attend_workspace(self.batch, shape[1], self.n_kv_heads, self.budget) if accumulate else 0
+        need = _attend_bytes(self.batch, shape[1], self.n_kv_heads, self.budget) if accumulate else 0
         if need and (self._scores is None or self._scores.numel() < need):
             self._scores = torch.empty(need, dtype=torch.uint8, device=dev)
-        sq, so = q.stride(), out.stride()
-        L.check(lib.linattn_heavy_attend(
-            self._desc, q.data_ptr(), shape[1], (L.c_i64 * 2)(sq[0], sq[1]),
-            1.0 / math.sqrt(self.head_dim) if scale is None else float(scale), int(accumulate), out.data_ptr(),
-            (L.c_i64 * 2)(so[0], so[1]), L.ptr(self._scores) if need else None, need, L.stream_of(self.k)))
+        L.check(self._lib.linattn_heavy_attend(
+            self._ref, q.data_ptr(), shape[1], L.strides2(q), self._scale if scale is None else float(scale), int(accumulate),
+            out.data_ptr(), L.strides2(out), self._scores.data_ptr() if need else None, need, L.raw_stream(dev.index)))
         return out
 
     def step(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: Optional[float] = None,
@@ -144,9 +146,15 @@ class HeavyCache:
         return self.attend(q, scale=scale, out=out)
 
 
+@functools.lru_cache(maxsize=1024)
+def _attend_bytes(batch: int, hq: int, hkv: int, budget: int) -> int:
+    return L.lib().linattn_heavy_attend_workspace(batch, hq, hkv, budget)
+
+
 def _rows16(x: torch.Tensor) -> torch.Tensor:
     """x with contiguous channels and rows on 16 bytes."""
-    st = x.stride()
-    if st[-1] != 1 or x.data_ptr() & 15 or any(s & 7 for s in st[:-1]):
-        x = x.contiguous()
-    return x
+    *outer, last = x.stride()
+    bits = x.data_ptr() >> 1
+    for s in outer:
+        bits |= s
+    return x.contiguous() if last != 1 or bits & 7 else x
