@@ -612,11 +612,12 @@ int linattn_heavy_append(const linattn_heavy_t* cache, const void* k_new, const 
  * accumulate != 0 each slot's mass grows by its weights summed over the group's query
  * heads.  q, out (batch, H_q, head_dim) in the cache's dtype, strides {sequence, head} in
  * elements.  f16 / bf16, head_dim 64 or 128.  A sequence without slots gets o = 0.
- * workspace: linattn_heavy_attend_workspace bytes (0 for most sizes), 16-byte aligned.
+ * ticket: batch * n_kv_heads int32 of scratch that holds zeros before and after every
+ * call.  workspace: linattn_heavy_attend_workspace bytes, 16-byte aligned.
  */
 int linattn_heavy_attend(const linattn_heavy_t* cache, const void* q, int64_t Hq, const int64_t* q_strides /*[2]*/,
                          float scale, int32_t accumulate, void* out, const int64_t* out_strides /*[2]*/,
-                         void* workspace, int64_t workspace_bytes, void* stream);
+                         int32_t* ticket, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
 int64_t linattn_heavy_attend_workspace(int64_t batch, int64_t Hq, int64_t Hkv, int64_t budget);
 
 

@@ -161,7 +161,7 @@ def _declare(lib: ctypes.CDLL) -> None:
                                        c_vp, c_vp]
     lib.linattn_heavy_append.argtypes = [P(Heavy), c_vp, c_vp, P(c_i64), P(c_i64), c_i64, c_vp, c_vp, c_vp]
     lib.linattn_heavy_attend.argtypes = [P(Heavy), c_vp, c_i64, P(c_i64), ctypes.c_float, c_i32, c_vp, P(c_i64), c_vp,
-                                         c_i64, c_vp]
+                                         c_vp, c_i64, c_vp, c_vp]
     lib.linattn_heavy_attend_workspace.argtypes = [c_i64] * 4
     lib.linattn_heavy_attend_workspace.restype = c_i64
     for name in ("linattn_packed_attention", "linattn_attention_mass", "linattn_heavy_load", "linattn_heavy_append",

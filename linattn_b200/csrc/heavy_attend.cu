@@ -3,19 +3,22 @@
 //
 //   o = sum_n p_n v_n,  p_n = exp(c q . k_n - lse),  mass_n += sum over the group's heads of p_n
 //
-// HBM-bound: K and V are read once (2 D elements a slot), everything else is small.  A
-// (sequence, kv head) is a cluster of CTAs that cut its slots; a warp takes 16 slots at a
-// time straight from global memory into mma.sync fragments: the contraction index of
-// S^T = K Q^T is permuted the same way in K and q, so that a lane's fragments are 16-byte
-// pieces of a row, and for O^T = V^T P^T the output channels are permuted instead, with
-// pairs of slots joined by byte permutes.  No shared-memory stage, no barrier in the loop.
-// The final weights need the whole row's lse, so the scores stay in shared memory (in the
-// workspace when a part of the slots is too long for that) until the cluster has merged its
-// (o, m, l) over distributed shared memory; every CTA then updates the masses of its own
-// slots.  One launch, no atomics: the sums have a fixed order.
-// P is split into hi + lo 16-bit parts (to ~2^-16), so o carries its own rounding only.
-#include <cooperative_groups.h>
-
+// HBM-bound: K and V are read once (2 D elements a slot), everything else is small.  One CTA to
+// an SM stays for the whole call and takes an equal share of all 128-slot tiles of all
+// (sequence, kv head) units, in order, so that no SM idles at the end whatever the lengths
+// are; a producer warp keeps a ring of tiles (K and V, 128-byte-swizzled tensor-map boxes) full,
+// across units too, so that the memory never waits for a unit's epilogue.  Eight warps work on
+// a tile: for S^T = K Q^T (mma.sync, 8 heads as columns) a warp has 16 slots, the weights go
+// through shared memory, and for O^T = V^T P^T a warp has 16 channels and all 128 slots (D = 64:
+// half of them), so that o is not spread over warps; one barrier a tile.  P is split into
+// hi + lo 16-bit parts (to ~2^-16), so o carries its own rounding only.
+//
+// The masses need a unit's final lse: its scores go to the workspace (4 bytes a slot and head,
+// which L2 holds until they are read back), and four more warps add a finished unit's weights
+// while the others go on with the next one (done by the same warps it cost 59 of 205 us at 64
+// sequences x 8 heads x 4096 slots).  A unit that one CTA has whole is finished there; of one
+// that several CTAs share, the last to arrive merges their (o, m, l): the parts are added in
+// their order, whoever does it, so results do not depend on it.
 #include <cstdio>
 #include <type_traits>
 
@@ -23,265 +26,589 @@
 #include "sparse_attention_mma.cuh"
 #include "umma.cuh"
 
-namespace cg = cooperative_groups;
-
 namespace linattn {
 
 namespace {
 
 struct HeavyAttendArgs {
-  const uint4* k;
-  const uint4* v;
   float* mass;
   const int32_t* seen;
   const void* q;
   void* out;
   int64_t qb, qh, ob, oh;
-  int H, M, G;
+  int B, H, M, G;
+  int h0, heads;     // heads [h0, h0 + heads) of every group in this launch
   float scale_log2;
   int accumulate;
-  float* scores;     // workspace (B, H, 8 NT, M), or NULL: scores in shared memory
-  int part_max;      // slots of a CTA's part at most (a multiple of 16)
+  float* scores;     // (B * H, heads, M) log2-domain scores
+  float* part_o;     // (CTAs, 2, HN, D) unnormalised o of units that this CTA shares
+  float* part_ml;    // (CTAs, 2, 2, HN) their maxima and sums
+  int32_t* ticket;   // (B * H) zeros: arrivals at a shared unit
+  int32_t* status;
 };
 
-constexpr int ATT_WARPS = 8;
+constexpr int AT_WARPS = 8;                     // on tiles; then one that loads, and the mass warps
+constexpr int AT_MASS = 128;                    // threads that add the masses
+constexpr int AT_THREADS = 32 * (AT_WARPS + 1) + AT_MASS;
+constexpr int AT_ROWS = 128;                    // slots of a tile
+constexpr int AT_BOX = 128;                     // slots of one tensor-map box
+constexpr int AT_PROW = AT_ROWS * 2 + 16;       // bytes of a row of P: banks apart
+constexpr int AT_PARTS = 192;                   // CTAs that may share a unit: more than the GPU has SMs
 
-template <int NT>
-constexpr int attend_fixed_smem(int D) {  // floats: per-warp o, the CTA's o, (m, l) per warp and of the CTA
-  return ATT_WARPS * 8 * NT * D + 8 * NT * D + 2 * ATT_WARPS * 8 * NT + 2 * 8 * NT;
+template <int D, int NT>
+struct AttendSmem {
+  static constexpr int HN = 8 * NT;
+  static constexpr int HALF = AT_ROWS * 128;              // 64 channels of K or V
+  static constexpr int STAGE = 2 * (D / 64) * HALF;       // K then V
+  static constexpr int STAGES = D == 64 ? (NT == 4 ? 4 : 6) : NT == 4 ? 2 : 3;
+  static constexpr int P = 2 * 2 * HN * AT_PROW;          // [buffer][hi, lo][head][slot]
+  // merge of a shared unit: weights of its parts, sums of its thread groups
+  static constexpr int MERGE = (AT_PARTS * HN + (HN * D > 1024 ? HN * D : 1024)) * 4;
+  static constexpr int BYTES = 1024 + STAGES * STAGE + (P > MERGE ? P : MERGE);
+};
+
+// The units of one CTA's share of the tiles, in order.
+struct AttendWalk {
+  const int32_t* seen;
+  int B, H, M;
+  int b, h, count, tiles;  // the current unit
+  __device__ __forceinline__ void sequence(int at) {
+    b = at;
+    count = b < B ? min(max(seen[b], 0), M) : 0;
+    tiles = (count + AT_ROWS - 1) / AT_ROWS;
+  }
+  __device__ __forceinline__ void next() {
+    if (++h < H) return;
+    h = 0;
+    do sequence(b + 1);
+    while (b < B && tiles == 0);
+  }
+};
+
+__device__ __forceinline__ bool attend_barrier_or(bool x) {
+  int r = x ? 1 : 0;
+  asm volatile(
+      "{\n\t.reg .pred a, b;\n\tsetp.ne.s32 a, %0, 0;\n\t"
+      "barrier.cta.red.or.pred b, 1, 256, a;\n\tselp.s32 %0, 1, 0, b;\n\t}"
+      : "+r"(r)
+      :
+      : "memory");
+  return r != 0;
 }
+__device__ __forceinline__ void attend_barrier() { asm volatile("barrier.cta.sync 1, 256;" ::: "memory"); }
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(32 * ATT_WARPS, NT == 1 ? 2 : 1) heavy_attend_kernel(const HeavyAttendArgs a) {
+__global__ void __launch_bounds__(AT_THREADS, 1)
+    heavy_attend_kernel(const HeavyAttendArgs a, const __grid_constant__ CUtensorMap tmk,
+                        const __grid_constant__ CUtensorMap tmv) {
   using M = MmaOp<T>;
-  constexpr int PIECES = D / 8;        // 16-byte pieces of a row
-  constexpr int KJ = D / 32;           // pieces of a K row per lane
-  constexpr int VJ = D / 64;           // pieces of a V row per lane
-  constexpr int MT = D / 16;           // 16-channel tiles of O^T
-  constexpr int HN = 8 * NT;           // head columns
-  extern __shared__ __align__(16) float dsm[];
-  float* o_warp = dsm;                               // [ATT_WARPS][HN][D]
-  float* o_cta = o_warp + ATT_WARPS * HN * D;        // [HN][D]
-  float* ml_warp = o_cta + HN * D;                   // [2][ATT_WARPS][HN]
-  float* ml_cta = ml_warp + 2 * ATT_WARPS * HN;      // [2][HN]
-  float* sc_smem = ml_cta + 2 * HN;                  // [HN][part_max]
-  cg::cluster_group cluster = cg::this_cluster();
-  const int cl = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
-  const int unit = blockIdx.x / cl, h = unit % a.H, b = unit / a.H;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tig = lane & 3;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int count = min(a.seen[b], a.M);
-  const int part = ((count + 16 * cl - 1) / (16 * cl)) * 16;
-  const int lo = min(count, rank * part), hi = min(count, lo + part);
-  const uint4* kp = a.k + static_cast<int64_t>(unit) * a.M * PIECES;
-  const uint4* vp = a.v + static_cast<int64_t>(unit) * a.M * PIECES;
-  float* mass = a.mass + static_cast<int64_t>(unit) * a.M;
-  const int64_t sc_stride = a.scores ? a.M : a.part_max;
-  float* sc = a.scores ? a.scores + static_cast<int64_t>(unit) * HN * a.M + lo : sc_smem;
+  using SM = AttendSmem<D, NT>;
+  constexpr int HN = SM::HN, ST = SM::STAGES, HALVES = D / 64, CT = D / 16;
+  extern __shared__ __align__(128) uint8_t atsmem_raw[];
+  uint8_t* ring = atsmem_raw + ((1024 - (smem_u32(atsmem_raw) & 1023)) & 1023);
+  uint8_t* pbuf = ring + ST * SM::STAGE;
+  __shared__ __align__(8) uint64_t full[ST], empty[ST], job_full[2], job_empty[2];
+  __shared__ float mx_w[AT_WARPS][HN], l_w[AT_WARPS][HN];
+  // finished units on their way to the mass warps: maxima and reciprocal sums of the heads
+  __shared__ float fin[2][2][HN];
+  __shared__ int64_t job_unit[2];
+  __shared__ int job_count[2];  // slots in use, or -1: no more
+  __shared__ float upper[D == 64 ? 4 * 32 * 4 * NT : 1];  // D = 64: o of the tile's upper slots
+  __shared__ int dead, arrived;
+  __shared__ int64_t share[3];  // first tile, end, all tiles
+  __shared__ int start[2];      // first tile's sequence, and its tile among the sequence's
 
-  for (int h0 = 0; h0 < a.G; h0 += HN) {  // groups of more than HN heads: HN at a time
-    const int heads = min(HN, a.G - h0);
-    // q of head g: the same permuted channels as the K fragments
-    uint4 q[NT][KJ];
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int j = 0; j < KJ; ++j) {
-        const int head = t * 8 + g;
-        q[t][j] = make_uint4(0u, 0u, 0u, 0u);
-        if (head < heads)
-          q[t][j] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + b * a.qb +
-                                                    (static_cast<int64_t>(h) * a.G + h0 + head) * a.qh + (tig + 4 * j) * 8);
-      }
-    float acc[NT][MT][4], m[NT][2], l[NT][2];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-#pragma unroll
-      for (int e = 0; e < MT; ++e)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[t][e][i] = 0.f;
-      m[t][0] = m[t][1] = -INFINITY;
-      l[t][0] = l[t][1] = 0.f;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], AT_WARPS);
     }
-    uint4 kf[KJ][2], vf[VJ][4];
-    auto load_k = [&](int base) {
-      const int r0 = min(base + g, hi - 1), r1 = min(base + g + 8, hi - 1);
-#pragma unroll
-      for (int j = 0; j < KJ; ++j) {
-        kf[j][0] = __ldg(kp + static_cast<int64_t>(r0) * PIECES + tig + 4 * j);
-        kf[j][1] = __ldg(kp + static_cast<int64_t>(r1) * PIECES + tig + 4 * j);
-      }
-    };
-    auto load_v = [&](int base) {
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int r = min(base + 2 * tig + (x & 1) + 8 * (x >> 1), hi - 1);
-#pragma unroll
-        for (int j = 0; j < VJ; ++j) vf[j][x] = __ldg(vp + static_cast<int64_t>(r) * PIECES + g + 8 * j);
-      }
-    };
-    int base = lo + 16 * warp;
-    if (base < hi) {
-      load_k(base);
-      load_v(base);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&job_full[s], 1);
+      mbar_init(&job_empty[s], AT_MASS);
     }
-    for (; base < hi; base += 16 * ATT_WARPS) {
-      const int next = base + 16 * ATT_WARPS;
-      float s[NT][4];
+    dead = 0;
+    mbar_fence_init();
+  }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // this CTA's share of the tiles
+  if (warp == 0) {
+    auto tiles_of = [&](int b) {
+      return b < a.B ? static_cast<int64_t>((min(max(a.seen[b], 0), a.M) + AT_ROWS - 1) / AT_ROWS) * a.H : int64_t(0);
+    };
+    const int64_t early = tiles_of(lane);  // of the first 32 sequences
+    int64_t all = early;
+    for (int b = lane + 32; b < a.B; b += 32) all += tiles_of(b);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+    for (int o = 16; o >= 1; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+    const int64_t ctas = lmin(gridDim.x, all), c = blockIdx.x;
+    const int64_t lo = c < ctas ? c * all / ctas : 0, hi = c < ctas ? (c + 1) * all / ctas : 0;
+    if (lane == 0) {
+      share[0] = lo;
+      share[1] = hi;
+      share[2] = all;
+    }
+    if (hi > lo) {
+      int64_t base = 0;
+      for (int b0 = 0; b0 < a.B && base <= lo; b0 += 32) {
+        const int64_t mine = b0 == 0 ? early : tiles_of(b0 + lane);
+        int64_t incl = mine;
 #pragma unroll
-      for (int j = 0; j < KJ; ++j) {
-        const uint32_t f0[4] = {kf[j][0].x, kf[j][1].x, kf[j][0].y, kf[j][1].y};
-        const uint32_t f1[4] = {kf[j][0].z, kf[j][1].z, kf[j][0].w, kf[j][1].w};
+        for (int o = 1; o < 32; o <<= 1) {
+          const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += y;
+        }
+        if (lo >= base + incl - mine && lo < base + incl) {
+          start[0] = b0 + lane;
+          start[1] = static_cast<int>(lo - (base + incl - mine));
+        }
+        base += __shfl_sync(0xffffffffu, incl, 31);
+      }
+    }
+  }
+  __syncthreads();
+  const int64_t t0 = share[0], t1 = share[1], total = share[2];
+  const int64_t nc = lmin(gridDim.x, total);
+  // sequences without slots: o = 0
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x)
+    if (a.seen[b] <= 0)
+      for (int i = tid; i < a.H * a.heads * D; i += AT_THREADS) {
+        const int head = i / D;
+        static_cast<T*>(a.out)[b * a.ob + (static_cast<int64_t>(head / a.heads) * a.G + a.h0 + head % a.heads) * a.oh + i % D] = T(0.f);
+      }
+  if (t1 <= t0) return;
+  AttendWalk w{a.seen, a.B, a.H, a.M};
+  w.sequence(start[0]);
+  w.h = start[1] / w.tiles;
+  int first = start[1] % w.tiles;  // of this CTA in its first unit
+
+  if (warp == AT_WARPS) {
+    if (lane == 0) {
+      int j = 0;
+      int64_t t = t0;
+      bool ok = true;
+      while (ok && t < t1) {
+        const int end = static_cast<int>(lmin(w.tiles, first + (t1 - t)));
+        const int64_t row0 = (static_cast<int64_t>(w.b) * a.H + w.h) * a.M;
+        for (int i = first; ok && i < end; ++i, ++j) {
+          const int st = j % ST;
+          if (j >= ST) ok = mbar_wait_bounded(&empty[st], static_cast<uint32_t>((j / ST - 1) & 1));
+          if (!ok || dead) {
+            ok = false;
+            break;
+          }
+          uint8_t* dst = ring + st * SM::STAGE;
+          const int boxes = (min(AT_ROWS, w.count - i * AT_ROWS) + AT_BOX - 1) / AT_BOX;
+          const int y = static_cast<int>(row0 + static_cast<int64_t>(i) * AT_ROWS);
+          mbar_arrive_expect_tx(&full[st], static_cast<uint32_t>(boxes) * 2 * HALVES * AT_BOX * 128);
+          for (int x = 0; x < boxes; ++x)
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          M::mma(s[t], f0, q[t][j].x, q[t][j].y);
-          M::mma(s[t], f1, q[t][j].z, q[t][j].w);
+            for (int c = 0; c < HALVES; ++c)
+              tma_load_3d(dst + c * SM::HALF + x * AT_BOX * 128, &tmk, 64 * c, y + x * AT_BOX, 0, &full[st]);
+          for (int x = 0; x < boxes; ++x)
+#pragma unroll
+            for (int c = 0; c < HALVES; ++c)
+              tma_load_3d(dst + (HALVES + c) * SM::HALF + x * AT_BOX * 128, &tmv, 64 * c, y + x * AT_BOX, 0, &full[st]);
+        }
+        t += end - first;
+        first = 0;
+        w.next();
+      }
+      if (!ok) {
+        report(a.status, LINATTN_DEV_TIMEOUT);
+        dead = 1;
+      }
+      // the copies in flight land before the CTA gives up its shared memory
+      for (int i = j > ST ? j - ST : 0; i < j; ++i)
+        (void)mbar_wait_bounded(&full[i % ST], static_cast<uint32_t>((i / ST) & 1), 200000000ull);
+    }
+    return;
+  }
+
+  if (warp > AT_WARPS) {
+    if (!a.accumulate) return;
+    const int at = tid - 32 * (AT_WARPS + 1);
+    for (int job = 0;; ++job) {
+      const int x = job & 1;
+      if (!__all_sync(0xffffffffu, mbar_wait_bounded(&job_full[x], static_cast<uint32_t>((job >> 1) & 1)))) {
+        if (lane == 0) report(a.status, LINATTN_DEV_TIMEOUT);
+        return;
+      }
+      const int count = job_count[x];
+      if (count < 0) return;
+      const int64_t unit = job_unit[x];
+      float* mass = a.mass + unit * a.M;
+      const float* sc = a.scores + unit * a.heads * a.M;
+      if ((a.M & 3) == 0) {  // rows on 16 bytes: 8 slots a thread at a time, the loads together
+        constexpr int U = 2;
+        const int quads = (count + 3) >> 2, stride = a.M >> 2;
+        for (int n0 = at; n0 < quads; n0 += U * AT_MASS) {
+          float4 v[U];
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            v[u] = n0 + u * AT_MASS < quads ? reinterpret_cast<const float4*>(mass)[n0 + u * AT_MASS] : make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int h0 = 0; h0 < a.heads; h0 += 4) {
+            float4 y[U][4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+              for (int u = 0; u < U; ++u)
+                if (h0 + e < a.heads && n0 + u * AT_MASS < quads)
+                  y[u][e] = __ldcg(reinterpret_cast<const float4*>(sc) + static_cast<int64_t>(h0 + e) * stride + n0 + u * AT_MASS);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (h0 + e < a.heads) {
+                const float f0 = fin[x][0][h0 + e], f1 = fin[x][1][h0 + e];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                  const int n = (n0 + u * AT_MASS) * 4;  // slots past the count keep what they hold
+                  if (n < count) v[u].x += ex2_approx(y[u][e].x - f0) * f1;
+                  if (n + 1 < count) v[u].y += ex2_approx(y[u][e].y - f0) * f1;
+                  if (n + 2 < count) v[u].z += ex2_approx(y[u][e].z - f0) * f1;
+                  if (n + 3 < count) v[u].w += ex2_approx(y[u][e].w - f0) * f1;
+                }
+              }
+          }
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (n0 + u * AT_MASS < quads) reinterpret_cast<float4*>(mass)[n0 + u * AT_MASS] = v[u];
+        }
+      } else {
+        for (int n = at; n < count; n += AT_MASS) {
+          float v = mass[n];
+#pragma unroll 4
+          for (int head = 0; head < a.heads; ++head)
+            v += ex2_approx(__ldcg(sc + static_cast<int64_t>(head) * a.M + n) - fin[x][0][head]) * fin[x][1][head];
+          mass[n] = v;
         }
       }
-      if (next < hi) load_k(next);  // K of the next slots behind this tile's softmax and P V
-      const bool in0 = base + g < hi, in1 = base + g + 8 < hi;
+      mbar_arrive(&job_empty[x]);
+    }
+  }
+
+  const int g = lane >> 2, tig = lane & 3;
+  const int ct = warp % CT, th = warp / CT;      // P V: 16-channel tile, slots (D = 64: half) of a tile
+  constexpr int KT = D == 64 ? 4 : 8;            // 16-slot steps of P V
+  const uint32_t ring_a = smem_u32(ring), p_a = smem_u32(pbuf);
+  // ldmatrix rows of this lane: K rows 16 warp + ..., V rows by step, P rows by head
+  const int krow = 16 * warp + (lane & 15), kchunk = lane >> 4;
+  const int vrow = (lane & 7) + ((lane >> 4) & 1) * 8, vchunk = ct * 2 + ((lane >> 3) & 1);
+  const uint32_t k_off = krow * 128, v_off = HALVES * SM::HALF + (vchunk >> 3) * SM::HALF;
+  int j = 0, jobs = 0;
+  int64_t t = t0;
+  bool ok = true;
+  // room for a unit's result: the mass warps are done with the one before the last
+  auto job_room = [&] {
+    if (a.accumulate && jobs >= 2 && ok)
+      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&job_empty[jobs & 1], static_cast<uint32_t>((jobs / 2 - 1) & 1)));
+  };
+  auto job_send = [&](int64_t unit, int count) {  // one thread, after a barrier
+    job_unit[jobs & 1] = unit;
+    job_count[jobs & 1] = count;
+    mbar_arrive(&job_full[jobs & 1]);
+  };
+  while (t < t1) {
+    const int end = static_cast<int>(lmin(w.tiles, first + (t1 - t)));
+    const int64_t unit = static_cast<int64_t>(w.b) * a.H + w.h;
+    // q as the B operand: channels 16 kk + 2 tig (+ 1, + 8, + 9) of head g
+    uint32_t q[NT][D / 16][2];
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+      const int head = x * 8 + g;
+      const T* src = static_cast<const T*>(a.q) + w.b * a.qb + (static_cast<int64_t>(w.h) * a.G + a.h0 + head) * a.qh + 2 * tig;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) q[x][kk][e] = head < a.heads ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + e * 8) : 0u;
+    }
+    float acc[NT][4], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+      acc[x][0] = acc[x][1] = acc[x][2] = acc[x][3] = 0.f;
+      m[x][0] = m[x][1] = -INFINITY;
+      l[x][0] = l[x][1] = 0.f;
+    }
+    float* sc = a.scores + unit * a.heads * a.M;
+    for (int i = first; i < end; ++i, ++j) {
+      const int st = j % ST, valid = min(AT_ROWS, w.count - i * AT_ROWS);
+      // a warp whose wait gave up goes on through the barriers
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full[st], static_cast<uint32_t>((j / ST) & 1)));
+      const uint32_t stage = ring_a + st * SM::STAGE;
+      float s[NT][4], s2[NT][4];  // two chains of products
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[x][e] = s2[x][e] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        uint32_t f[4];
+        const int chunk = (kk & 3) * 2 + kchunk;
+        ldsm_x4(stage + (kk >> 2) * SM::HALF + k_off + ((chunk ^ (krow & 7)) << 4), f[0], f[1], f[2], f[3]);
+#pragma unroll
+        for (int x = 0; x < NT; ++x) M::mma((kk & 1) ? s2[x] : s[x], f, q[x][kk][0], q[x][kk][1]);
+      }
+      const int r0 = 16 * warp + g, r1 = r0 + 8;
       bool grow = false;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
+      for (int x = 0; x < NT; ++x)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bool in = i < 2 ? in0 : in1;
-          const float x = in ? s[t][i] * a.scale_log2 : -INFINITY;
-          s[t][i] = x;
-          const int head = t * 8 + 2 * tig + (i & 1);
-          if (in && a.accumulate && head < heads) sc[head * sc_stride + (base - lo) + g + (i < 2 ? 0 : 8)] = x;
-          grow |= x > m[t][i & 1] + 8.f;
+        for (int e = 0; e < 4; ++e) {
+          const int r = e < 2 ? r0 : r1, head = x * 8 + 2 * tig + (e & 1);
+          const float v = r < valid ? (s[x][e] + s2[x][e]) * a.scale_log2 : -INFINITY;
+          s[x][e] = v;
+          if (a.accumulate && r < valid && head < a.heads) sc[static_cast<int64_t>(head) * a.M + i * AT_ROWS + r] = v;
+          grow |= v > m[x][e & 1] + 8.f;
         }
-      }
-      if (__any_sync(0xffffffffu, grow)) {  // the running maximum moves only past a margin of 2^8
+      uint8_t* pb = pbuf + (j & 1) * (2 * HN * AT_PROW);
+      float ps[NT][2];  // this lane's share of the tile's sums
+      auto weights = [&] {
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int x = 0; x < NT; ++x) {
+          const float z0 = m[x][0] == -INFINITY ? 0.f : m[x][0], z1 = m[x][1] == -INFINITY ? 0.f : m[x][1];
+          const float p0 = ex2_approx(s[x][0] - z0), p1 = ex2_approx(s[x][1] - z1);
+          const float p2 = ex2_approx(s[x][2] - z0), p3 = ex2_approx(s[x][3] - z1);
+          ps[x][0] = p0 + p2;
+          ps[x][1] = p1 + p3;
+          const uint32_t h01 = M::pack(p0, p1), h23 = M::pack(p2, p3);
+          const float2 u01 = M::unpack(h01), u23 = M::unpack(h23);
+          // transposed: head g, slots 2 tig and 2 tig + 1
+          uint8_t* row = pb + (x * 8 + g) * AT_PROW + (16 * warp + 2 * tig) * 2;
+          *reinterpret_cast<uint32_t*>(row) = movmatrix_t(h01);
+          *reinterpret_cast<uint32_t*>(row + 16) = movmatrix_t(h23);
+          *reinterpret_cast<uint32_t*>(row + HN * AT_PROW) = movmatrix_t(M::pack(p0 - u01.x, p1 - u01.y));
+          *reinterpret_cast<uint32_t*>(row + HN * AT_PROW + 16) = movmatrix_t(M::pack(p2 - u23.x, p3 - u23.y));
+        }
+      };
+      weights();
+      if (attend_barrier_or(grow)) {  // the running maximum moves only past a margin of 2^8
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float mx = fmaxf(s[t][c], s[t][c + 2]);
+            float v = fmaxf(s[x][c], s[x][c + 2]);
 #pragma unroll
-            for (int o = 4; o <= 16; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-            mx = fmaxf(mx, m[t][c]);
-            const float f = m[t][c] == -INFINITY ? 0.f : ex2_approx(m[t][c] - mx);
-            m[t][c] = mx;
-            l[t][c] *= f;
+            for (int o = 4; o <= 16; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+            if (g == 0) mx_w[warp][x * 8 + 2 * tig + c] = v;
+          }
+        attend_barrier();
 #pragma unroll
-            for (int e = 0; e < MT; ++e) {
-              acc[t][e][c] *= f;
-              acc[t][e][c + 2] *= f;
+        for (int x = 0; x < NT; ++x)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float v = m[x][c];
+#pragma unroll
+            for (int y = 0; y < AT_WARPS; ++y) v = fmaxf(v, mx_w[y][x * 8 + 2 * tig + c]);
+            const float f = m[x][c] == -INFINITY ? 0.f : ex2_approx(m[x][c] - v);
+            m[x][c] = v;
+            l[x][c] *= f;
+            acc[x][c] *= f;
+            acc[x][c + 2] *= f;
+          }
+        weights();
+        attend_barrier();
+      }
+#pragma unroll
+      for (int x = 0; x < NT; ++x) {
+        l[x][0] += ps[x][0];
+        l[x][1] += ps[x][1];
+      }
+      // O^T += V^T P^T, the lo parts in a chain of their own
+      float low[NT][4];
+#pragma unroll
+      for (int x = 0; x < NT; ++x) low[x][0] = low[x][1] = low[x][2] = low[x][3] = 0.f;
+      const uint32_t prow = p_a + (j & 1) * (2 * HN * AT_PROW) + (lane & 7) * AT_PROW + th * KT * 32 + (lane >> 3) * 16;
+#pragma unroll
+      for (int k2 = 0; k2 < KT / 2; ++k2) {  // 32 slots
+        uint32_t f[2][4];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = (th * KT + 2 * k2 + e) * 16 + vrow;
+          ldsm_x4_t(stage + v_off + r * 128 + (((vchunk & 7) ^ (r & 7)) << 4), f[e][0], f[e][1], f[e][2], f[e][3]);
+          if (valid < AT_ROWS) {  // slots that are not in use may hold anything: 0 x Inf
+            const int s0 = (th * KT + 2 * k2 + e) * 16 + 2 * tig;
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              const int sl = s0 + (y >> 1) * 8;
+              f[e][y] &= sl + 1 < valid ? 0xffffffffu : sl < valid ? 0xffffu : 0u;
             }
           }
-      }
-      uint32_t bh[NT][2], bl[NT][2];
+        }
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const float z0 = m[t][0] == -INFINITY ? 0.f : m[t][0], z1 = m[t][1] == -INFINITY ? 0.f : m[t][1];
-        const float p0 = ex2_approx(s[t][0] - z0), p1 = ex2_approx(s[t][1] - z1);
-        const float p2 = ex2_approx(s[t][2] - z0), p3 = ex2_approx(s[t][3] - z1);
-        l[t][0] += p0 + p2;
-        l[t][1] += p1 + p3;
-        const uint32_t h01 = M::pack(p0, p1), h23 = M::pack(p2, p3);
-        const float2 r01 = M::unpack(h01), r23 = M::unpack(h23);
-        bh[t][0] = movmatrix_t(h01);
-        bh[t][1] = movmatrix_t(h23);
-        bl[t][0] = movmatrix_t(M::pack(p0 - r01.x, p1 - r01.y));
-        bl[t][1] = movmatrix_t(M::pack(p2 - r23.x, p3 - r23.y));
-      }
-      // O^T: rows g / g + 8 of tile e are channel e of pieces g and g + 8 (D = 128), or
-      // channels e and e + 4 of piece g (D = 64)
-#pragma unroll
-      for (int e = 0; e < MT; ++e) {
-        const int e0 = e, e1 = VJ == 2 ? e : e + MT, j1 = VJ == 2 ? VJ - 1 : 0;
-        auto word = [&](const uint4& w, int c) { return c < 2 ? w.x : c < 4 ? w.y : c < 6 ? w.z : w.w; };
-        auto join = [&](int j, int c, int x) {
-          return __byte_perm(word(vf[j][x], c), word(vf[j][x + 1], c), (c & 1) ? 0x7632 : 0x5410);
-        };
-        const uint32_t f[4] = {join(0, e0, 0), join(j1, e1, 0), join(0, e0, 2), join(j1, e1, 2)};
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          M::mma(acc[t][e], f, bh[t][0], bh[t][1]);
-          M::mma(acc[t][e], f, bl[t][0], bl[t][1]);
+        for (int x = 0; x < NT; ++x) {
+          uint32_t b[4];
+          ldsm_x4(prow + x * 8 * AT_PROW + k2 * 64, b[0], b[1], b[2], b[3]);
+          M::mma(acc[x], f[0], b[0], b[1]);
+          M::mma(acc[x], f[1], b[2], b[3]);
+          ldsm_x4(prow + (HN + x * 8) * AT_PROW + k2 * 64, b[0], b[1], b[2], b[3]);
+          M::mma(low[x], f[0], b[0], b[1]);
+          M::mma(low[x], f[1], b[2], b[3]);
         }
       }
-      if (next < hi) load_v(next);
-    }
-    // ---- the CTA's (o, m, l)
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[x][e] += low[x][e];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[st]);
+    }
+    // ---- the unit's part is done: sums over the warps
+#pragma unroll
+    for (int x = 0; x < NT; ++x)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
 #pragma unroll
-        for (int o = 4; o <= 16; o <<= 1) l[t][c] += __shfl_xor_sync(0xffffffffu, l[t][c], o);
-        if (g == 0) {
-          ml_warp[warp * HN + t * 8 + 2 * tig + c] = m[t][c];
-          ml_warp[(ATT_WARPS + warp) * HN + t * 8 + 2 * tig + c] = l[t][c];
-        }
+        for (int o = 4; o <= 16; o <<= 1) l[x][c] += __shfl_xor_sync(0xffffffffu, l[x][c], o);
+        if (g == 0) l_w[warp][x * 8 + 2 * tig + c] = l[x][c];
+      }
+    if (D == 64 && th == 1) {
 #pragma unroll
-        for (int e = 0; e < MT; ++e)
+      for (int x = 0; x < NT; ++x)
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const int ch = VJ == 2 ? (g + 8 * r) * 8 + e : g * 8 + e + 4 * r;
-            o_warp[(warp * HN + t * 8 + 2 * tig + c) * D + ch] = acc[t][e][c + 2 * r];
+        for (int e = 0; e < 4; ++e) upper[((ct * 32 + lane) * NT + x) * 4 + e] = acc[x][e];
+    }
+    attend_barrier();
+#pragma unroll
+    for (int x = 0; x < NT; ++x)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float v = 0.f;
+#pragma unroll
+        for (int y = 0; y < AT_WARPS; ++y) v += l_w[y][x * 8 + 2 * tig + c];
+        l[x][c] = v;
+      }
+    if (D == 64 && th == 0) {
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[x][e] += upper[((ct * 32 + lane) * NT + x) * 4 + e];
+    }
+    T* out = static_cast<T*>(a.out) + w.b * a.ob + (static_cast<int64_t>(w.h) * a.G + a.h0) * a.oh;
+    const int64_t u0 = t - first, u1 = u0 + w.tiles;                       // the unit's tiles among all
+    const int64_t c0 = ((u0 + 1) * nc - 1) / total, c1 = (u1 * nc - 1) / total;  // the CTAs that share it
+    bool finish = true;
+    job_room();
+    float (*result)[HN] = fin[jobs & 1];
+    if (c0 == c1) {
+      if (warp == 0 && g == 0) {
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            result[0][x * 8 + 2 * tig + c] = m[x][c] == -INFINITY ? 0.f : m[x][c];
+            result[1][x * 8 + 2 * tig + c] = l[x][c] != 0.f ? 1.f / l[x][c] : 0.f;
           }
       }
-    __syncthreads();
-    for (int i = tid; i < HN * D; i += 32 * ATT_WARPS) {
-      const int head = i / D;
-      float mx = -INFINITY;
+      if (th == 0) {
 #pragma unroll
-      for (int w = 0; w < ATT_WARPS; ++w) mx = fmaxf(mx, ml_warp[w * HN + head]);
-      float o = 0.f, sum = 0.f;
+        for (int x = 0; x < NT; ++x)
 #pragma unroll
-      for (int w = 0; w < ATT_WARPS; ++w) {
-        // a warp without slots (m = -inf, l = 0) is left out; one whose scores are all NaN
-        // (m = -inf, l = NaN) is not
-        const float mw = ml_warp[w * HN + head], lw = ml_warp[(ATT_WARPS + w) * HN + head];
-        const float f = mw == -INFINITY ? lw : ex2_approx(mw - mx);
-        if (f != 0.f) {
-          o += f * o_warp[w * HN * D + i];
-          sum += f * lw;
+          for (int e = 0; e < 4; ++e) {
+            const int head = x * 8 + 2 * tig + (e & 1);
+            const float inv = l[x][e & 1] != 0.f ? 1.f / l[x][e & 1] : 0.f;
+            if (head < a.heads) out[head * a.oh + ct * 16 + g + (e >> 1) * 8] = T(acc[x][e] * inv);
+          }
+      }
+      attend_barrier();
+    } else {
+      // slot 0: the unit began in an earlier CTA's share
+      const int64_t at = static_cast<int64_t>(blockIdx.x) * 2 + (first > 0 ? 0 : 1);
+      float* po = a.part_o + at * HN * D;
+      float* pml = a.part_ml + at * 2 * HN;
+      if (th == 0) {
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) po[(x * 8 + 2 * tig + (e & 1)) * D + ct * 16 + g + (e >> 1) * 8] = acc[x][e];
+      }
+      if (warp == 0 && g == 0) {
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            pml[x * 8 + 2 * tig + c] = m[x][c];
+            pml[HN + x * 8 + 2 * tig + c] = l[x][c];
+          }
+      }
+      __threadfence();
+      attend_barrier();
+      if (tid == 0) {
+        const int n = atomicAdd(a.ticket + unit, 1);
+        arrived = n;
+        if (n == static_cast<int>(c1 - c0)) a.ticket[unit] = 0;
+      }
+      attend_barrier();
+      finish = arrived == static_cast<int>(c1 - c0);
+      if (finish) {
+        __threadfence();
+        // part of CTA c: its second slot where the unit begins, else its first
+        auto slot = [&](int c) { return (c0 + c) * 2 + (c == 0 ? 1 : 0); };
+        const int parts = static_cast<int>(c1 - c0) + 1;
+        float* weight = reinterpret_cast<float*>(pbuf);  // [parts][HN]; P is not read any more
+        float* sums = weight + AT_PARTS * HN;            // [groups][heads * D]
+        for (int head = warp; head < a.heads; head += AT_WARPS) {  // lanes over the parts
+          float mx = -INFINITY, sum = 0.f;
+          for (int c = lane; c < parts; c += 32) mx = fmaxf(mx, __ldcg(a.part_ml + slot(c) * 2 * HN + head));
+#pragma unroll
+          for (int o = 16; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+          for (int c = lane; c < parts; c += 32) {
+            const float mc = __ldcg(a.part_ml + slot(c) * 2 * HN + head);
+            const float f = mc == -INFINITY ? 1.f : ex2_approx(mc - mx);  // scores of NaN only: m = -inf, l = NaN
+            weight[c * HN + head] = f;
+            sum += f * __ldcg(a.part_ml + slot(c) * 2 * HN + HN + head);
+          }
+#pragma unroll
+          for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          if (lane == 0) {
+            result[0][head] = mx == -INFINITY ? 0.f : mx;
+            result[1][head] = sum != 0.f ? 1.f / sum : 0.f;
+          }
         }
-      }
-      o_cta[i] = o;
-      if (i % D == 0) {
-        ml_cta[head] = mx;
-        ml_cta[HN + head] = sum;
+        attend_barrier();
+        // groups of threads over the parts, four channels a thread
+        const int quads = a.heads * (D / 4), groups = max(1, 32 * AT_WARPS / quads);
+        for (int y0 = 0; y0 < quads; y0 += 32 * AT_WARPS) {
+          const int y = y0 + tid % min(quads, 32 * AT_WARPS), grp = tid / min(quads, 32 * AT_WARPS);
+          if (y < quads && grp < groups) {
+            const int head = y / (D / 4);
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+            for (int c = grp; c < parts; c += groups) {
+              const float4 p = __ldcg(reinterpret_cast<const float4*>(a.part_o + slot(c) * HN * D) + y);
+              const float f = weight[c * HN + head];
+              o.x += f * p.x;
+              o.y += f * p.y;
+              o.z += f * p.z;
+              o.w += f * p.w;
+            }
+            reinterpret_cast<float4*>(sums)[grp * quads + y] = o;
+          }
+        }
+        attend_barrier();
+        for (int y = tid; y < a.heads * D; y += 32 * AT_WARPS) {
+          float o = 0.f;
+          for (int x = 0; x < groups; ++x) o += sums[x * quads * 4 + y];
+          out[(y / D) * a.oh + y % D] = T(o * result[1][y / D]);
+        }
+        attend_barrier();  // P is written again
       }
     }
-    cluster.sync();
-    // ---- merge over the cluster; this CTA writes its share of the outputs
-    float* lse2 = ml_warp;  // [HN] maximum, then [HN] 1 / sum (ml_warp is no longer read)
-    if (tid < HN) {
-      float mx = -INFINITY, sum = 0.f;
-      for (int r = 0; r < cl; ++r) mx = fmaxf(mx, cluster.map_shared_rank(ml_cta, r)[tid]);
-      for (int r = 0; r < cl; ++r) {
-        const float* o = cluster.map_shared_rank(ml_cta, r);
-        sum += o[tid] == -INFINITY ? o[HN + tid] : ex2_approx(o[tid] - mx) * o[HN + tid];
-      }
-      lse2[tid] = mx == -INFINITY ? 0.f : mx;
-      lse2[HN + tid] = sum != 0.f ? 1.f / sum : 0.f;
+    if (finish && a.accumulate) {
+      if (tid == 0) job_send(unit, w.count);
+      ++jobs;
     }
-    __syncthreads();
-    for (int i = rank * 32 * ATT_WARPS + tid; i < heads * D; i += cl * 32 * ATT_WARPS) {
-      const int head = i / D;
-      float o = 0.f;
-      for (int r = 0; r < cl; ++r) {
-        const float* ml = cluster.map_shared_rank(ml_cta, r);
-        const float f = ml[head] == -INFINITY ? ml[HN + head] : ex2_approx(ml[head] - lse2[head]);
-        if (f != 0.f) o += f * cluster.map_shared_rank(o_cta, r)[i];
-      }
-      store_any(a.out, b * a.ob + (static_cast<int64_t>(h) * a.G + h0 + head) * a.oh + i % D,
-                std::is_same<T, __half>::value ? LINATTN_F16 : LINATTN_BF16, o * lse2[HN + head]);
-    }
-    if (a.accumulate)
-      for (int n = tid; n < hi - lo; n += 32 * ATT_WARPS) {
-        float w = 0.f;
-        for (int e = 0; e < heads; ++e) w += ex2_approx(sc[e * sc_stride + n] - lse2[e]) * lse2[HN + e];
-        mass[lo + n] += w;
-      }
-    cluster.sync();  // o_cta and ml_cta are read by the other CTAs; the buffers are free again
+    t += end - first;
+    first = 0;
+    w.next();
+  }
+  if (a.accumulate) {
+    job_room();
+    if (tid == 0) job_send(0, -1);
+  }
+  if (!ok && lane == 0) {
+    report(a.status, LINATTN_DEV_TIMEOUT);
+    dead = 1;
   }
 }
 
@@ -291,54 +618,34 @@ int attend_fail(int code, const char* what) {
   return set_error(code, msg);
 }
 
-struct AttendPlan {
-  int nt, cl, part, smem;
-  bool global_scores;
-};
+constexpr int AT_HEADS = 32;  // query heads of a group in one launch
 
-constexpr int ATT_SMEM_SCORES = 64 * 1024;  // scores of a part kept in shared memory at most
-
-// Cluster size: enough CTAs for about four rounds of the GPU's 296 (two to an SM), with at
-// least 128 slots each (16 for each warp).
-AttendPlan attend_plan(int64_t units, int64_t G, int64_t M, int D) {
-  AttendPlan p;
-  p.nt = G > 8 ? 2 : 1;
-  p.cl = 1;
-  while (p.cl < 8 && units * p.cl < 592 && M > 128 * p.cl) p.cl *= 2;
-  p.part = static_cast<int>((M + 16 * p.cl - 1) / (16 * p.cl)) * 16;
-  const int64_t heads = 8 * p.nt;
-  const int64_t scores = heads * p.part * 4;
-  p.global_scores = scores > ATT_SMEM_SCORES;
-  const int fixed = (p.nt == 1 ? attend_fixed_smem<1>(D) : attend_fixed_smem<2>(D)) * 4;
-  p.smem = fixed + (p.global_scores ? 0 : static_cast<int>(scores));
-  return p;
-}
+int attend_nt(int64_t heads) { return heads > 16 ? 4 : heads > 8 ? 2 : 1; }
 
 template <typename T, int D, int NT>
-cudaError_t launch_attend(const HeavyAttendArgs& a, const AttendPlan& p, int64_t units, cudaStream_t st) {
+cudaError_t launch_attend(const HeavyAttendArgs& a, const CUtensorMap& k, const CUtensorMap& v, unsigned grid, cudaStream_t st) {
   auto kern = heavy_attend_kernel<T, D, NT>;
   static int allowed[64] = {};
-  cudaError_t e = allow_smem(kern, p.smem, allowed);
+  const cudaError_t e = allow_smem(kern, AttendSmem<D, NT>::BYTES, allowed);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
-  cfg.gridDim = dim3(static_cast<unsigned>(units * p.cl));
-  cfg.blockDim = dim3(32 * ATT_WARPS);
-  cfg.dynamicSmemBytes = static_cast<size_t>(p.smem);
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(AT_THREADS);
+  cfg.dynamicSmemBytes = AttendSmem<D, NT>::BYTES;
   cfg.stream = st;
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(p.cl);
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, a);
+  return cudaLaunchKernelEx(&cfg, kern, a, k, v);
 }
 
-template <typename T>
-cudaError_t dispatch_attend(const HeavyAttendArgs& a, const AttendPlan& p, int D, int64_t units, cudaStream_t st) {
-  if (D == 128) return p.nt == 1 ? launch_attend<T, 128, 1>(a, p, units, st) : launch_attend<T, 128, 2>(a, p, units, st);
-  return p.nt == 1 ? launch_attend<T, 64, 1>(a, p, units, st) : launch_attend<T, 64, 2>(a, p, units, st);
+template <typename T, int D>
+cudaError_t dispatch_attend(const HeavyAttendArgs& a, const CUtensorMap& k, const CUtensorMap& v, unsigned grid, cudaStream_t st) {
+  const int nt = attend_nt(a.heads);
+  return nt == 1 ? launch_attend<T, D, 1>(a, k, v, grid, st)
+                 : nt == 2 ? launch_attend<T, D, 2>(a, k, v, grid, st) : launch_attend<T, D, 4>(a, k, v, grid, st);
 }
 
 }  // namespace
@@ -347,36 +654,46 @@ cudaError_t dispatch_attend(const HeavyAttendArgs& a, const AttendPlan& p, int D
 
 using namespace linattn;
 
+namespace {
+
+int64_t attend_ctas(int64_t units, int64_t budget) { return lmin(lmin(sm_count(), AT_PARTS), units * ((budget + AT_ROWS - 1) / AT_ROWS)); }
+
+}  // namespace
+
 extern "C" int64_t linattn_heavy_attend_workspace(int64_t batch, int64_t Hq, int64_t Hkv, int64_t budget) {
-  if (batch < 1 || Hkv < 1 || Hq < 1 || budget < 1) return 0;
-  const AttendPlan p = attend_plan(batch * Hkv, Hq / Hkv, budget, 128);
-  return p.global_scores ? batch * Hkv * 8 * p.nt * budget * 4 : 0;
+  if (batch < 1 || Hkv < 1 || Hq < Hkv || budget < 1) return 0;
+  const int64_t heads = lmin(Hq / Hkv, AT_HEADS), hn = 8 * attend_nt(heads);
+  return batch * Hkv * heads * budget * 4 + sm_count() * 2 * hn * (128 + 2) * 4 + 64;
 }
 
 extern "C" int linattn_heavy_attend(const linattn_heavy_t* cache, const void* q, int64_t Hq, const int64_t* q_strides,
                                     float scale, int32_t accumulate, void* out, const int64_t* out_strides,
-                                    void* workspace, int64_t workspace_bytes, void* stream) {
-  if (!cache || !cache->k || !cache->v || !cache->mass || !cache->seen || !q || !out || !q_strides || !out_strides)
+                                    int32_t* ticket, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream) {
+  if (!cache || !cache->k || !cache->v || !cache->mass || !cache->seen || !q || !out || !q_strides || !out_strides || !ticket)
     return attend_fail(LINATTN_EINVAL, "NULL pointer");
   if (cache->dtype != LINATTN_F16 && cache->dtype != LINATTN_BF16)
     return attend_fail(LINATTN_EUNSUPPORTED, "f16 or bf16 caches");
-  if (cache->head_dim != 64 && cache->head_dim != 128) return attend_fail(LINATTN_EUNSUPPORTED, "head_dim must be 64 or 128");
+  const int64_t D = cache->head_dim;
+  if (D != 64 && D != 128) return attend_fail(LINATTN_EUNSUPPORTED, "head_dim must be 64 or 128");
   if (cache->batch < 1 || cache->n_kv_heads < 1 || cache->budget < 1 || cache->budget > (1 << 24))
     return attend_fail(LINATTN_EINVAL, "batch, n_kv_heads and budget must be > 0 (budget <= 2^24)");
   if (Hq < 1 || Hq % cache->n_kv_heads) return attend_fail(LINATTN_EINVAL, "H_q must be a multiple of H_kv");
   if (!(scale > 0.f) || scale > 1e30f) return attend_fail(LINATTN_EINVAL, "scale must be positive and finite");
-  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache->k) | reinterpret_cast<uintptr_t>(cache->v)) % 16 ||
-      q_strides[0] % 8 || q_strides[1] % 8)
-    return attend_fail(LINATTN_EINVAL, "q, K and V rows must be 16-byte aligned");
-  const int64_t units = static_cast<int64_t>(cache->batch) * cache->n_kv_heads;
-  const int64_t G = Hq / cache->n_kv_heads;
-  const AttendPlan p = attend_plan(units, G, cache->budget, cache->head_dim);
-  if (units * p.cl >= (int64_t(1) << 31) || G > 1024) return attend_fail(LINATTN_EUNSUPPORTED, "too many heads");
-  if (p.global_scores && accumulate && (!workspace || workspace_bytes < units * 8 * p.nt * cache->budget * 4))
-    return attend_fail(LINATTN_EINVAL, "workspace too small");
+  if ((reinterpret_cast<uintptr_t>(cache->k) | reinterpret_cast<uintptr_t>(cache->v)) % 16 || reinterpret_cast<uintptr_t>(q) % 4 ||
+      q_strides[0] % 2 || q_strides[1] % 2)
+    return attend_fail(LINATTN_EINVAL, "K and V must be 16-byte aligned, q rows 4-byte aligned");
+  const int64_t units = static_cast<int64_t>(cache->batch) * cache->n_kv_heads, rows = units * cache->budget;
+  if (rows >= (int64_t(1) << 31)) return attend_fail(LINATTN_EUNSUPPORTED, "too many slots for 32-bit TMA coordinates");
+  if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 ||
+      workspace_bytes < linattn_heavy_attend_workspace(cache->batch, Hq, cache->n_kv_heads, cache->budget))
+    return attend_fail(LINATTN_EINVAL, "workspace too small or not 16-byte aligned");
+  const CUtensorMapDataType cu = cache->dtype == LINATTN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUtensorMap tk, tv;
+  const int64_t dims[3] = {D, rows, 1}, strides[2] = {D * 2, rows * D * 2};
+  const int box[3] = {64, AT_BOX, 1};
+  if (!tensor_map_3d(&tk, cache->k, cu, dims, strides, box) || !tensor_map_3d(&tv, cache->v, cu, dims, strides, box))
+    return attend_fail(LINATTN_ECUDA, "tensor map encoding failed");
   HeavyAttendArgs a;
-  a.k = static_cast<const uint4*>(cache->k);
-  a.v = static_cast<const uint4*>(cache->v);
   a.mass = cache->mass;
   a.seen = cache->seen;
   a.q = q;
@@ -385,15 +702,25 @@ extern "C" int linattn_heavy_attend(const linattn_heavy_t* cache, const void* q,
   a.qh = q_strides[1];
   a.ob = out_strides[0];
   a.oh = out_strides[1];
+  a.B = cache->batch;
   a.H = cache->n_kv_heads;
   a.M = cache->budget;
-  a.G = static_cast<int>(G);
+  a.G = static_cast<int>(Hq / cache->n_kv_heads);
   a.scale_log2 = scale * 1.4426950408889634f;
   a.accumulate = accumulate ? 1 : 0;
-  a.scores = p.global_scores && accumulate ? static_cast<float*>(workspace) : nullptr;
-  a.part_max = p.part;
+  a.ticket = ticket;
+  a.status = status;
+  const unsigned grid = static_cast<unsigned>(attend_ctas(units, cache->budget));
+  const int64_t most = lmin(a.G, AT_HEADS), hn = 8 * attend_nt(most);
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = a.part_o + sm_count() * 2 * hn * D;
+  a.scores = a.part_ml + sm_count() * 2 * 2 * hn;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = cache->dtype == LINATTN_F16 ? dispatch_attend<__half>(a, p, cache->head_dim, units, st)
-                                                    : dispatch_attend<__nv_bfloat16>(a, p, cache->head_dim, units, st);
+  cudaError_t e = cudaSuccess;
+  for (a.h0 = 0; e == cudaSuccess && a.h0 < a.G; a.h0 += AT_HEADS) {  // larger groups: 32 heads at a time
+    a.heads = static_cast<int>(lmin(a.G - a.h0, AT_HEADS));
+    if (cache->dtype == LINATTN_F16) e = D == 128 ? dispatch_attend<__half, 128>(a, tk, tv, grid, st) : dispatch_attend<__half, 64>(a, tk, tv, grid, st);
+    else e = D == 128 ? dispatch_attend<__nv_bfloat16, 128>(a, tk, tv, grid, st) : dispatch_attend<__nv_bfloat16, 64>(a, tk, tv, grid, st);
+  }
   return e == cudaSuccess ? LINATTN_OK : attend_fail(LINATTN_ECUDA, cudaGetErrorString(e));
 }

@@ -34,7 +34,7 @@ class HeavyCache:
     """``budget`` slots per (sequence, kv head) with accumulated attention weights.
 
     Every update runs on the device and on the current stream: no host copy of the lengths,
-    no allocation, so a decode step can be captured in a CUDA graph.  ``seen (B,)`` counts
+    no allocation after the first step, so a decode step can be captured in a CUDA graph.  ``seen (B,)`` counts
     the tokens of each sequence; ``min(seen, budget)`` slots are in use."""
 
     def __init__(self, batch: int, n_kv_heads: int, head_dim: int, budget: int, *, sinks: int = 0, recent: int = 1,
@@ -60,11 +60,13 @@ class HeavyCache:
         self.seen = torch.zeros(batch, dtype=torch.int32, device=self.device)
         self._ticket = torch.zeros(batch, dtype=torch.int32, device=self.device)
         self.device = self.k.device
-        self._scores: Optional[torch.Tensor] = None  # attend()'s workspace, when it needs one
+        self._unit_ticket = torch.zeros(batch * n_kv_heads, dtype=torch.int32, device=self.device)
+        self._workspace: Optional[torch.Tensor] = None  # attend()'s, by its first call
         self._desc = L.Heavy(self.k.data_ptr(), self.v.data_ptr(), self.mass.data_ptr(), self.pos.data_ptr(),
                              self.seen.data_ptr(), L.dtype_code(self.k), batch, n_kv_heads, budget, head_dim, sinks, recent)
         # what every call passes
         self._lib, self._ref, self._ticket_ptr = L.lib(), ctypes.byref(self._desc), self._ticket.data_ptr()
+        self._unit_ticket_ptr = self._unit_ticket.data_ptr()
         self._status_ptr = L.status_word(self.device).data_ptr()
         self._scale = 1.0 / math.sqrt(head_dim)
 
@@ -131,12 +133,15 @@ class HeavyCache:
             out = torch.empty(shape, dtype=q.dtype, device=dev)
         elif out.shape != shape or out.dtype != q.dtype or out.stride(3) != 1:
             raise ValueError("out must have q's shape and dtype with contiguous channels")
-        need = _attend_bytes(self.batch, shape[1], self.n_kv_heads, self.budget) if accumulate else 0
-        if need and (self._scores is None or self._scores.numel() < need):
-            self._scores = torch.empty(need, dtype=torch.uint8, device=dev)
+        need = _attend_bytes(self.batch, shape[1], self.n_kv_heads, self.budget)
+        if self._workspace is None or self._workspace.numel() < need:
+            self._workspace = torch.empty(need, dtype=torch.uint8, device=dev)
         L.check(self._lib.linattn_heavy_attend(
             self._ref, q.data_ptr(), shape[1], L.strides2(q), self._scale if scale is None else float(scale), int(accumulate),
-            out.data_ptr(), L.strides2(out), self._scores.data_ptr() if need else None, need, L.raw_stream(dev.index)))
+            out.data_ptr(), L.strides2(out), self._unit_ticket_ptr, self._workspace.data_ptr(), need, self._status_ptr,
+            L.raw_stream(dev.index)))
+        if L.strict():
+            L.check_status(dev)
         return out
 
     def step(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: Optional[float] = None,

@@ -87,10 +87,10 @@ def test_heavy_calls():
     assert lib.linattn_heavy_load(_heavy(), P, P, I2, I2, 10, None, 10, P, None, 1, None, None) == 1
     assert lib.linattn_heavy_load(_heavy(), P, P, I2, I2, 10, P, 10, P, None, 0, None, None) == 0
     bad = [dict(cache=_heavy(dtype=L.F32)), dict(cache=_heavy(head_dim=128 + 64)), dict(hq=3), dict(scale=-1.0), dict(q=None),
-           dict(qs=(L.c_i64 * 2)(64, 63))]
+           dict(qs=(L.c_i64 * 2)(64, 63)), dict(ticket=None), dict(ws=None), dict(ws_bytes=64)]
     for b in bad:
         a = dict(cache=_heavy(), q=P, hq=4, qs=(L.c_i64 * 2)(256, 64), scale=0.1, acc=1, out=P, os=(L.c_i64 * 2)(256, 64),
-                 ws=None, ws_bytes=0, stream=None)
+                 ticket=P, ws=P, ws_bytes=1 << 30, status=None, stream=None)
         a.update(b)
         assert lib.linattn_heavy_attend(*a.values()) in (1, 2)
 
