@@ -3,21 +3,27 @@
 // the keys with a running maximum and sum.
 //
 // A row tile is 128 / G tokens times the G heads of one kv head (128 rows, brought in by one
-// 3-D tensor-map box), so that the group shares its K and V; a CTA works on two row tiles of
-// one sequence with the same 128-key tiles of K and V.  Warp roles (384 threads, one CTA to
-// an SM):
-//   warp 0      TMA: Q once, K and V through two rings;
+// 3-D tensor-map box), so that the group shares its K and V; a work item is two row tiles of
+// one sequence with the same 128-key tiles of K and V.  One CTA to an SM stays for the whole
+// call and takes every gridDim-th item, those of a sequence from its end (the most keys) on.
+// Warp roles (384 threads):
+//   warp 0      TMA: Q of an item, K and V through two rings, on into the next item;
 //   warp 1      issues tcgen05.mma: S_i = Q_i K_j^T (128 x 128, TMEM), O_i += P_i V_j with P_i
 //               read from TMEM over its scores; while one tile's softmax runs, the tensor
-//               cores have the other tile's P V and the next scores;
+//               cores have the other tile's P V and the next scores, and while an item's
+//               outputs are written, the next item's first scores;
 //   warp 2      clears the rows of a sequence's last V tile that belong to the next sequence
 //               (0 x their Inf or NaN would reach this one);
-//   warps 4-7   softmax of row tile 0, warps 8-11 of row tile 1: one thread a row.
+//   warps 4-7   softmax of row tile 0, warps 8-11 of row tile 1: one thread a row, with the
+//               registers that the other warps give up; P leaves in two halves, so that P V
+//               of the first runs while the second is computed.
 // The running maximum moves, and O is rescaled in TMEM, only past a margin of 2^8; the sums
 // are kept in fp32 from the unrounded weights, P is rounded to the inputs' 16-bit type (the
 // same relative rounding as the output's).
 // Bound at D = 128: a 128 x 128 tile takes 1024 clocks of the tensor cores and 1024 clocks of
-// the exponential unit (16 a clock), which the two row tiles overlap.
+// the exponential unit (16 a clock), which the two row tiles overlap.  Taking 2 of 8 weights
+// from a polynomial on the FMA pipe instead was slower (2161 against 1798 us for 16384
+// tokens, 32 / 8 heads): the added instructions cost more issue slots and power than they save.
 // Few rows: the key range is cut into n_splits parts, merged by lse_combine.
 #include <cstdio>
 #include <type_traits>
@@ -48,6 +54,9 @@ struct PackedArgs {
 };
 
 constexpr int PA_THREADS = 384;
+// Registers: 168 a thread at launch; the loading and issuing warpgroup gives up what the two
+// softmax warpgroups take (88 + 2 x 208 = 3 x 168).
+constexpr int PA_REGS_LOW = 88, PA_REGS_HIGH = 208;
 
 template <int D>
 struct PackedSmem {
@@ -56,6 +65,53 @@ struct PackedSmem {
   static constexpr int VS = D == 128 ? 3 : 4;        // V ring stages
   static constexpr int BYTES = 1024 + TILE * (2 + KS + VS);
 };
+
+// One work item: two row tiles of a sequence, a kv head, a part of the keys.
+struct PackedItem {
+  int q_first, lq, k_first, lk, t0, shift, kvh, split;
+  int j0, n0, n1, n;  // first key tile, key tiles of each row tile and of both
+  int ragged;         // the key tile that another sequence's rows end, or -1
+};
+
+// The item of this CTA's `turn`-th turn, back and forth over the CTAs (items get smaller along
+// a sequence: always the same order would give the first CTA the largest of every turn).
+// All lanes of a warp together; false past the last item.
+__device__ __forceinline__ bool packed_item(const PackedArgs& p, int64_t turn, PackedItem* w) {
+  const int64_t item = turn * gridDim.x + ((turn & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+  const int per = p.Hkv * p.n_splits;
+  const int64_t at = item / per;
+  const int rest = static_cast<int>(item - at * per);
+  w->kvh = rest / p.n_splits;
+  w->split = rest - w->kvh * p.n_splits;
+  int seq, tile;
+  if (!packed_tile(p.cu_q, p.S, p.Nq, 2 * p.tokens, at, &seq, &tile)) return false;
+  bool sound = packed_range(p.cu_q, seq, p.Nq, &w->q_first, &w->lq);
+  sound &= packed_range(p.cu_k, seq, p.Nk, &w->k_first, &w->lk);
+  if (!sound && threadIdx.x == 0) report(p.status, LINATTN_DEV_BAD_ID);
+  // the last tokens of a sequence see the most keys: they come first
+  tile = (w->lq + 2 * p.tokens - 1) / (2 * p.tokens) - 1 - tile;
+  w->t0 = tile * 2 * p.tokens;
+  w->shift = w->lk - w->lq;  // token t reads keys up to t + shift
+  int nt[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int first = w->t0 + i * p.tokens, end = min(w->lq, first + p.tokens);
+    const int keys = first >= end ? 0 : p.causal ? max(0, min(w->lk, end + w->shift)) : w->lk;
+    nt[i] = (keys + 127) >> 7;
+  }
+  int j0 = 0, j1 = max(nt[0], nt[1]);
+  if (p.n_splits > 1) {
+    const int share = (j1 + p.n_splits - 1) / p.n_splits;
+    j0 = min(j1, w->split * share);
+    j1 = min(j1, j0 + share);
+  }
+  w->j0 = j0;
+  w->n0 = max(0, min(nt[0], j1) - j0);
+  w->n1 = max(0, min(nt[1], j1) - j0);
+  w->n = max(w->n0, w->n1);
+  w->ragged = (w->lk & 127) && j0 + w->n == (w->lk + 127) >> 7 ? w->n - 1 : -1;
+  return true;
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(PA_THREADS, 1)
@@ -71,41 +127,13 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
   uint8_t* sq = asmem_raw + ((1024 - (smem_u32(asmem_raw) & 1023)) & 1023);  // two row tiles
   uint8_t* sk = sq + 2 * TILE;
   uint8_t* sv_ring = sk + KS * TILE;
-  __shared__ __align__(8) uint64_t q_full[2], k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], v_ragged, s_full[2],
-      p_full[2], pv_done[2], last;
+  __shared__ __align__(8) uint64_t q_full[2], q_empty[2], k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], v_ragged,
+      s_full[2], p_full[2][2], pv_done[2], last;
   __shared__ uint32_t tmem_sh;
   __shared__ int dead;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int kvh = blockIdx.x % p.Hkv;
-  int seq, tile;
-  if (!packed_tile(p.cu_q, p.S, p.Nq, 2 * p.tokens, blockIdx.x / p.Hkv, &seq, &tile)) return;
-  int q_first, lq, k_first, lk;
-  bool sound = packed_range(p.cu_q, seq, p.Nq, &q_first, &lq);
-  sound &= packed_range(p.cu_k, seq, p.Nk, &k_first, &lk);
-  if (!sound && tid == 0) report(p.status, LINATTN_DEV_BAD_ID);
-  // the last tokens of a sequence see the most keys: they come first
-  tile = (lq + 2 * p.tokens - 1) / (2 * p.tokens) - 1 - tile;
-  const int t0 = tile * 2 * p.tokens, shift = lk - lq;  // token t reads keys up to t + shift
-  // key tiles of each row tile, and this split's share [j0, j0 + n)
-  int nt[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int first = t0 + i * p.tokens, end = min(lq, first + p.tokens);
-    const int keys = first >= end ? 0 : p.causal ? max(0, min(lk, end + shift)) : lk;
-    nt[i] = (keys + 127) >> 7;
-  }
-  int j0 = 0, j1 = max(nt[0], nt[1]);
-  if (p.n_splits > 1) {
-    const int share = (j1 + p.n_splits - 1) / p.n_splits;
-    j0 = min(j1, static_cast<int>(blockIdx.y) * share);
-    j1 = min(j1, j0 + share);
-  }
-  const int n0 = max(0, min(nt[0], j1) - j0), n1 = max(0, min(nt[1], j1) - j0), n = max(n0, n1);
   const int boxb = p.tokens * p.G * 128;
-  // the last key tile, if another sequence's rows end it
-  const int ragged = (lk & 127) && j0 + n == (lk + 127) >> 7 ? n - 1 : -1;
-
   if (tid == 0) {
     for (int s = 0; s < KS; ++s) {
       mbar_init(&k_full[s], 1);
@@ -117,8 +145,10 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&q_full[s], 1);
+      mbar_init(&q_empty[s], 1);
       mbar_init(&s_full[s], 1);
-      mbar_init(&p_full[s], 128);
+      mbar_init(&p_full[s][0], 128);
+      mbar_init(&p_full[s][1], 128);
       mbar_init(&pv_done[s], 1);
     }
     mbar_init(&v_ragged, 1);
@@ -135,277 +165,309 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
   tc_fence_after();
   // columns [128 i, 128 i + 128): S / P of row tile i; [256 + 128 i, ...): O of row tile i
   const uint32_t tmem = tmem_sh;
+  PackedItem w;
 
-  if (warp == 0) {
-    if (lane == 0 && n > 0) {
-      int ki = 0, vi = 0;
-      bool ok = true;
-      auto load_q = [&](int i) {
-        mbar_arrive_expect_tx(&q_full[i], boxb * HALVES);
-        for (int c = 0; c < HALVES; ++c)
-          tma_load_3d(sq + i * TILE + c * 16384, &tmq, 64 * c, kvh * p.G, q_first + t0 + i * p.tokens, &q_full[i]);
-      };
-      auto load = [&](const CUtensorMap* tm, uint8_t* ring, uint64_t* full, uint64_t* empty, int stages, int j) {
-        const int st = j % stages;
-        if (j >= stages) ok = mbar_wait_bounded(&empty[st], static_cast<uint32_t>((j / stages - 1) & 1));
-        if (!ok || dead) return false;
-        // a ragged V tile goes to warp 2 first, which passes it on
-        uint64_t* bar = full == v_full && j == ragged ? &v_ragged : &full[st];
-        mbar_arrive_expect_tx(bar, TILE);
-        for (int c = 0; c < HALVES; ++c)
-          tma_load_3d(ring + st * TILE + c * 16384, tm, 64 * c, kvh, k_first + (j0 + j) * 128, bar);
-        return true;
-      };
-      if (n0 > 0) load_q(0);
-      if (load(&tmk, sk, k_full, k_empty, KS, 0)) ki = 1;
-      if (n1 > 0) load_q(1);
-      for (int j = 0; j < n; ++j) {
-        if (!load(&tmv, sv_ring, v_full, v_empty, VS, j)) break;
-        vi = j + 1;
-        if (j + 1 < n) {
-          if (!load(&tmk, sk, k_full, k_empty, KS, j + 1)) break;
-          ki = j + 2;
+  if (warp < 4) {
+    regs_dec<PA_REGS_LOW>();
+    if (warp == 0) {
+      int kc = 0, vc = 0, rc = 0, qc[2] = {0, 0};  // loads so far: K, V and ragged V tiles, Q of each row tile
+      bool ok = true, ragged_last = false;
+      for (int64_t turn = 0; ok && packed_item(p, turn, &w); ++turn) {
+        if (lane == 0) {
+          auto load_q = [&](int i) {
+            if (qc[i] > 0) ok = ok && mbar_wait_bounded(&q_empty[i], static_cast<uint32_t>((qc[i] - 1) & 1));
+            if (!ok || dead) return;
+            mbar_arrive_expect_tx(&q_full[i], boxb * HALVES);
+            for (int c = 0; c < HALVES; ++c)
+              tma_load_3d(sq + i * TILE + c * 16384, &tmq, 64 * c, w.kvh * p.G, w.q_first + w.t0 + i * p.tokens, &q_full[i]);
+            ++qc[i];
+          };
+          auto load_k = [&](int j) {
+            const int st = kc % KS;
+            if (kc >= KS) ok = ok && mbar_wait_bounded(&k_empty[st], static_cast<uint32_t>((kc / KS - 1) & 1));
+            if (!ok || dead) return;
+            mbar_arrive_expect_tx(&k_full[st], TILE);
+            for (int c = 0; c < HALVES; ++c)
+              tma_load_3d(sk + st * TILE + c * 16384, &tmk, 64 * c, w.kvh, w.k_first + (w.j0 + j) * 128, &k_full[st]);
+            ++kc;
+          };
+          auto load_v = [&](int j) {
+            const int st = vc % VS;
+            if (vc >= VS) ok = ok && mbar_wait_bounded(&v_empty[st], static_cast<uint32_t>((vc / VS - 1) & 1));
+            if (!ok || dead) return;
+            // a ragged V tile goes to warp 2 first, which passes it on
+            ragged_last = j == w.ragged;
+            if (ragged_last) ++rc;
+            uint64_t* bar = ragged_last ? &v_ragged : &v_full[st];
+            mbar_arrive_expect_tx(bar, TILE);
+            for (int c = 0; c < HALVES; ++c)
+              tma_load_3d(sv_ring + st * TILE + c * 16384, &tmv, 64 * c, w.kvh, w.k_first + (w.j0 + j) * 128, bar);
+            ++vc;
+          };
+          if (w.n > 0) {
+            if (w.n0 > 0) load_q(0);
+            load_k(0);
+            if (w.n1 > 0) load_q(1);
+            for (int j = 0; ok && !dead && j < w.n; ++j) {
+              load_v(j);
+              if (j + 1 < w.n) load_k(j + 1);
+            }
+          }
+          if (!ok) report(p.status, LINATTN_DEV_TIMEOUT);
+          if (dead) ok = false;
         }
+        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
       }
-      if (!ok) {
-        report(p.status, LINATTN_DEV_TIMEOUT);
+      if (!ok && lane == 0) {  // the copies in flight land before the CTA gives up its shared memory
         dead = 1;
-      }
-      if (dead) {  // the copies in flight land before the CTA gives up its shared memory
-        if (n0 > 0) (void)mbar_wait_bounded(&q_full[0], 0, 200000000ull);
-        if (n1 > 0) (void)mbar_wait_bounded(&q_full[1], 0, 200000000ull);
-        for (int j = ki > KS ? ki - KS : 0; j < ki; ++j)
+        for (int i = 0; i < 2; ++i)
+          if (qc[i] > 0) (void)mbar_wait_bounded(&q_full[i], static_cast<uint32_t>((qc[i] - 1) & 1), 200000000ull);
+        for (int j = kc > KS ? kc - KS : 0; j < kc; ++j)
           (void)mbar_wait_bounded(&k_full[j % KS], static_cast<uint32_t>((j / KS) & 1), 200000000ull);
-        for (int j = vi > VS ? vi - VS : 0; j < vi; ++j)
-          (void)(j == ragged ? mbar_wait_bounded(&v_ragged, 0, 200000000ull)
-                             : mbar_wait_bounded(&v_full[j % VS], static_cast<uint32_t>((j / VS) & 1), 200000000ull));
+        for (int j = vc > VS ? vc - VS : 0; j < vc; ++j)
+          if (!(ragged_last && j == vc - 1))
+            (void)mbar_wait_bounded(&v_full[j % VS], static_cast<uint32_t>((j / VS) & 1), 200000000ull);
+        if (rc > 0) (void)mbar_wait_bounded(&v_ragged, static_cast<uint32_t>((rc - 1) & 1), 200000000ull);
       }
-    }
-  } else if (warp == 1) {
-    if (lane == 0 && n > 0) {
+    } else if (warp == 1) {
+      int kc = 0, vc = 0, qc0 = 0, qc1 = 0, pc0 = 0, pc1 = 0;  // tiles so far: K, V, Q and P of each row tile
       bool ok = true;
-      const uint32_t qa = smem_u32(sq), ka = smem_u32(sk), va = smem_u32(sv_ring);
-      auto scores = [&](int i, int j) {  // S_i of key tile j
-        const uint32_t kb = ka + (j % KS) * TILE;
+      const uint64_t q_desc = umma_desc(smem_u32(sq), 16, 1024), k_desc = umma_desc(smem_u32(sk), 16, 1024),
+                     v_desc = umma_desc(smem_u32(sv_ring), 16384, 1024);
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      for (int64_t turn = 0; ok && packed_item(p, turn, &w); ++turn) {
+        if (w.n > 0) {
+          auto scores = [&](int i, int j) {  // S_i of the item's key tile j
+            const uint64_t a0 = q_desc + i * (TILE >> 4), b0 = k_desc + ((kc + j) % KS) * (TILE >> 4);
+            if (elect_lane()) {
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * 16384 + (kk & 3) * 32;
-          umma_f16(tmem + i * 128, umma_desc(qa + i * TILE + off, 16, 1024), umma_desc(kb + off, 16, 1024), IDESC_S,
-                   kk > 0 ? 1u : 0u);
+              for (int kk = 0; kk < D / 16; ++kk) {
+                const uint32_t off = ((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;
+                umma_f16(tm + i * 128, a0 + off, b0 + off, IDESC_S, kk > 0 ? 1u : 0u);
+              }
+              umma_commit(&s_full[i]);
+              if (j + 1 == (i ? w.n1 : w.n0)) umma_commit(&q_empty[i]);
+            }
+          };
+          auto key_tile = [&](int j) {
+            ok = ok && warp_wait(&k_full[(kc + j) % KS], static_cast<uint32_t>(((kc + j) / KS) & 1));
+            if (ok) tc_fence_after();
+          };
+          key_tile(0);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (ok && (i ? w.n1 : w.n0) > 0) {
+              ok = warp_wait(&q_full[i], static_cast<uint32_t>((i ? qc1++ : qc0++) & 1));
+              if (ok) {
+                tc_fence_after();
+                scores(i, 0);
+              }
+            }
+          if (ok && elect_lane()) umma_commit(&k_empty[kc % KS]);
+          for (int j = 0; ok && j < w.n; ++j) {
+            bool v_there = false, k_there = false;
+            const uint64_t vd = v_desc + ((vc + j) % VS) * (TILE >> 4);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int ni = i ? w.n1 : w.n0;
+              if (!ok || j >= ni) continue;
+              if (!v_there) ok = warp_wait(&v_full[(vc + j) % VS], static_cast<uint32_t>(((vc + j) / VS) & 1));
+              v_there = true;
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {  // the first 64 keys while the others' weights are computed
+                ok = ok && warp_wait(&p_full[i][h], static_cast<uint32_t>((i ? pc1 : pc0) & 1));
+                if (!ok) break;
+                tc_fence_after();
+                if (elect_lane()) {
+#pragma unroll
+                  for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
+                    umma_f16_ts(tm + 256 + i * 128, tm + i * 128 + 8 * kk, vd + kk * (2048 >> 4), IDESC_O,
+                                (j > 0 || kk > 0) ? 1u : 0u);
+                  if (h == 1) umma_commit(&pv_done[i]);
+                }
+              }
+              if (!ok) break;
+              i ? ++pc1 : ++pc0;
+              if (j + 1 < ni) {
+                if (!k_there) key_tile(j + 1);
+                k_there = true;
+                if (ok) scores(i, j + 1);
+              }
+            }
+            if (ok && elect_lane()) {
+              umma_commit(&v_empty[(vc + j) % VS]);
+              if (k_there) umma_commit(&k_empty[(kc + j + 1) % KS]);
+            }
+          }
+          if (!ok && lane == 0) {
+            report(p.status, LINATTN_DEV_TIMEOUT);
+            dead = 1;
+          }
+          kc += w.n;
+          vc += w.n;
         }
-        umma_commit(&s_full[i]);
-      };
-      auto key_tile = [&](int j) {
-        ok = ok && mbar_wait_bounded(&k_full[j % KS], static_cast<uint32_t>((j / KS) & 1));
-        if (ok) tc_fence_after();
-      };
-      key_tile(0);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (ok && (i ? n1 : n0) > 0) {
-          ok = mbar_wait_bounded(&q_full[i], 0);
+      }
+    } else if (warp == 2) {
+      int vc = 0, rc = 0;
+      bool ok = true;
+      for (int64_t turn = 0; ok && packed_item(p, turn, &w); ++turn) {
+        if (w.ragged >= 0) {
+          ok = __all_sync(0xffffffffu, mbar_wait_bounded(&v_ragged, static_cast<uint32_t>(rc++ & 1)));
           if (ok) {
-            tc_fence_after();
-            scores(i, 0);
+            const int st = (vc + w.ragged) % VS;
+            const int from = (w.lk & 127) * 8;  // 16-byte pieces of the 128-byte rows of one channel half
+            uint8_t* t = sv_ring + st * TILE;
+            for (int c = 0; c < HALVES; ++c)
+              for (int x = from + lane; x < 1024; x += 32)
+                *reinterpret_cast<uint4*>(t + c * 16384 + x * 16) = make_uint4(0u, 0u, 0u, 0u);
+            umma_fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&v_full[st]);
           }
         }
-      if (ok) umma_commit(&k_empty[0]);
-      for (int j = 0; ok && j < n; ++j) {
-        bool v_there = false, k_there = false;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int ni = i ? n1 : n0;
-          if (!ok || j >= ni) continue;
-          if (!v_there) {
-            ok = mbar_wait_bounded(&v_full[j % VS], static_cast<uint32_t>((j / VS) & 1));
-            v_there = true;
-          }
-          ok = ok && mbar_wait_bounded(&p_full[i], static_cast<uint32_t>(j & 1));
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t vb = va + (j % VS) * TILE;
-#pragma unroll
-          for (int kk = 0; kk < 8; ++kk)
-            umma_f16_ts(tmem + 256 + i * 128, tmem + i * 128 + 8 * kk, umma_desc(vb + kk * 2048, 16384, 1024), IDESC_O,
-                        (j > 0 || kk > 0) ? 1u : 0u);
-          umma_commit(&pv_done[i]);
-          if (j + 1 < ni) {
-            if (!k_there) key_tile(j + 1);
-            k_there = true;
-            if (ok) scores(i, j + 1);
-          }
-        }
-        if (ok) {
-          umma_commit(&v_empty[j % VS]);
-          if (k_there) umma_commit(&k_empty[(j + 1) % KS]);
-        }
-      }
-      if (!ok) {
-        report(p.status, LINATTN_DEV_TIMEOUT);
-        dead = 1;
+        vc += w.n;
       }
     }
-  } else if (warp == 2) {
-    if (ragged >= 0) {
-      const bool ok = __all_sync(0xffffffffu, mbar_wait_bounded(&v_ragged, 0));
-      if (ok) {
-        const int from = (lk & 127) * 8;  // 16-byte pieces of the 128-byte rows of one channel half
-        uint8_t* t = sv_ring + (ragged % VS) * TILE;
-        for (int c = 0; c < HALVES; ++c)
-          for (int x = from + lane; x < 1024; x += 32)
-            *reinterpret_cast<uint4*>(t + c * 16384 + x * 16) = make_uint4(0u, 0u, 0u, 0u);
-        umma_fence_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&v_full[ragged % VS]);
-      }
-    }
-  } else if (warp >= 4) {
-    const int i = (warp >> 2) - 1, r = tid & 127, ni = i ? n1 : n0;
+  } else {
+    regs_inc<PA_REGS_HIGH>();
+    const int i = (warp >> 2) - 1, r = tid & 127;
     const uint32_t lane_addr = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
     const uint32_t s_addr = lane_addr + i * 128, o_addr = lane_addr + 256 + i * 128;
-    const int rt = r / p.G, t = t0 + i * p.tokens + rt;
-    const bool row_ok = rt < p.tokens && t < lq;
-    const int klim = !row_ok ? 0 : p.causal ? max(0, min(lk, t + shift + 1)) : lk;  // keys this row reads
+    const int rt = r / p.G, rg = r - rt * p.G;
     const float sl = p.scale_log2;
     const uint64_t sl2 = pack_f2(sl, sl);
-    float m = -INFINITY, l = 0.f;
+    int sc = 0;  // score tiles so far
     bool ok = true;
-    for (int j = 0; j < ni; ++j) {
-      if (!__all_sync(0xffffffffu, mbar_wait_bounded(&s_full[i], static_cast<uint32_t>(j & 1)))) {
-        ok = false;
+    for (int64_t turn = 0; ok && packed_item(p, turn, &w); ++turn) {
+      const int ni = i ? w.n1 : w.n0, t = w.t0 + i * p.tokens + rt;
+      const bool row_ok = rt < p.tokens && t < w.lq;
+      const int klim = (!row_ok ? 0 : p.causal ? max(0, min(w.lk, t + w.shift + 1)) : w.lk) - w.j0 * 128;  // keys this row reads
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < ni; ++j, ++sc) {
+        if (!__all_sync(0xffffffffu, mbar_wait_bounded(&s_full[i], static_cast<uint32_t>(sc & 1)))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t sv[4][32];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) tmem_ld32(s_addr + q * 32, sv[q]);
+        tmem_wait_ld();
+        const int lim = klim - j * 128;
+        if (!__all_sync(0xffffffffu, lim >= 128)) {
+#pragma unroll
+          for (int c = 0; c < 128; ++c)
+            if (c >= lim) sv[c >> 5][c & 31] = 0xff800000u;  // -inf
+        }
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < 128; c += 2)
+          mx4[(c >> 1) & 3] = fmaxf(fmaxf(mx4[(c >> 1) & 3], __uint_as_float(sv[c >> 5][c & 31])),
+                                    __uint_as_float(sv[c >> 5][(c & 31) + 1]));
+        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sl;
+        const bool grow = mx > m + 8.f;
+        if (__any_sync(0xffffffffu, grow)) {
+          const float alpha = grow ? (m == -INFINITY ? 0.f : ex2_approx(m - mx)) : 1.f;
+          if (j > 0) {  // O holds the tiles before this one once their P V is done
+            if (!__all_sync(0xffffffffu, mbar_wait_bounded(&pv_done[i], static_cast<uint32_t>((sc - 1) & 1)))) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t ov[32];
+              tmem_ld32(o_addr + c * 32, ov);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
+              tmem_st32(o_addr + c * 32, ov);
+            }
+            tmem_wait_st();
+          }
+          l *= alpha;
+          if (grow) m = mx;
+        }
+        const float neg = m == -INFINITY ? 0.f : -m;  // nothing read yet: every score is -inf, P = 0
+        const uint64_t neg2 = pack_f2(neg, neg);
+        uint64_t sum[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {  // keys [64 h, 64 h + 64)
+          uint32_t pk[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const int c = h * 64 + 2 * e;
+            const float2 x = unpack_f2(
+                fma_f2(pack_f2(__uint_as_float(sv[c >> 5][c & 31]), __uint_as_float(sv[c >> 5][(c & 31) + 1])), sl2, neg2));
+            const float y0 = ex2_approx(x.x), y1 = ex2_approx(x.y);
+            pk[e] = M::pack(y0, y1);
+            sum[e & 3] = add_f2(sum[e & 3], pack_f2(y0, y1));
+          }
+          tmem_st32(s_addr + h * 32, pk);
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(&p_full[i][h]);
+        }
+        const float2 ts = unpack_f2(add_f2(add_f2(sum[0], sum[1]), add_f2(sum[2], sum[3])));
+        l += ts.x + ts.y;
+      }
+      if (ok && ni > 0)
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&pv_done[i], static_cast<uint32_t>((sc - 1) & 1)));
+      if (!ok) {
+        report(p.status, LINATTN_DEV_TIMEOUT);
+        dead = 1;
         break;
       }
       tc_fence_after();
-      uint32_t sv[4][32];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) tmem_ld32(s_addr + q * 32, sv[q]);
-      tmem_wait_ld();
-      const int lim = klim - (j0 + j) * 128;
-      if (!__all_sync(0xffffffffu, lim >= 128)) {
-#pragma unroll
-        for (int c = 0; c < 128; ++c)
-          if (c >= lim) sv[c >> 5][c & 31] = 0xff800000u;  // -inf
-      }
-      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int c = 0; c < 128; c += 2)
-        mx4[(c >> 1) & 3] = fmaxf(fmaxf(mx4[(c >> 1) & 3], __uint_as_float(sv[c >> 5][c & 31])),
-                                  __uint_as_float(sv[c >> 5][(c & 31) + 1]));
-      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sl;
-      const bool grow = mx > m + 8.f;
-      if (__any_sync(0xffffffffu, grow)) {
-        const float alpha = grow ? (m == -INFINITY ? 0.f : ex2_approx(m - mx)) : 1.f;
-        if (j > 0) {  // O holds the tiles before this one once their P V is done
-          if (!__all_sync(0xffffffffu, mbar_wait_bounded(&pv_done[i], static_cast<uint32_t>((j - 1) & 1)))) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
+      const float inv = l != 0.f ? 1.f / l : 0.f;
+      const float lse = l != 0.f ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
+      const int64_t token = static_cast<int64_t>(w.q_first) + t;
+      const int head = w.kvh * p.G + rg;
+      if (p.n_splits > 1) {
+        const int64_t row = w.split * (p.Nq * p.Hq) + token * p.Hq + head;
+        if (row_ok) p.part_lse[row] = lse;
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t ov[32];
-            tmem_ld32(o_addr + c * 32, ov);
-            tmem_wait_ld();
-#pragma unroll
-            for (int e = 0; e < 32; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
-            tmem_st32(o_addr + c * 32, ov);
-          }
-          tmem_wait_st();
-        }
-        l *= alpha;
-        if (grow) m = mx;
-      }
-      const float neg = m == -INFINITY ? 0.f : -m;  // nothing read yet: every score is -inf, P = 0
-      const uint64_t neg2 = pack_f2(neg, neg);
-      uint64_t sum[4] = {0ull, 0ull, 0ull, 0ull};
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t pk[32];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const int c = h * 64 + 2 * e;
-          const float2 x = unpack_f2(fma_f2(
-              pack_f2(__uint_as_float(sv[c >> 5][c & 31]), __uint_as_float(sv[c >> 5][(c & 31) + 1])), sl2, neg2));
-          const float a = ex2_approx(x.x), b = ex2_approx(x.y);
-          pk[e] = M::pack(a, b);
-          sum[e & 3] = add_f2(sum[e & 3], pack_f2(a, b));
-        }
-        tmem_st32(s_addr + h * 32, pk);
-      }
-      const float2 ts = unpack_f2(add_f2(add_f2(sum[0], sum[1]), add_f2(sum[2], sum[3])));
-      l += ts.x + ts.y;
-      tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive(&p_full[i]);
-    }
-    if (ok && ni > 0)
-      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&pv_done[i], static_cast<uint32_t>((ni - 1) & 1)));
-    if (!ok) {
-      report(p.status, LINATTN_DEV_TIMEOUT);
-      dead = 1;
-    }
-    tc_fence_after();
-    const float inv = l != 0.f ? 1.f / l : 0.f;
-    const float lse = l != 0.f ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
-    const int64_t row = (static_cast<int64_t>(q_first) + t) * p.Hq + kvh * p.G + (r - rt * p.G);
-    const bool have = ok && ni > 0;  // warp-uniform
-    if (p.n_splits > 1) {
-      if (row_ok) p.part_lse[blockIdx.y * (p.Nq * p.Hq) + row] = lse;
-#pragma unroll 1
-      for (int c = 0; c < (have ? D / 32 : 0); ++c) {
-        uint32_t ov[32];
-        tmem_ld32(o_addr + c * 32, ov);
-        tmem_wait_ld();
-        if (row_ok) {
-          float4* dst = reinterpret_cast<float4*>(p.part_o + (blockIdx.y * (p.Nq * p.Hq) + row) * D + c * 32);
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            dst[e] = make_float4(__uint_as_float(ov[4 * e]) * inv, __uint_as_float(ov[4 * e + 1]) * inv,
-                                 __uint_as_float(ov[4 * e + 2]) * inv, __uint_as_float(ov[4 * e + 3]) * inv);
-        }
-      }
-    } else {
-      if (row_ok && p.lse) p.lse[row] = lse;
-      // rows staged in this row tile's Q (every MMA that reads it is done), then written
-      // whole rows at a time: only the rows of this sequence
-      uint8_t* st = sq + i * TILE;
-#pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t ov[32];
-        if (have) {
+        for (int c = 0; c < (ni > 0 ? D / 32 : 0); ++c) {
+          uint32_t ov[32];
           tmem_ld32(o_addr + c * 32, ov);
           tmem_wait_ld();
-        } else {
+          if (row_ok) {
+            float4* dst = reinterpret_cast<float4*>(p.part_o + row * D + c * 32);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) ov[e] = 0u;
+            for (int e = 0; e < 8; ++e)
+              dst[e] = make_float4(__uint_as_float(ov[4 * e]) * inv, __uint_as_float(ov[4 * e + 1]) * inv,
+                                   __uint_as_float(ov[4 * e + 2]) * inv, __uint_as_float(ov[4 * e + 3]) * inv);
+          }
         }
+      } else {
+        if (row_ok && p.lse) p.lse[token * p.Hq + head] = lse;
+        // each thread writes its row, 64 bytes at a time
+        T* dst = static_cast<T*>(p.out) + token * p.ot + head * p.oh;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t ov[32];
+          if (ni > 0) {  // warp-uniform
+            tmem_ld32(o_addr + c * 32, ov);
+            tmem_wait_ld();
+          }
+          if (row_ok) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint32_t w[4];
+            for (int q = 0; q < 4; ++q) {
+              uint32_t y[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            w[e] = l != 0.f ? M::pack(__uint_as_float(ov[q * 8 + 2 * e]) * inv, __uint_as_float(ov[q * 8 + 2 * e + 1]) * inv) : 0u;
-          const int piece = (c & 1) * 4 + q;
-          *reinterpret_cast<uint4*>(st + (c >> 1) * 16384 + r * 128 + ((piece ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+              for (int e = 0; e < 4; ++e)
+                y[e] = l != 0.f ? M::pack(__uint_as_float(ov[q * 8 + 2 * e]) * inv, __uint_as_float(ov[q * 8 + 2 * e + 1]) * inv) : 0u;
+              *reinterpret_cast<uint4*>(dst + c * 32 + q * 8) = make_uint4(y[0], y[1], y[2], y[3]);
+            }
+          }
         }
       }
-      __syncwarp();
-      constexpr int PIECES = D / 8, RPI = 32 / PIECES;  // 16-byte pieces of a row, rows of one step
-      const int piece = lane % PIECES;
-#pragma unroll 4
-      for (int x = 0; x < 32; x += RPI) {
-        const int rr = 32 * (warp & 3) + x + lane / PIECES, tt = rr / p.G, tok = t0 + i * p.tokens + tt;
-        if (tt < p.tokens && tok < lq) {
-          const uint4 w = *reinterpret_cast<const uint4*>(st + (piece >> 3) * 16384 + rr * 128 + (((piece & 7) ^ (rr & 7)) << 4));
-          *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (static_cast<int64_t>(q_first) + tok) * p.ot +
-                                    (static_cast<int64_t>(kvh) * p.G + rr - tt * p.G) * p.oh + piece * 8) = w;
-        }
-      }
+      tc_fence_before();  // the next item's first P V overwrites O after this warp's next P
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (dead && tid == 32 && n > 0) {  // MMAs may still be in flight: wait for them before TMEM goes
+  if (dead && tid == 32) {  // MMAs may still be in flight: wait for them before TMEM goes
     umma_commit(&last);
     (void)mbar_wait_bounded(&last, 0, 200000000ull);
   }
@@ -421,7 +483,7 @@ int packed_fail(int code, const char* what) {
 }
 
 template <typename T, int D>
-cudaError_t launch_packed(const PackedArgs& p, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, dim3 grid,
+cudaError_t launch_packed(const PackedArgs& p, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, unsigned grid,
                           cudaStream_t st) {
   auto kern = packed_attention_kernel<T, D>;
   static int allowed[64] = {};
@@ -503,9 +565,9 @@ extern "C" int linattn_packed_attention(const void* q, const void* k, const void
   p.part_lse = n_splits > 1 ? p.part_o + n_splits * N_q * Hq * D : nullptr;
   p.status = status;
   const int64_t tiles = packed_tiles(N_q, p.G, S, max_q);
-  if (tiles * Hkv >= (int64_t(1) << 31) || n_splits > 1024) return packed_fail(LINATTN_EUNSUPPORTED, "too many tiles");
+  if (Hkv * static_cast<int64_t>(n_splits) >= (int64_t(1) << 31) || n_splits > 1024) return packed_fail(LINATTN_EUNSUPPORTED, "too many tiles");
   if (tiles == 0) return LINATTN_OK;
-  const dim3 grid(static_cast<unsigned>(tiles * Hkv), static_cast<unsigned>(n_splits));
+  const unsigned grid = static_cast<unsigned>(lmin(sm_count(), tiles * Hkv * n_splits));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (dtype == LINATTN_BF16) e = D == 128 ? launch_packed<__nv_bfloat16, 128>(p, tq, tk, tv, grid, st) : launch_packed<__nv_bfloat16, 64>(p, tq, tk, tv, grid, st);

@@ -115,5 +115,57 @@ __device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// 2^x of two values x in [.., 127] on the FMA pipe, beside the exponential unit's 16 a clock:
+// x = n + f with n the nearest integer (added and taken off at 1.5 2^23, whose low bits then
+// hold n), 2^f by the degree-4 polynomial of least relative error on [-1/2, 1/2] (Remez
+// exchange: 2.7e-6 in fp32), n into the exponent.  x below -126 gives 2^-126.  A NaN does not
+// come through: the caller sees to it.
+__device__ __forceinline__ uint64_t ex2_poly2(uint64_t x) {
+  const float2 in = unpack_f2(x);
+  const uint64_t y = pack_f2(fmaxf(in.x, -126.f), fmaxf(in.y, -126.f));
+  const uint64_t t = add_f2(y, pack_f2(12582912.f, 12582912.f));
+  const uint64_t f = fma_f2(add_f2(t, pack_f2(-12582912.f, -12582912.f)), pack_f2(-1.f, -1.f), y);
+  uint64_t p = fma_f2(f, pack_f2(0.009570102207362652f, 0.009570102207362652f),
+                      pack_f2(0.05591785907745361f, 0.05591785907745361f));
+  p = fma_f2(p, f, pack_f2(0.240247443318367f, 0.240247443318367f));
+  p = fma_f2(p, f, pack_f2(0.6931217908859253f, 0.6931217908859253f));
+  p = fma_f2(p, f, pack_f2(0.9999992847442627f, 0.9999992847442627f));
+  const float2 n = unpack_f2(t), r = unpack_f2(p);
+  return pack_f2(__uint_as_float(__float_as_uint(r.x) + (__float_as_uint(n.x) << 23)),
+                 __uint_as_float(__float_as_uint(r.y) + (__float_as_uint(n.y) << 23)));
+}
+// Waits for a whole warp: a warp-uniform answer.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity));
+}
+// One lane of a converged warp.  A warp that issues MMAs runs its loops as a whole and elects
+// the lane at each issue: descriptors and addresses then stay warp-uniform (uniform
+// registers), where a loop of one lane computes and moves them for every instruction.
+__device__ __forceinline__ bool elect_lane() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+// Registers of a warpgroup: given up (all four warps), or taken from what others gave up.
+template <int N>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
 
 }  // namespace linattn
