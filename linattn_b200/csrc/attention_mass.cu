@@ -69,13 +69,11 @@ __global__ void __launch_bounds__(MT_THREADS, 1)
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int kvh = blockIdx.x % p.Hkv;
-  int seq, kt;
-  if (!packed_tile(p.cu_k, p.S, p.Nk, 128, blockIdx.x / p.Hkv, &seq, &kt)) return;
-  int k_first, lk, q_first, lq;
-  bool sound = packed_range(p.cu_k, seq, p.Nk, &k_first, &lk);
-  sound &= packed_range(p.cu_q, seq, p.Nq, &q_first, &lq);
-  if (!sound && tid == 0) report(p.status, LINATTN_DEV_BAD_ID);
-  const int key0 = kt * 128, shift = lk - lq;  // query i stands at position i + shift
+  PackedTile tl;
+  if (!packed_tile(p.cu_k, p.cu_q, p.S, p.Nk, p.Nq, 128, blockIdx.x / p.Hkv, &tl)) return;
+  if (!tl.sound && tid == 0) report(p.status, LINATTN_DEV_BAD_ID);
+  const int k_first = tl.first, lk = tl.n, q_first = tl.other_first, lq = tl.other_n;
+  const int key0 = tl.tile * 128, shift = lk - lq;  // query i stands at position i + shift
   // query tiles that read these keys, and this split's share of them
   const int w_lo = p.window > 0 && p.window < lq ? lq - static_cast<int>(p.window) : 0;
   const int q_lo = max(w_lo, p.causal ? key0 - shift : 0);
@@ -142,25 +140,28 @@ __global__ void __launch_bounds__(MT_THREADS, 1)
           (void)mbar_wait_bounded(&q_full[j % ST], static_cast<uint32_t>((j / ST) & 1), 200000000ull);
     }
   } else if (warp == 1) {
-    if (lane == 0 && n > 0) {
-      bool ok = mbar_wait_bounded(&k_full, 0);
-      const uint32_t ka = smem_u32(sk), qa = smem_u32(sq);
+    if (n > 0) {
+      bool ok = warp_wait(&k_full, 0);
+      const uint64_t k_desc = umma_desc(smem_u32(sk), 16, 1024), q_desc = umma_desc(smem_u32(sq), 16, 1024);
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
       for (int j = 0; ok && j < n; ++j) {
         const int st = j % ST, sb = j % MT_BUFS;
-        ok = mbar_wait_bounded(&q_full[st], static_cast<uint32_t>((j / ST) & 1));
-        if (ok && j >= MT_BUFS) ok = mbar_wait_bounded(&s_empty[sb], static_cast<uint32_t>((j / MT_BUFS - 1) & 1));
+        ok = warp_wait(&q_full[st], static_cast<uint32_t>((j / ST) & 1));
+        if (ok && j >= MT_BUFS) ok = warp_wait(&s_empty[sb], static_cast<uint32_t>((j / MT_BUFS - 1) & 1));
         if (!ok) break;
         tc_fence_after();
+        const uint64_t qd = q_desc + st * (SM::TILE >> 4);
+        if (elect_lane()) {
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * 16384 + (kk & 3) * 32;
-          umma_f16(tmem + sb * 128, umma_desc(ka + off, 16, 1024), umma_desc(qa + st * SM::TILE + off, 16, 1024), IDESC,
-                   kk > 0 ? 1u : 0u);
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = ((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;
+            umma_f16(tm + sb * 128, k_desc + off, qd + off, IDESC, kk > 0 ? 1u : 0u);
+          }
+          umma_commit(&s_full[sb]);
+          umma_commit(&q_empty[st]);
         }
-        umma_commit(&s_full[sb]);
-        umma_commit(&q_empty[st]);
       }
-      if (!ok) {
+      if (!ok && lane == 0) {
         report(p.status, LINATTN_DEV_TIMEOUT);
         dead = 1;
       }

@@ -5,7 +5,7 @@
 // A row tile is 128 / G tokens times the G heads of one kv head (128 rows, brought in by one
 // 3-D tensor-map box), so that the group shares its K and V; a work item is two row tiles of
 // one sequence with the same 128-key tiles of K and V.  One CTA to an SM stays for the whole
-// call and takes every gridDim-th item, those of a sequence from its end (the most keys) on.
+// call and takes every gridDim-th item, back and forth, the items with the most keys first.
 // Warp roles (384 threads):
 //   warp 0      TMA: Q of an item, K and V through two rings, on into the next item;
 //   warp 1      issues tcgen05.mma: S_i = Q_i K_j^T (128 x 128, TMEM), O_i += P_i V_j with P_i
@@ -14,6 +14,8 @@
 //               outputs are written, the next item's first scores;
 //   warp 2      clears the rows of a sequence's last V tile that belong to the next sequence
 //               (0 x their Inf or NaN would reach this one);
+//   warp 3      finds the items (which sequence, which keys) and hands them to the others
+//               through shared memory, a few ahead;
 //   warps 4-7   softmax of row tile 0, warps 8-11 of row tile 1: one thread a row, with the
 //               registers that the other warps give up; P leaves in two halves, so that P V
 //               of the first runs while the second is computed.
@@ -50,10 +52,12 @@ struct PackedArgs {
   int n_splits;
   float* part_o;     // (n_splits, N_q, H_q, D)
   float* part_lse;   // (n_splits, N_q, H_q)
+  int64_t items;     // at most: tiles x H_kv x n_splits
   int32_t* status;
 };
 
 constexpr int PA_THREADS = 384;
+constexpr int PA_ITEMS = 3;  // items handed out ahead
 // Registers: 168 a thread at launch; the loading and issuing warpgroup gives up what the two
 // softmax warpgroups take (88 + 2 x 208 = 3 x 168).
 constexpr int PA_REGS_LOW = 88, PA_REGS_HIGH = 208;
@@ -71,26 +75,96 @@ struct PackedItem {
   int q_first, lq, k_first, lk, t0, shift, kvh, split;
   int j0, n0, n1, n;  // first key tile, key tiles of each row tile and of both
   int ragged;         // the key tile that another sequence's rows end, or -1
+  int more;           // 0: no item any more
 };
 
-// The item of this CTA's `turn`-th turn, back and forth over the CTAs (items get smaller along
-// a sequence: always the same order would give the first CTA the largest of every turn).
-// All lanes of a warp together; false past the last item.
-__device__ __forceinline__ bool packed_item(const PackedArgs& p, int64_t turn, PackedItem* w) {
+// Up to 64 sequences, two to a lane: the pairs of row tiles of all of them from the longest
+// key range to the shortest.  Pair x of a sequence has about (x + base) units of keys, so the
+// pairs at or above a level are counted in closed form and a level is found by bisection.
+// (Sequence after sequence, the static shares of a ragged batch were 35% apart.)
+struct PackedOrder {
+  int first[2], n[2], other_first[2], other_n[2], base[2], pairs[2];
+  bool sound[2];
+  int levels;
+  __device__ __forceinline__ void load(const PackedArgs& p) {
+    const int lane = threadIdx.x & 31;
+    levels = 0;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int s = lane + 32 * e;
+      first[e] = n[e] = other_first[e] = other_n[e] = 0;
+      sound[e] = true;
+      if (s < p.S) {
+        sound[e] = packed_range(p.cu_q, s, p.Nq, &first[e], &n[e]);
+        sound[e] &= packed_range(p.cu_k, s, p.Nk, &other_first[e], &other_n[e]);
+      }
+      pairs[e] = (n[e] + 2 * p.tokens - 1) / (2 * p.tokens);
+      base[e] = max(0, other_n[e] - n[e]) / (2 * p.tokens);
+      levels = max(levels, base[e] + pairs[e]);
+    }
+    levels = __reduce_max_sync(0xffffffffu, levels);
+  }
+  __device__ __forceinline__ int above(int level) const {  // pairs at this level or over it
+    int c = 0;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) c += max(0, min(pairs[e], base[e] + pairs[e] - level));
+    return __reduce_add_sync(0xffffffffu, c);
+  }
+  __device__ __forceinline__ bool find(int64_t idx, PackedTile* t) const {
+    if (idx >= above(0)) return false;
+    int lo = 0, hi = levels;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (idx < above(mid)) lo = mid;
+      else hi = mid;
+    }
+    int rank = static_cast<int>(idx) - above(lo + 1);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const bool here = lo >= base[e] && lo < base[e] + pairs[e];
+      const unsigned mask = __ballot_sync(0xffffffffu, here);
+      const unsigned below = mask & ((1u << (threadIdx.x & 31)) - 1u);
+      const unsigned owner = __ballot_sync(0xffffffffu, here && __popc(below) == rank);
+      if (owner) {
+        const int l = __ffs(owner) - 1;
+        t->tile = lo - __shfl_sync(0xffffffffu, base[e], l);
+        t->first = __shfl_sync(0xffffffffu, first[e], l);
+        t->n = __shfl_sync(0xffffffffu, n[e], l);
+        t->other_first = __shfl_sync(0xffffffffu, other_first[e], l);
+        t->other_n = __shfl_sync(0xffffffffu, other_n[e], l);
+        t->sound = __shfl_sync(0xffffffffu, sound[e] ? 1 : 0, l) != 0;
+        return true;
+      }
+      rank -= __popc(mask);
+    }
+    return false;
+  }
+};
+
+// The item of this CTA's `turn`-th turn, back and forth over the CTAs (items get smaller: always
+// the same order would give the first CTA the largest of every turn).  All lanes of a warp
+// together; false past the last item.
+__device__ __forceinline__ bool packed_item(const PackedArgs& p, const PackedOrder& order, int64_t turn, PackedItem* w) {
   const int64_t item = turn * gridDim.x + ((turn & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+  if (item >= p.items) return false;
   const int per = p.Hkv * p.n_splits;
   const int64_t at = item / per;
   const int rest = static_cast<int>(item - at * per);
   w->kvh = rest / p.n_splits;
   w->split = rest - w->kvh * p.n_splits;
-  int seq, tile;
-  if (!packed_tile(p.cu_q, p.S, p.Nq, 2 * p.tokens, at, &seq, &tile)) return false;
-  bool sound = packed_range(p.cu_q, seq, p.Nq, &w->q_first, &w->lq);
-  sound &= packed_range(p.cu_k, seq, p.Nk, &w->k_first, &w->lk);
-  if (!sound && threadIdx.x == 0) report(p.status, LINATTN_DEV_BAD_ID);
-  // the last tokens of a sequence see the most keys: they come first
-  tile = (w->lq + 2 * p.tokens - 1) / (2 * p.tokens) - 1 - tile;
-  w->t0 = tile * 2 * p.tokens;
+  PackedTile t;
+  if (p.S <= 64) {
+    if (!order.find(at, &t)) return false;
+  } else {  // sequence after sequence, each from its end
+    if (!packed_tile(p.cu_q, p.cu_k, p.S, p.Nq, p.Nk, 2 * p.tokens, at, &t)) return false;
+    t.tile = (t.n + 2 * p.tokens - 1) / (2 * p.tokens) - 1 - t.tile;
+  }
+  if (!t.sound && (threadIdx.x & 31) == 0) report(p.status, LINATTN_DEV_BAD_ID);
+  w->q_first = t.first;
+  w->lq = t.n;
+  w->k_first = t.other_first;
+  w->lk = t.other_n;
+  w->t0 = t.tile * 2 * p.tokens;
   w->shift = w->lk - w->lq;  // token t reads keys up to t + shift
   int nt[2];
 #pragma unroll
@@ -128,12 +202,19 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
   uint8_t* sk = sq + 2 * TILE;
   uint8_t* sv_ring = sk + KS * TILE;
   __shared__ __align__(8) uint64_t q_full[2], q_empty[2], k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], v_ragged,
-      s_full[2], p_full[2][2], pv_done[2], last;
+      s_full[2], p_full[2][2], pv_done[2], i_full[PA_ITEMS], i_empty[PA_ITEMS], last;
+  __shared__ PackedItem items[PA_ITEMS];
   __shared__ uint32_t tmem_sh;
   __shared__ int dead;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int boxb = p.tokens * p.G * 128;
+  PackedItem ahead;
+  PackedOrder order;
+  if (warp == 3) {
+    if (p.S <= 64) order.load(p);
+    ahead.more = packed_item(p, order, 0, &ahead) ? 1 : 0;
+  }
   if (tid == 0) {
     for (int s = 0; s < KS; ++s) {
       mbar_init(&k_full[s], 1);
@@ -151,6 +232,10 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       mbar_init(&p_full[s][1], 128);
       mbar_init(&pv_done[s], 1);
     }
+    for (int s = 0; s < PA_ITEMS; ++s) {
+      mbar_init(&i_full[s], 1);
+      mbar_init(&i_empty[s], PA_THREADS / 32 - 1);
+    }
     mbar_init(&v_ragged, 1);
     mbar_init(&last, 1);
     dead = 0;
@@ -163,16 +248,28 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // the item of a turn, and its slot's return
+  auto take = [&](int turn, bool* ok) -> const PackedItem* {
+    const int slot = turn % PA_ITEMS;
+    *ok = *ok && warp_wait(&i_full[slot], static_cast<uint32_t>((turn / PA_ITEMS) & 1));
+    return *ok && items[slot].more ? &items[slot] : nullptr;
+  };
+  auto give_back = [&](int turn) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&i_empty[turn % PA_ITEMS]);
+  };
   // columns [128 i, 128 i + 128): S / P of row tile i; [256 + 128 i, ...): O of row tile i
   const uint32_t tmem = tmem_sh;
-  PackedItem w;
 
   if (warp < 4) {
     regs_dec<PA_REGS_LOW>();
     if (warp == 0) {
       int kc = 0, vc = 0, rc = 0, qc[2] = {0, 0};  // loads so far: K, V and ragged V tiles, Q of each row tile
       bool ok = true, ragged_last = false;
-      for (int64_t turn = 0; ok && packed_item(p, turn, &w); ++turn) {
+      for (int turn = 0;; ++turn) {
+        const PackedItem* item = take(turn, &ok);
+        if (!item) break;
+        const PackedItem& w = *item;
         if (lane == 0) {
           auto load_q = [&](int i) {
             if (qc[i] > 0) ok = ok && mbar_wait_bounded(&q_empty[i], static_cast<uint32_t>((qc[i] - 1) & 1));
@@ -217,6 +314,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           if (dead) ok = false;
         }
         ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+        give_back(turn);
       }
       if (!ok && lane == 0) {  // the copies in flight land before the CTA gives up its shared memory
         dead = 1;
@@ -235,7 +333,11 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       const uint64_t q_desc = umma_desc(smem_u32(sq), 16, 1024), k_desc = umma_desc(smem_u32(sk), 16, 1024),
                      v_desc = umma_desc(smem_u32(sv_ring), 16384, 1024);
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-      for (int64_t turn = 0; ok && packed_item(p, turn, &w); ++turn) {
+      for (int turn = 0;; ++turn) {
+        const PackedItem* item = take(turn, &ok);
+        if (!item) break;
+        const PackedItem w = *item;
+        give_back(turn);
         if (w.n > 0) {
           auto scores = [&](int i, int j) {  // S_i of the item's key tile j
             const uint64_t a0 = q_desc + i * (TILE >> 4), b0 = k_desc + ((kc + j) % KS) * (TILE >> 4);
@@ -310,7 +412,10 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     } else if (warp == 2) {
       int vc = 0, rc = 0;
       bool ok = true;
-      for (int64_t turn = 0; ok && packed_item(p, turn, &w); ++turn) {
+      for (int turn = 0;; ++turn) {
+        const PackedItem* item = take(turn, &ok);
+        if (!item) break;
+        const PackedItem& w = *item;
         if (w.ragged >= 0) {
           ok = __all_sync(0xffffffffu, mbar_wait_bounded(&v_ragged, static_cast<uint32_t>(rc++ & 1)));
           if (ok) {
@@ -326,6 +431,23 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           }
         }
         vc += w.n;
+        give_back(turn);
+      }
+    } else {
+      for (int turn = 0;; ++turn) {
+        if (turn > 0) ahead.more = packed_item(p, order, turn, &ahead) ? 1 : 0;
+        if (turn >= PA_ITEMS && !warp_wait(&i_empty[turn % PA_ITEMS], static_cast<uint32_t>((turn / PA_ITEMS - 1) & 1))) {
+          if (lane == 0) {
+            report(p.status, LINATTN_DEV_TIMEOUT);
+            dead = 1;
+          }
+          break;
+        }
+        if (lane == 0) {
+          items[turn % PA_ITEMS] = ahead;
+          mbar_arrive(&i_full[turn % PA_ITEMS]);
+        }
+        if (!ahead.more) break;
       }
     }
   } else {
@@ -338,7 +460,10 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     const uint64_t sl2 = pack_f2(sl, sl);
     int sc = 0;  // score tiles so far
     bool ok = true;
-    for (int64_t turn = 0; ok && packed_item(p, turn, &w); ++turn) {
+    for (int turn = 0;; ++turn) {
+      const PackedItem* item = take(turn, &ok);
+      if (!item) break;
+      const PackedItem& w = *item;
       const int ni = i ? w.n1 : w.n0, t = w.t0 + i * p.tokens + rt;
       const bool row_ok = rt < p.tokens && t < w.lq;
       const int klim = (!row_ok ? 0 : p.causal ? max(0, min(w.lk, t + w.shift + 1)) : w.lk) - w.j0 * 128;  // keys this row reads
@@ -392,32 +517,29 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         const uint64_t neg2 = pack_f2(neg, neg);
         uint64_t sum[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {  // keys [64 h, 64 h + 64)
-          uint32_t pk[32];
+        for (int h = 0; h < 4; ++h) {  // keys [32 h, 32 h + 32)
+          uint32_t pk[16];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const int c = h * 64 + 2 * e;
+          for (int e = 0; e < 16; ++e) {
             const float2 x = unpack_f2(
-                fma_f2(pack_f2(__uint_as_float(sv[c >> 5][c & 31]), __uint_as_float(sv[c >> 5][(c & 31) + 1])), sl2, neg2));
+                fma_f2(pack_f2(__uint_as_float(sv[h][2 * e]), __uint_as_float(sv[h][2 * e + 1])), sl2, neg2));
             const float y0 = ex2_approx(x.x), y1 = ex2_approx(x.y);
             pk[e] = M::pack(y0, y1);
             sum[e & 3] = add_f2(sum[e & 3], pack_f2(y0, y1));
           }
-          tmem_st32(s_addr + h * 32, pk);
-          tmem_wait_st();
-          tc_fence_before();
-          mbar_arrive(&p_full[i][h]);
+          tmem_st16(s_addr + h * 16, pk);
+          if (h & 1) {
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(&p_full[i][h >> 1]);
+          }
         }
         const float2 ts = unpack_f2(add_f2(add_f2(sum[0], sum[1]), add_f2(sum[2], sum[3])));
         l += ts.x + ts.y;
       }
       if (ok && ni > 0)
         ok = __all_sync(0xffffffffu, mbar_wait_bounded(&pv_done[i], static_cast<uint32_t>((sc - 1) & 1)));
-      if (!ok) {
-        report(p.status, LINATTN_DEV_TIMEOUT);
-        dead = 1;
-        break;
-      }
+      if (!ok) break;
       tc_fence_after();
       const float inv = l != 0.f ? 1.f / l : 0.f;
       const float lse = l != 0.f ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
@@ -463,6 +585,11 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         }
       }
       tc_fence_before();  // the next item's first P V overwrites O after this warp's next P
+      give_back(turn);
+    }
+    if (!ok) {
+      report(p.status, LINATTN_DEV_TIMEOUT);
+      dead = 1;
     }
   }
   tc_fence_before();
@@ -567,7 +694,8 @@ extern "C" int linattn_packed_attention(const void* q, const void* k, const void
   const int64_t tiles = packed_tiles(N_q, p.G, S, max_q);
   if (Hkv * static_cast<int64_t>(n_splits) >= (int64_t(1) << 31) || n_splits > 1024) return packed_fail(LINATTN_EUNSUPPORTED, "too many tiles");
   if (tiles == 0) return LINATTN_OK;
-  const unsigned grid = static_cast<unsigned>(lmin(sm_count(), tiles * Hkv * n_splits));
+  p.items = tiles * Hkv * n_splits;
+  const unsigned grid = static_cast<unsigned>(lmin(sm_count(), p.items));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (dtype == LINATTN_BF16) e = D == 128 ? launch_packed<__nv_bfloat16, 128>(p, tq, tk, tv, grid, st) : launch_packed<__nv_bfloat16, 64>(p, tq, tk, tv, grid, st);

@@ -16,15 +16,24 @@ __device__ __forceinline__ bool packed_range(const int32_t* cu, int s, int64_t N
   return a == lo && b == hi;
 }
 
-// Sequence and tile of the `idx`-th tile of `rows` rows, sequence after sequence; all
-// lanes of a warp call it and get the same answer.  False past the last tile.
-__device__ __forceinline__ bool packed_tile(const int32_t* cu, int S, int64_t N, int rows, int64_t idx, int* seq,
-                                            int* tile) {
+// The sequence of the `idx`-th tile of `rows` rows of `cu`'s sequences, one after the other:
+// the tile among its sequence's, and the sequence's range in both `cu` and `other`.  All lanes
+// of a warp call it and get the same answer.  False past the last tile.
+struct PackedTile {
+  int tile, first, n, other_first, other_n;
+  bool sound;  // no offset had to be clamped
+};
+__device__ __forceinline__ bool packed_tile(const int32_t* cu, const int32_t* other, int S, int64_t N, int64_t N_other,
+                                            int rows, int64_t idx, PackedTile* t) {
   const int lane = threadIdx.x & 31;
   int64_t base = 0;
   for (int s0 = 0; s0 < S; s0 += 32) {
-    int first, n = 0;
-    if (s0 + lane < S) (void)packed_range(cu, s0 + lane, N, &first, &n);
+    int first = 0, n = 0, other_first = 0, other_n = 0;
+    bool sound = true;
+    if (s0 + lane < S) {  // both ranges in one round trip
+      sound = packed_range(cu, s0 + lane, N, &first, &n);
+      sound &= packed_range(other, s0 + lane, N_other, &other_first, &other_n);
+    }
     const int mine = (n + rows - 1) / rows;
     int incl = mine;
 #pragma unroll
@@ -35,10 +44,13 @@ __device__ __forceinline__ bool packed_tile(const int32_t* cu, int S, int64_t N,
     const int total = __shfl_sync(0xffffffffu, incl, 31);
     if (idx < base + total) {
       const int off = static_cast<int>(idx - base);
-      const unsigned owner = __ballot_sync(0xffffffffu, off >= incl - mine && off < incl);
-      const int l = __ffs(owner) - 1;
-      *seq = s0 + l;
-      *tile = off - __shfl_sync(0xffffffffu, incl - mine, l);
+      const int l = __ffs(__ballot_sync(0xffffffffu, off >= incl - mine && off < incl)) - 1;
+      t->tile = off - __shfl_sync(0xffffffffu, incl - mine, l);
+      t->first = __shfl_sync(0xffffffffu, first, l);
+      t->n = __shfl_sync(0xffffffffu, n, l);
+      t->other_first = __shfl_sync(0xffffffffu, other_first, l);
+      t->other_n = __shfl_sync(0xffffffffu, other_n, l);
+      t->sound = __shfl_sync(0xffffffffu, sound ? 1 : 0, l) != 0;
       return true;
     }
     base += total;
