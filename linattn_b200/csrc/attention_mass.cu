@@ -9,8 +9,9 @@
 // times the group's G heads, which one 3-D tensor-map box brings in as 128 rows.
 //
 // One CTA = 128 keys; warp 0 loads K once and Q tiles through a ring (TMA), warp 1 issues
-// tcgen05.mma into one of four TMEM buffers of 128 columns, two warpgroups take the tiles
-// in turn: a thread reads its key's 128 scores, then one packed FMA, two exponentials and
+// tcgen05.mma into one of four TMEM buffers of 128 columns, four warpgroups take the tiles
+// in turn (two, with the whole tile in registers, left the pipes idle waiting: 1520 us where four
+// take MASS_US for 16384 tokens, 32 / 8 heads, D = 128): a thread reads its key's 128 scores, then one packed FMA, two exponentials and
 // one packed add for two of them.  Keys with the most queries (the first of a sequence)
 // come first in the grid.
 // Bound: the exponentials (16 a clock and SM: 1024 clocks a tile, against 512 for its MMAs
@@ -41,8 +42,19 @@ struct MassArgs {
   int32_t* status;
 };
 
-constexpr int MT_THREADS = 384;
-constexpr int MT_BUFS = 4;   // TMEM score buffers of 128 columns
+constexpr int MT_GROUPS = 4;  // warpgroups on scores, each with a TMEM buffer of 128 columns
+constexpr int MT_THREADS = 128 * (1 + MT_GROUPS);
+constexpr int MT_BUFS = MT_GROUPS;
+
+#ifndef MT_POLY_BITS
+#define MT_POLY_BITS 0x52
+#endif
+constexpr uint32_t MT_POLY = MT_POLY_BITS;
+
+__device__ __forceinline__ uint64_t ex2_pair(uint64_t x) {
+  const float2 v = unpack_f2(x);
+  return pack_f2(ex2_approx(v.x), ex2_approx(v.y));
+}
 
 template <int D>
 struct MassSmem {
@@ -64,8 +76,8 @@ __global__ void __launch_bounds__(MT_THREADS, 1)
   __shared__ __align__(8) uint64_t k_full, q_full[ST], q_empty[ST], s_full[MT_BUFS], s_empty[MT_BUFS], last;
   __shared__ uint32_t tmem_sh;
   __shared__ int dead;
-  __shared__ __align__(16) float nl[2][2][128];  // [warpgroup][parity][column]: -lse2, or -inf for a column that does not count
-  __shared__ float part[128];
+  __shared__ __align__(16) float nl[MT_GROUPS][2][128];  // [warpgroup][parity][column]: -lse2, or -inf for a column that does not count
+  __shared__ float part[MT_GROUPS][128];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int kvh = blockIdx.x % p.Hkv;
@@ -183,71 +195,69 @@ __global__ void __launch_bounds__(MT_THREADS, 1)
     float total = 0.f;
     bool ok = true;
     float mine = column(wg);
-    for (int j = wg; j < n; j += 2) {
-      const int sb = j % MT_BUFS, par = (j >> 1) & 1;
+    for (int j = wg; j < n; j += MT_GROUPS) {
+      const int par = (j / MT_GROUPS) & 1;
       float* row = nl[wg][par];
       row[c] = mine;
       // every column with a query counts for every key of the tile (the rows of a tile that
       // hold none are zeros, and their -inf leaves nothing of them)
       const int pos0 = (qt0 + j) * p.tokens + shift;
-      int whole = ((mine != -INFINITY || !used) && (!p.causal || pos0 >= key0 + 127)) ? 1 : 0;
+      int whole = (((mine == mine && mine != -INFINITY) || !used) && (!p.causal || pos0 >= key0 + 127)) ? 1 : 0;
       asm volatile(
           "{\n\t.reg .pred a, b;\n\tsetp.ne.s32 a, %0, 0;\n\t"
           "barrier.cta.red.and.pred b, %1, 128, a;\n\tselp.s32 %0, 1, 0, b;\n\t}"
           : "+r"(whole)
           : "r"(1 + wg)
           : "memory");
-      mine = column(j + 2);
+      mine = column(j + MT_GROUPS);
       // a warp whose wait gave up goes on through the named barriers, without scores
-      if (ok) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_full[sb], static_cast<uint32_t>((j / MT_BUFS) & 1)));
+      ok = ok && warp_wait(&s_full[wg], static_cast<uint32_t>(par));
       if (!ok) continue;
       tc_fence_after();
-      uint32_t sv[4][32];
+      // columns of queries before this key, past the sequence or outside the window do not
+      // count, whatever their scores are
+      const int c_lo = p.causal ? (key - pos0) * p.G : 0;
+      uint64_t sum[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
-      for (int q = 0; q < 4; ++q) tmem_ld32(lane_addr + sb * 128 + q * 32, sv[q]);
-      tmem_wait_ld();
-      tc_fence_before();
-      mbar_arrive(&s_empty[sb]);
-      if (whole) {
-        uint64_t sum[4] = {0ull, 0ull, 0ull, 0ull};
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
+      for (int q = 0; q < 4; ++q) {
+        uint32_t sv[32];
+        tmem_ld32(lane_addr + wg * 128 + q * 32, sv);
+        tmem_wait_ld();
+        if (q == 3) {
+          tc_fence_before();
+          mbar_arrive(&s_empty[wg]);
+        }
+        if (whole) {  // MT_POLY of every 8 pairs of weights on the FMA pipe
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const float4 b = *reinterpret_cast<const float4*>(row + q * 32 + e * 4);
-            const float2 x = unpack_f2(fma_f2(
-                pack_f2(__uint_as_float(sv[q][4 * e]), __uint_as_float(sv[q][4 * e + 1])), c2, pack_f2(b.x, b.y)));
-            const float2 y = unpack_f2(fma_f2(
-                pack_f2(__uint_as_float(sv[q][4 * e + 2]), __uint_as_float(sv[q][4 * e + 3])), c2, pack_f2(b.z, b.w)));
-            sum[e & 1] = add_f2(sum[e & 1], pack_f2(ex2_approx(x.x), ex2_approx(x.y)));
-            sum[2 + (e & 1)] = add_f2(sum[2 + (e & 1)], pack_f2(ex2_approx(y.x), ex2_approx(y.y)));
+            const uint64_t x = fma_f2(pack_f2(__uint_as_float(sv[4 * e]), __uint_as_float(sv[4 * e + 1])), c2, pack_f2(b.x, b.y));
+            const uint64_t y = fma_f2(pack_f2(__uint_as_float(sv[4 * e + 2]), __uint_as_float(sv[4 * e + 3])), c2, pack_f2(b.z, b.w));
+            sum[e & 1] = add_f2(sum[e & 1], ((MT_POLY >> ((2 * e) & 7)) & 1) ? ex2_poly2(x) : ex2_pair(x));
+            sum[2 + (e & 1)] = add_f2(sum[2 + (e & 1)], ((MT_POLY >> ((2 * e + 1) & 7)) & 1) ? ex2_poly2(y) : ex2_pair(y));
           }
-        const float2 t = unpack_f2(add_f2(add_f2(sum[0], sum[1]), add_f2(sum[2], sum[3])));
-        total += t.x + t.y;
-      } else {
-        // columns of queries before this key, past the sequence or outside the window do not
-        // count, whatever their scores are
-        const int c_lo = p.causal ? (key - pos0) * p.G : 0;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        } else {
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const float b = row[q * 32 + e];
-            const float x = fmaf(__uint_as_float(sv[q][e]), p.scale_log2, b);
-            sum[e & 3] += (q * 32 + e >= c_lo && b != -INFINITY) ? ex2_approx(x) : 0.f;
+          for (int e = 0; e < 32; e += 2) {
+            const float b0 = row[q * 32 + e], b1 = row[q * 32 + e + 1];
+            const bool in0 = q * 32 + e >= c_lo && b0 != -INFINITY, in1 = q * 32 + e + 1 >= c_lo && b1 != -INFINITY;
+            const float x0 = fmaf(__uint_as_float(sv[e]), p.scale_log2, b0), x1 = fmaf(__uint_as_float(sv[e + 1]), p.scale_log2, b1);
+            sum[(e >> 1) & 3] = add_f2(sum[(e >> 1) & 3], pack_f2(in0 ? ex2_approx(x0) : 0.f, in1 ? ex2_approx(x1) : 0.f));
           }
-        total += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        }
       }
+      const float2 t = unpack_f2(add_f2(add_f2(sum[0], sum[1]), add_f2(sum[2], sum[3])));
+      total += t.x + t.y;
     }
     if (!ok) {
       report(p.status, LINATTN_DEV_TIMEOUT);
       dead = 1;
     }
-    if (wg == 1) part[c] = total;
-    asm volatile("barrier.cta.sync 3, 256;" ::: "memory");
+    part[wg][c] = total;
+    asm volatile("barrier.cta.sync 8, 512;" ::: "memory");
     if (wg == 0 && key < lk)
-      p.mass[blockIdx.y * p.split_stride + kvh * p.mass_stride + k_first + key] = total + part[c];
+      p.mass[blockIdx.y * p.split_stride + kvh * p.mass_stride + k_first + key] =
+          (part[0][c] + part[1][c]) + (part[2][c] + part[3][c]);
   }
   tc_fence_before();
   __syncthreads();
