@@ -8,12 +8,14 @@
 // no reduction across threads, no atomics, a fixed order.  The columns are 128 / G tokens
 // times the group's G heads, which one 3-D tensor-map box brings in as 128 rows.
 //
-// One CTA = 128 keys; warp 0 loads K once and Q tiles through a ring (TMA), warp 1 issues
-// tcgen05.mma into one of four TMEM buffers of 128 columns, four warpgroups take the tiles
-// in turn (two, with the whole tile in registers, left the pipes idle waiting: 1520 us where four
-// take MASS_US for 16384 tokens, 32 / 8 heads, D = 128): a thread reads its key's 128 scores, then one packed FMA, two exponentials and
-// one packed add for two of them.  Keys with the most queries (the first of a sequence)
-// come first in the grid.
+// One CTA = 512 keys, four tiles of 128 that share every Q tile; warp 0 loads K once and Q
+// tiles through a ring (TMA), warp 1 issues tcgen05.mma, a tile of keys to each of four TMEM
+// buffers of 128 columns, and each buffer has a warpgroup: a thread reads its key's 128 scores,
+// then one packed FMA, two exponentials and one packed add for two of them.  (Two warpgroups
+// with a whole tile in registers left the pipes idle, 1570 us where four took 1290; with one
+// key tile to a CTA and its Q tiles dealt to the warpgroups, a short window paid a CTA's start
+// and end for every 128 keys.)  Keys with the most queries (the first of a sequence) come first
+// in the grid.
 // Bound: the exponentials (16 a clock and SM: 1024 clocks a tile, against 512 for its MMAs
 // at D = 128).
 #include <cstdio>
@@ -44,7 +46,7 @@ struct MassArgs {
 
 constexpr int MT_GROUPS = 4;  // warpgroups on scores, each with a TMEM buffer of 128 columns
 constexpr int MT_THREADS = 128 * (1 + MT_GROUPS);
-constexpr int MT_BUFS = MT_GROUPS;
+constexpr int MT_KEYS = 128 * MT_GROUPS;  // keys of a CTA
 
 #ifndef MT_POLY_BITS
 #define MT_POLY_BITS 0x52
@@ -59,8 +61,8 @@ __device__ __forceinline__ uint64_t ex2_pair(uint64_t x) {
 template <int D>
 struct MassSmem {
   static constexpr int TILE = 128 * D * 2;
-  static constexpr int STAGES = D == 128 ? 5 : 8;
-  static constexpr int BYTES = 1024 + TILE * (1 + STAGES);
+  static constexpr int STAGES = D == 128 ? 2 : 6;
+  static constexpr int BYTES = 1024 + TILE * (MT_GROUPS + STAGES);
 };
 
 template <typename T, int D>
@@ -72,20 +74,21 @@ __global__ void __launch_bounds__(MT_THREADS, 1)
   constexpr uint32_t IDESC = umma_idesc(std::is_same<T, __nv_bfloat16>::value ? 1 : 0, 128, 128, 0);
   extern __shared__ __align__(128) uint8_t msmem_raw[];
   uint8_t* sk = msmem_raw + ((1024 - (smem_u32(msmem_raw) & 1023)) & 1023);
-  uint8_t* sq = sk + SM::TILE;
-  __shared__ __align__(8) uint64_t k_full, q_full[ST], q_empty[ST], s_full[MT_BUFS], s_empty[MT_BUFS], last;
+  uint8_t* sq = sk + MT_GROUPS * SM::TILE;
+  __shared__ __align__(8) uint64_t k_full[MT_GROUPS], q_full[ST], q_empty[ST], s_full[MT_GROUPS], s_empty[MT_GROUPS], last;
   __shared__ uint32_t tmem_sh;
   __shared__ int dead;
   __shared__ __align__(16) float nl[MT_GROUPS][2][128];  // [warpgroup][parity][column]: -lse2, or -inf for a column that does not count
-  __shared__ float part[MT_GROUPS][128];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int kvh = blockIdx.x % p.Hkv;
+  // the parts of the keys with the most queries come first
+  const int split = blockIdx.x % p.n_splits, kvh = blockIdx.x / p.n_splits % p.Hkv;
   PackedTile tl;
-  if (!packed_tile(p.cu_k, p.cu_q, p.S, p.Nk, p.Nq, 128, blockIdx.x / p.Hkv, &tl)) return;
+  if (!packed_tile(p.cu_k, p.cu_q, p.S, p.Nk, p.Nq, MT_KEYS, blockIdx.x / p.n_splits / p.Hkv, &tl)) return;
   if (!tl.sound && tid == 0) report(p.status, LINATTN_DEV_BAD_ID);
   const int k_first = tl.first, lk = tl.n, q_first = tl.other_first, lq = tl.other_n;
-  const int key0 = tl.tile * 128, shift = lk - lq;  // query i stands at position i + shift
+  const int key0 = tl.tile * MT_KEYS, shift = lk - lq;  // query i stands at position i + shift
+  const int key_tiles = min(MT_GROUPS, (lk - key0 + 127) >> 7);
   // query tiles that read these keys, and this split's share of them
   const int w_lo = p.window > 0 && p.window < lq ? lq - static_cast<int>(p.window) : 0;
   const int q_lo = max(w_lo, p.causal ? key0 - shift : 0);
@@ -93,20 +96,25 @@ __global__ void __launch_bounds__(MT_THREADS, 1)
   int n = max(0, (lq + p.tokens - 1) / p.tokens - qt0);
   if (q_lo >= lq) n = 0;
   if (p.n_splits > 1) {
-    const int share = (n + p.n_splits - 1) / p.n_splits, at = min(n, static_cast<int>(blockIdx.y) * share);
+    const int share = (n + p.n_splits - 1) / p.n_splits, at = min(n, split * share);
     qt0 += at;
     n = min(n - at, share);
   }
+  // the first of these tiles that key tile x takes part in (a later key has fewer queries)
+  auto begins = [&](int x) {
+    const int first = max(w_lo, p.causal ? key0 + 128 * x - shift : 0);
+    return x < key_tiles && first < lq ? max(0, first / p.tokens - qt0) : n;
+  };
   const int boxb = p.tokens * p.G * 128;  // bytes of one 64-channel box of queries
 
   if (tid == 0) {
-    mbar_init(&k_full, 1);
     mbar_init(&last, 1);
     for (int s = 0; s < ST; ++s) {
       mbar_init(&q_full[s], 1);
       mbar_init(&q_empty[s], 1);
     }
-    for (int s = 0; s < MT_BUFS; ++s) {
+    for (int s = 0; s < MT_GROUPS; ++s) {
+      mbar_init(&k_full[s], 1);
       mbar_init(&s_full[s], 1);
       mbar_init(&s_empty[s], 128);
     }
@@ -131,8 +139,12 @@ __global__ void __launch_bounds__(MT_THREADS, 1)
 
   if (warp == 0) {
     if (lane == 0 && n > 0) {
-      mbar_arrive_expect_tx(&k_full, SM::TILE);
-      for (int c = 0; c < HALVES; ++c) tma_load_3d(sk + c * 16384, &tmk, 64 * c, kvh, k_first + key0, &k_full);
+      auto load_k = [&](int x) {
+        mbar_arrive_expect_tx(&k_full[x], SM::TILE);
+        for (int c = 0; c < HALVES; ++c)
+          tma_load_3d(sk + x * SM::TILE + c * 16384, &tmk, 64 * c, kvh, k_first + key0 + 128 * x, &k_full[x]);
+      };
+      load_k(0);
       int issued = 0;
       for (int j = 0; j < n; ++j) {
         const int st = j % ST;
@@ -146,32 +158,45 @@ __global__ void __launch_bounds__(MT_THREADS, 1)
         for (int c = 0; c < HALVES; ++c)
           tma_load_3d(sq + st * SM::TILE + c * 16384, &tmq, 64 * c, kvh * p.G, q_first + (qt0 + j) * p.tokens, &q_full[st]);
         issued = j + 1;
+        if (j == 0)
+          for (int x = 1; x < key_tiles; ++x) load_k(x);
       }
-      if (dead)  // the copies in flight land before the CTA gives up its shared memory
+      if (dead) {  // the copies in flight land before the CTA gives up its shared memory
+        for (int x = 0; x < (issued > 0 ? key_tiles : 1); ++x) (void)mbar_wait_bounded(&k_full[x], 0, 200000000ull);
         for (int j = issued > ST ? issued - ST : 0; j < issued; ++j)
           (void)mbar_wait_bounded(&q_full[j % ST], static_cast<uint32_t>((j / ST) & 1), 200000000ull);
+      }
     }
   } else if (warp == 1) {
     if (n > 0) {
-      bool ok = warp_wait(&k_full, 0);
+      bool ok = true;
       const uint64_t k_desc = umma_desc(smem_u32(sk), 16, 1024), q_desc = umma_desc(smem_u32(sq), 16, 1024);
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-      for (int j = 0; ok && j < n; ++j) {
-        const int st = j % ST, sb = j % MT_BUFS;
-        ok = warp_wait(&q_full[st], static_cast<uint32_t>((j / ST) & 1));
-        if (ok && j >= MT_BUFS) ok = warp_wait(&s_empty[sb], static_cast<uint32_t>((j / MT_BUFS - 1) & 1));
-        if (!ok) break;
-        tc_fence_after();
-        const uint64_t qd = q_desc + st * (SM::TILE >> 4);
-        if (elect_lane()) {
+      int from[MT_GROUPS];
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = ((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;
-            umma_f16(tm + sb * 128, k_desc + off, qd + off, IDESC, kk > 0 ? 1u : 0u);
+      for (int x = 0; x < MT_GROUPS; ++x) from[x] = begins(x);
+      for (int j = 0; ok && j < n; ++j) {
+        const int st = j % ST;
+        ok = warp_wait(&q_full[st], static_cast<uint32_t>((j / ST) & 1));
+        const uint64_t qd = q_desc + st * (SM::TILE >> 4);
+#pragma unroll
+        for (int x = 0; x < MT_GROUPS; ++x) {
+          if (!ok || j < from[x]) continue;
+          const int round = j - from[x];  // of this buffer
+          if (round == 0) ok = warp_wait(&k_full[x], 0);
+          else ok = warp_wait(&s_empty[x], static_cast<uint32_t>((round - 1) & 1));
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_lane()) {
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t off = ((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;
+              umma_f16(tm + x * 128, k_desc + x * (SM::TILE >> 4) + off, qd + off, IDESC, kk > 0 ? 1u : 0u);
+            }
+            umma_commit(&s_full[x]);
           }
-          umma_commit(&s_full[sb]);
-          umma_commit(&q_empty[st]);
         }
+        if (ok && elect_lane()) umma_commit(&q_empty[st]);
       }
       if (!ok && lane == 0) {
         report(p.status, LINATTN_DEV_TIMEOUT);
@@ -181,7 +206,7 @@ __global__ void __launch_bounds__(MT_THREADS, 1)
   } else if (warp >= 4) {
     const int wg = (warp >> 2) - 1, c = tid & 127;
     const uint32_t lane_addr = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
-    const int key = key0 + c;  // this thread's key
+    const int tile0 = key0 + 128 * wg, key = tile0 + c;  // this warpgroup's keys, this thread's
     const int ct = c / p.G, cg = c - ct * p.G;
     const bool used = ct < p.tokens;
     // -lse2 of column c of tile j
@@ -194,22 +219,23 @@ __global__ void __launch_bounds__(MT_THREADS, 1)
     const uint64_t c2 = pack_f2(p.scale_log2, p.scale_log2);
     float total = 0.f;
     bool ok = true;
-    float mine = column(wg);
-    for (int j = wg; j < n; j += MT_GROUPS) {
-      const int par = (j / MT_GROUPS) & 1;
+    const int from = begins(wg);
+    float mine = column(from);
+    for (int j = from; j < n; ++j) {
+      const int par = (j - from) & 1;
       float* row = nl[wg][par];
       row[c] = mine;
       // every column with a query counts for every key of the tile (the rows of a tile that
       // hold none are zeros, and their -inf leaves nothing of them)
       const int pos0 = (qt0 + j) * p.tokens + shift;
-      int whole = (((mine == mine && mine != -INFINITY) || !used) && (!p.causal || pos0 >= key0 + 127)) ? 1 : 0;
+      int whole = (((mine == mine && mine != -INFINITY) || !used) && (!p.causal || pos0 >= tile0 + 127)) ? 1 : 0;
       asm volatile(
           "{\n\t.reg .pred a, b;\n\tsetp.ne.s32 a, %0, 0;\n\t"
           "barrier.cta.red.and.pred b, %1, 128, a;\n\tselp.s32 %0, 1, 0, b;\n\t}"
           : "+r"(whole)
           : "r"(1 + wg)
           : "memory");
-      mine = column(j + MT_GROUPS);
+      mine = column(j + 1);
       // a warp whose wait gave up goes on through the named barriers, without scores
       ok = ok && warp_wait(&s_full[wg], static_cast<uint32_t>(par));
       if (!ok) continue;
@@ -253,11 +279,7 @@ __global__ void __launch_bounds__(MT_THREADS, 1)
       report(p.status, LINATTN_DEV_TIMEOUT);
       dead = 1;
     }
-    part[wg][c] = total;
-    asm volatile("barrier.cta.sync 8, 512;" ::: "memory");
-    if (wg == 0 && key < lk)
-      p.mass[blockIdx.y * p.split_stride + kvh * p.mass_stride + k_first + key] =
-          (part[0][c] + part[1][c]) + (part[2][c] + part[3][c]);
+    if (key < lk) p.mass[split * p.split_stride + kvh * p.mass_stride + k_first + key] = total;
   }
   tc_fence_before();
   __syncthreads();
@@ -290,7 +312,7 @@ int mass_fail(int code, const char* what) {
 }
 
 template <typename T, int D>
-cudaError_t launch_mass(const MassArgs& p, const CUtensorMap& q, const CUtensorMap& k, dim3 grid, cudaStream_t st) {
+cudaError_t launch_mass(const MassArgs& p, const CUtensorMap& q, const CUtensorMap& k, unsigned grid, cudaStream_t st) {
   auto kern = attention_mass_kernel<T, D>;
   static int allowed[64] = {};
   const cudaError_t e = allow_smem(kern, MassSmem<D>::BYTES, allowed);
@@ -309,12 +331,14 @@ extern "C" int32_t linattn_attention_mass_splits(int64_t Hq, int64_t Hkv, int64_
                                                  int64_t window) {
   if (Hkv < 1 || Hq < Hkv || S < 1 || max_q < 1 || max_k < 1) return 1;
   const int64_t tokens = lmax(1, 128 / (Hq / Hkv));
-  const int64_t ctas = S * ((max_k + 127) / 128) * Hkv;
+  const int64_t ctas = S * ((max_k + MT_KEYS - 1) / MT_KEYS) * Hkv;
   const int64_t q_tiles = ((window > 0 ? lmin(window, max_q) : max_q) + tokens - 1) / tokens;
   const int64_t sms = sm_count();
-  // CTAs differ in length (causal), so a handful of rounds; at least 8 query tiles to a split
-  if (ctas >= 4 * sms) return 1;
-  return static_cast<int32_t>(lmax(1, lmin(lmin((4 * sms + ctas - 1) / ctas, q_tiles / 8), 64)));
+  // CTAs differ in length (causal), so a few rounds of the GPU (4096 tokens, D = 128: 2 / 3 / 4 /
+  // 6 rounds 91 / 92 / 96 / 103 us; 8192 tokens, D = 64: 315 / 299 / 301 / 304); at least 8
+  // query tiles to a split
+  if (ctas >= 3 * sms) return 1;
+  return static_cast<int32_t>(lmax(1, lmin(lmin((3 * sms + ctas - 1) / ctas, q_tiles / 8), 64)));
 }
 
 extern "C" int64_t linattn_attention_mass_workspace(int64_t N_k, int64_t Hkv, int32_t n_splits) {
@@ -364,10 +388,10 @@ extern "C" int linattn_attention_mass(const void* q, const void* k, int32_t dtyp
   p.split_stride = n_splits > 1 ? N_k * Hkv : 0;
   p.n_splits = n_splits;
   p.status = status;
-  const int64_t tiles = lmin(N_k / 128 + S, S * ((max_k + 127) / 128));
-  if (tiles * Hkv >= (int64_t(1) << 31) || n_splits > 65535) return mass_fail(LINATTN_EUNSUPPORTED, "too many tiles");
+  const int64_t tiles = lmin(N_k / MT_KEYS + S, S * ((max_k + MT_KEYS - 1) / MT_KEYS));
+  if (n_splits > 65535 || tiles * Hkv * n_splits >= (int64_t(1) << 31)) return mass_fail(LINATTN_EUNSUPPORTED, "too many tiles");
   if (tiles == 0) return LINATTN_OK;
-  const dim3 grid(static_cast<unsigned>(tiles * Hkv), static_cast<unsigned>(n_splits));
+  const unsigned grid = static_cast<unsigned>(tiles * Hkv * n_splits);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (dtype == LINATTN_BF16) e = D == 128 ? launch_mass<__nv_bfloat16, 128>(p, tq, tk, grid, st) : launch_mass<__nv_bfloat16, 64>(p, tq, tk, grid, st);
