@@ -26,7 +26,8 @@
 // the exponential unit (16 a clock), which the two row tiles overlap.  Taking 2 of 8 weights
 // from a polynomial on the FMA pipe instead was slower (2161 against 1798 us for 16384
 // tokens, 32 / 8 heads): the added instructions cost more issue slots and power than they save.
-// Few rows: the key range is cut into n_splits parts, merged by lse_combine.
+// Few rows: the key range is cut into n_splits parts, whose normalised outputs and lse a second
+// kernel merges.
 #include <cstdio>
 #include <type_traits>
 
@@ -603,6 +604,61 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
+// Merge of the parts of a key range: D / 4 lanes a row, four channels a lane, every part's
+// weight 2^(lse_s - max) computed by the lanes together (at most 32 parts, one to a lane).
+// Part by part in their order.  (The row-per-CTA merge of the decode path took about half of
+// the call at thousands of rows.)
+constexpr int PM_THREADS = 256;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(PM_THREADS) packed_merge_kernel(const PackedArgs p) {
+  using M = MmaOp<T>;
+  constexpr int LANES = D / 4;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int64_t rows = p.Nq * p.Hq;
+  const int64_t row = (static_cast<int64_t>(blockIdx.x) * PM_THREADS + threadIdx.x) / LANES;
+  const int lane = threadIdx.x & 31, in = threadIdx.x % LANES, base = lane - in;
+  const bool there = row < rows;
+  // lanes of a row take its parts in turn: with 16 lanes to a row, two rounds
+  float mine[32 / LANES], mx = -INFINITY;
+#pragma unroll
+  for (int e = 0; e < 32 / LANES; ++e) {
+    const int s = in + e * LANES;
+    mine[e] = there && s < p.n_splits ? p.part_lse[s * rows + row] : -INFINITY;
+    mx = fmaxf(mx, mine[e]);
+  }
+#pragma unroll
+  for (int o = LANES / 2; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  float sum = 0.f;
+#pragma unroll
+  for (int e = 0; e < 32 / LANES; ++e) {
+    // a part that reads nothing has no weight; one of NaN keeps it
+    mine[e] = mine[e] == -INFINITY ? 0.f : ex2_approx((mine[e] - mx) * 1.4426950408889634f);
+    sum += mine[e];
+  }
+#pragma unroll
+  for (int o = LANES / 2; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  const float4* src = reinterpret_cast<const float4*>(p.part_o) + row * LANES + in;
+#pragma unroll 4
+  for (int s = 0; s < p.n_splits; ++s) {
+    const float f = __shfl_sync(0xffffffffu, LANES == 32 || s < LANES ? mine[0] : mine[32 / LANES - 1], base + s % LANES);
+    if (there && f != 0.f) {
+      const float4 o = __ldg(src + static_cast<int64_t>(s) * rows * LANES);
+      acc.x += f * o.x;
+      acc.y += f * o.y;
+      acc.z += f * o.z;
+      acc.w += f * o.w;
+    }
+  }
+  if (!there) return;
+  const float inv = sum != 0.f ? 1.f / sum : 0.f;
+  const int64_t token = row / p.Hq;
+  *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + token * p.ot + (row - token * p.Hq) * p.oh + in * 4) =
+      make_uint2(M::pack(acc.x * inv, acc.y * inv), M::pack(acc.z * inv, acc.w * inv));
+  if (p.lse && in == 0) p.lse[row] = sum != 0.f ? mx + logf(sum) : -INFINITY;
+}
+
 int packed_fail(int code, const char* what) {
   char msg[256];
   snprintf(msg, sizeof(msg), "packed_attention: %s", what);
@@ -617,7 +673,19 @@ cudaError_t launch_packed(const PackedArgs& p, const CUtensorMap& q, const CUten
   const cudaError_t e = allow_smem(kern, PackedSmem<D>::BYTES, allowed);
   if (e != cudaSuccess) return e;
   kern<<<grid, PA_THREADS, PackedSmem<D>::BYTES, st>>>(p, q, k, v);
-  return cudaGetLastError();
+  const cudaError_t launched = cudaGetLastError();
+  if (launched != cudaSuccess || p.n_splits == 1) return launched;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  const int64_t threads = p.Nq * p.Hq * (D / 4);
+  cfg.gridDim = dim3(static_cast<unsigned>((threads + PM_THREADS - 1) / PM_THREADS));
+  cfg.blockDim = dim3(PM_THREADS);
+  cfg.stream = st;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, packed_merge_kernel<T, D>, p);
 }
 
 int64_t packed_tiles(int64_t N_q, int64_t G, int64_t S, int64_t max_q) {
@@ -692,7 +760,7 @@ extern "C" int linattn_packed_attention(const void* q, const void* k, const void
   p.part_lse = n_splits > 1 ? p.part_o + n_splits * N_q * Hq * D : nullptr;
   p.status = status;
   const int64_t tiles = packed_tiles(N_q, p.G, S, max_q);
-  if (Hkv * static_cast<int64_t>(n_splits) >= (int64_t(1) << 31) || n_splits > 1024) return packed_fail(LINATTN_EUNSUPPORTED, "too many tiles");
+  if (Hkv * static_cast<int64_t>(n_splits) >= (int64_t(1) << 31) || n_splits > 32) return packed_fail(LINATTN_EUNSUPPORTED, "too many tiles, or more than 32 splits");
   if (tiles == 0) return LINATTN_OK;
   p.items = tiles * Hkv * n_splits;
   const unsigned grid = static_cast<unsigned>(lmin(sm_count(), p.items));
@@ -700,10 +768,5 @@ extern "C" int linattn_packed_attention(const void* q, const void* k, const void
   cudaError_t e;
   if (dtype == LINATTN_BF16) e = D == 128 ? launch_packed<__nv_bfloat16, 128>(p, tq, tk, tv, grid, st) : launch_packed<__nv_bfloat16, 64>(p, tq, tk, tv, grid, st);
   else e = D == 128 ? launch_packed<__half, 128>(p, tq, tk, tv, grid, st) : launch_packed<__half, 64>(p, tq, tk, tv, grid, st);
-  if (e == cudaSuccess && n_splits > 1) {
-    // rows (token, head): the merge's innermost index is the head
-    const int64_t os[4] = {0, out_strides[0], out_strides[1], 1};
-    e = launch_lse_combine(p.part_o, p.part_lse, n_splits, N_q * Hq, D, out, dtype, N_q, Hq, os, lse, st);
-  }
   return e == cudaSuccess ? LINATTN_OK : packed_fail(LINATTN_ECUDA, cudaGetErrorString(e));
 }

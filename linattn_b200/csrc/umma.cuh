@@ -61,6 +61,13 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
       : LINATTN_R8(0), LINATTN_R8(8), LINATTN_R8(16), LINATTN_R8(24)
       : "r"(taddr));
 }
+// 16 consecutive ones
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : LINATTN_R8(0), LINATTN_R8(8)
+      : "r"(taddr));
+}
 #undef LINATTN_R8
 #define LINATTN_W8(i) "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3]), "r"(v[i + 4]), "r"(v[i + 5]), \
                       "r"(v[i + 6]), "r"(v[i + 7])
