@@ -127,15 +127,17 @@ __global__ void __launch_bounds__(APPEND_THREADS) heavy_append_kernel(const Heav
 // bins that the shared-memory atomics rarely meet).  The CTAs read one another's histograms
 // over distributed shared memory in two steps, the sums of 64 groups of bins and then the 32
 // bins of the group that holds the R-th: one remote load a thread and step, where reading
-// all 2048 bins of 8 CTAs took most of the time (16 ragged prompts, 8 heads: 247 us).  Then every
-// CTA knows how many kept tokens lie before its part and writes the positions and masses of
-// its own in order.  The rows are moved by a second kernel, spread evenly over the GPU: what is
+// all 2048 bins of 8 CTAs took most of the time (16 ragged prompts, 8 heads: 247 us).  Once a
+// bin holds 1024 candidates or fewer (mostly after the first digit) they are ranked against one
+// another instead.  Then every CTA knows how many kept tokens lie before its part and writes
+// the positions and masses of its own in order.  The rows are moved by a second kernel, spread evenly over the GPU: what is
 // kept is not spread evenly over the prompt (`recent` tokens all lie at its end).
 constexpr int SEL_THREADS = 512;
 constexpr int SEL_PER = 16;                        // tokens of a thread in one round
 constexpr int SEL_ROUND = SEL_THREADS * SEL_PER;   // tokens of a CTA in one round
 constexpr int SEL_BINS = 2048;
 constexpr int SEL_GROUPS = 64;                     // groups of 32 bins
+constexpr int SEL_LIST = 1024;                     // candidates that are ranked against one another at most
 
 struct HeavyLoadArgs {
   const float* mass;   // (H, N)
@@ -165,13 +167,19 @@ __device__ __forceinline__ uint32_t sum_from_above(uint32_t x) {
   return x;
 }
 
-__global__ void __launch_bounds__(SEL_THREADS) heavy_select_kernel(const HeavyCacheArgs c, const HeavyLoadArgs a) {
+__global__ void __launch_bounds__(SEL_THREADS, 2) heavy_select_kernel(const HeavyCacheArgs c, const HeavyLoadArgs a) {
   cg::cluster_group cluster = cg::this_cluster();
   __shared__ __align__(16) uint32_t hist[SEL_BINS];
   __shared__ uint32_t groups[SEL_GROUPS];   // sums of this CTA's bins
   __shared__ uint32_t totals[SEL_GROUPS];   // of all CTAs: groups, then the bins of one group
   __shared__ uint32_t scan[SEL_THREADS / 32 + 1];
-  __shared__ uint32_t picked[2];            // group or bin that holds the R-th largest, how many lie above it
+  __shared__ uint32_t picked[3];            // group or bin that holds the R-th largest, how many lie above it and in it
+  // the candidates of that bin, of this CTA and of all (key over complemented position: the
+  // larger word comes first), and those that stay
+  __shared__ uint64_t own_list[SEL_LIST], all_list[SEL_LIST];
+  __shared__ uint32_t counts[8];
+  __shared__ uint32_t stays[SEL_ROUND / 32];
+  __shared__ uint32_t own_n, kept_n;
   __shared__ uint32_t above[2];             // this CTA's candidates over the threshold / equal to it
   const int tid = threadIdx.x, lane = tid & 31, cl = static_cast<int>(cluster.num_blocks()),
             rank = static_cast<int>(cluster.block_rank());
@@ -215,6 +223,7 @@ __global__ void __launch_bounds__(SEL_THREADS) heavy_select_kernel(const HeavyCa
   };
   auto candidate = [&](int e) { return e < per && base + e < hi && base + e >= c_lo && base + e < c_hi; };
   if (rounds == 1) fetch(0);
+  int listed = -1;  // digits below this bit are left to the list
   if (want > 0) {
 #pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
@@ -276,12 +285,87 @@ __global__ void __launch_bounds__(SEL_THREADS) heavy_select_kernel(const HeavyCa
         if (over < left && left <= over + t) {
           picked[0] = group * 32 + lane;
           picked[1] = over;
+          picked[2] = t;
         }
       }
       cluster.sync();  // picked[] is there, and every CTA has read the histograms
       prefix = pass == 0 ? picked[0] : (prefix << (pass == 1 ? 11 : 10)) | picked[0];
       left -= picked[1];
+      if (rounds == 1 && picked[2] <= SEL_LIST) {
+        listed = shift;
+        break;
+      }
     }
+  }
+  if (listed >= 0) {
+    // Few enough candidates share the threshold's digits: every CTA gets all of them, and each of
+    // its own stays if fewer than `left` come before it (larger key, or equal and lower position).
+    if (tid == 0) own_n = 0;
+    for (int i = tid; i < SEL_ROUND / 32; i += SEL_THREADS) stays[i] = 0;
+    __syncthreads();
+    uint32_t keep = 0;  // one bit a token
+#pragma unroll
+    for (int e = 0; e < SEL_PER; ++e) {
+      const int i = base + e;
+      const uint32_t digits = mass_key(m[e]) >> listed;
+      if (candidate(e)) {
+        keep |= static_cast<uint32_t>(digits > prefix) << e;
+        if (digits == prefix) {
+          const uint32_t at = atomicAdd(&own_n, 1u);
+          own_list[at] = (static_cast<uint64_t>(mass_key(m[e])) << 32) | ~static_cast<uint32_t>(i);
+        }
+      } else {
+        keep |= static_cast<uint32_t>(e < per && i < hi) << e;
+      }
+    }
+    cluster.sync();
+    if (tid < cl) counts[tid] = *cluster.map_shared_rank(&own_n, tid);
+    __syncthreads();
+    uint32_t all = 0, mine_at = 0;
+    const int from = tid / (SEL_THREADS / cl);  // a group of threads copies one CTA's list
+    for (int r = 0; r < cl; ++r) {
+      if (r == from) mine_at = all;
+      all += counts[r];
+    }
+    for (uint32_t x = tid % (SEL_THREADS / cl); x < counts[from]; x += SEL_THREADS / cl)
+      all_list[mine_at + x] = cluster.map_shared_rank(own_list, from)[x];
+    __syncthreads();
+    for (uint32_t x0 = 0; x0 < own_n; x0 += SEL_THREADS / 8) {  // eight threads a candidate
+      const uint32_t x = x0 + tid / 8;
+      const uint64_t me = x < own_n ? own_list[x] : ~0ull;
+      uint32_t before = 0;
+#pragma unroll 4
+      for (uint32_t y = tid & 7; y < all; y += 8) before += all_list[y] > me;
+      before += __shfl_xor_sync(0xffffffffu, before, 1);
+      before += __shfl_xor_sync(0xffffffffu, before, 2);
+      before += __shfl_xor_sync(0xffffffffu, before, 4);
+      if (x < own_n && (tid & 7) == 0 && before < left) {
+        const uint32_t at = ~static_cast<uint32_t>(me) - static_cast<uint32_t>(lo);
+        atomicOr(&stays[at >> 5], 1u << (at & 31));
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < SEL_PER; ++e) {
+      const int i = tid * per + e;
+      if (e < per && base + e < hi) keep |= ((stays[i >> 5] >> (i & 31)) & 1u) << e;
+    }
+    uint32_t total;
+    uint32_t slot = block_exclusive_scan<SEL_THREADS>(__popc(keep), scan, &total);
+    if (tid == 0) kept_n = total;
+    cluster.sync();
+    for (int r = 0; r < rank; ++r) slot += *cluster.map_shared_rank(&kept_n, r);
+#pragma unroll
+    for (int e = 0; e < SEL_PER; ++e)
+      if ((keep >> e) & 1u) {
+        if (slot < static_cast<uint32_t>(c.M)) {
+          out_mass[slot] = m[e];
+          out_pos[slot] = base + e;
+        }
+        ++slot;
+      }
+    cluster.sync();  // kept_n is read by the other CTAs
+    return;
   }
   // prefix is the threshold key; `left` of its equals stay, the lowest ones
   const uint32_t thr = prefix, ties = left;
@@ -510,7 +594,15 @@ extern "C" int linattn_heavy_load(const linattn_heavy_t* cache, const void* k, c
   const int per = GATHER_THREADS / c.pieces * GATHER_ROWS;
   const unsigned gx = static_cast<unsigned>((lmin(c.M, N) + per - 1) / per);
   if (gx == 0) return LINATTN_OK;
-  heavy_gather_kernel<<<dim3(gx, c.H, static_cast<unsigned>(S)), GATHER_THREADS, 0, st>>>(
-      c, a, static_cast<const uint4*>(k), ks[0], ks[1], static_cast<const uint4*>(v), vs[0], vs[1]);
-  return cuda_result(cudaGetLastError());
+  // set up while the selection runs; the positions are read after its end
+  cudaLaunchConfig_t next = {};
+  next.gridDim = dim3(gx, c.H, static_cast<unsigned>(S));
+  next.blockDim = dim3(GATHER_THREADS);
+  next.stream = st;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  next.attrs = attr;
+  next.numAttrs = 1;
+  return cuda_result(cudaLaunchKernelEx(&next, heavy_gather_kernel, c, a, static_cast<const uint4*>(k), ks[0], ks[1],
+                                        static_cast<const uint4*>(v), vs[0], vs[1]));
 }
