@@ -535,7 +535,7 @@ int linattn_shard_merge(const float* scores, const int32_t* ids, int64_t R, int6
  * a kv head.  Strides in elements {token, head}, channels contiguous, rows and strides
  * multiples of 16 bytes.  lse (N_q, H_q) contiguous, or NULL.  max_q / max_k: at least the
  * longest sequence's query / key rows (they size the grid; rows beyond them are not
- * written).  n_splits > 1 cuts every key range and merges the parts through
+ * written).  n_splits > 1 (at most 32) cuts every key range and merges the parts through
  * `workspace` (linattn_packed_attention_workspace bytes, 16-byte aligned);
  * linattn_packed_attention_splits proposes a number.  Offsets that are not ascending or
  * leave the buffers are clamped and reported (LINATTN_DEV_BAD_ID).  No reference
@@ -582,7 +582,16 @@ typedef struct {
   int32_t* pos;
   int32_t* seen;
   int32_t dtype, batch, n_kv_heads, budget, head_dim, sinks, recent;
+  const void* maps; /* what linattn_heavy_maps wrote for this cache, or NULL */
 } linattn_heavy_t;
+
+/*
+ * Tensor maps of a cache's K and V (LINATTN_HEAVY_MAPS bytes of host memory) for
+ * linattn_heavy_attend, so that it need not encode them on every call.  They hold the
+ * addresses and sizes of k and v: write them again when those change.
+ */
+enum { LINATTN_HEAVY_MAPS = 256 };
+int linattn_heavy_maps(const linattn_heavy_t* cache, void* maps);
 
 /*
  * Packed prompts into the cache: sequence s of k, v (N, H_kv, head_dim) (strides {token,

@@ -54,8 +54,11 @@ class Heavy(ctypes.Structure):
     _fields_ = [
         ("k", c_vp), ("v", c_vp), ("mass", c_vp), ("pos", c_vp), ("seen", c_vp),
         ("dtype", c_i32), ("batch", c_i32), ("n_kv_heads", c_i32), ("budget", c_i32), ("head_dim", c_i32),
-        ("sinks", c_i32), ("recent", c_i32),
+        ("sinks", c_i32), ("recent", c_i32), ("maps", c_vp),
     ]
+
+
+HEAVY_MAPS = 256
 
 
 def rows_addressable(t: torch.Tensor, head_dim: int) -> int:
@@ -157,6 +160,7 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.linattn_attention_mass_splits.restype = c_i32
     lib.linattn_attention_mass_workspace.argtypes = [c_i64, c_i64, c_i32]
     lib.linattn_attention_mass_workspace.restype = c_i64
+    lib.linattn_heavy_maps.argtypes = [P(Heavy), c_vp]
     lib.linattn_heavy_load.argtypes = [P(Heavy), c_vp, c_vp, P(c_i64), P(c_i64), c_i64, c_vp, c_i64, c_vp, c_vp, c_i64,
                                        c_vp, c_vp]
     lib.linattn_heavy_append.argtypes = [P(Heavy), c_vp, c_vp, P(c_i64), P(c_i64), c_i64, c_vp, c_vp, c_vp]
@@ -164,7 +168,7 @@ def _declare(lib: ctypes.CDLL) -> None:
                                          c_vp, c_i64, c_vp, c_vp]
     lib.linattn_heavy_attend_workspace.argtypes = [c_i64] * 4
     lib.linattn_heavy_attend_workspace.restype = c_i64
-    for name in ("linattn_packed_attention", "linattn_attention_mass", "linattn_heavy_load", "linattn_heavy_append",
+    for name in ("linattn_packed_attention", "linattn_attention_mass", "linattn_heavy_maps", "linattn_heavy_load", "linattn_heavy_append",
                  "linattn_heavy_attend"):
         getattr(lib, name).restype = ctypes.c_int
     for name in ("linattn_read_bandwidth", "linattn_block_score_topk", "linattn_shard_merge", "linattn_quest_decode_candidates", "linattn_lse_combine_strided", "linattn_block_sparse_prefill", "linattn_prefill_v_to_f16", "linattn_block_mean", "linattn_csa2_pool_quant", "linattn_merge_block_lists", "linattn_token_attention", "linattn_indexer_scores", "linattn_row_topk", "linattn_page_bounds", "linattn_paged_page_bounds", "linattn_paged_append", "linattn_quest_scores", "linattn_page_topk",

@@ -20,6 +20,7 @@
 // that several CTAs share, the last to arrive merges their (o, m, l): the parts are added in
 // their order, whoever does it, so results do not depend on it.
 #include <cstdio>
+#include <cstring>
 #include <type_traits>
 
 #include "launchers.cuh"
@@ -666,33 +667,61 @@ extern "C" int64_t linattn_heavy_attend_workspace(int64_t batch, int64_t Hq, int
   return batch * Hkv * heads * budget * 4 + sm_count() * 2 * hn * (128 + 2) * 4 + 64;
 }
 
+namespace {
+
+bool attend_maps(const linattn_heavy_t* cache, CUtensorMap* tk, CUtensorMap* tv) {
+  const int64_t D = cache->head_dim, rows = static_cast<int64_t>(cache->batch) * cache->n_kv_heads * cache->budget;
+  const CUtensorMapDataType cu = cache->dtype == LINATTN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const int64_t dims[3] = {D, rows, 1}, strides[2] = {D * 2, rows * D * 2};
+  const int box[3] = {64, AT_BOX, 1};
+  return tensor_map_3d(tk, cache->k, cu, dims, strides, box) && tensor_map_3d(tv, cache->v, cu, dims, strides, box);
+}
+
+// what both entry points ask of a cache
+int attend_cache(const linattn_heavy_t* cache) {
+  if (!cache || !cache->k || !cache->v || !cache->mass || !cache->seen) return attend_fail(LINATTN_EINVAL, "NULL pointer");
+  if (cache->dtype != LINATTN_F16 && cache->dtype != LINATTN_BF16)
+    return attend_fail(LINATTN_EUNSUPPORTED, "f16 or bf16 caches");
+  if (cache->head_dim != 64 && cache->head_dim != 128) return attend_fail(LINATTN_EUNSUPPORTED, "head_dim must be 64 or 128");
+  if (cache->batch < 1 || cache->n_kv_heads < 1 || cache->budget < 1 || cache->budget > (1 << 24))
+    return attend_fail(LINATTN_EINVAL, "batch, n_kv_heads and budget must be > 0 (budget <= 2^24)");
+  if ((reinterpret_cast<uintptr_t>(cache->k) | reinterpret_cast<uintptr_t>(cache->v) | reinterpret_cast<uintptr_t>(cache->mass)) % 16)
+    return attend_fail(LINATTN_EINVAL, "K, V and mass must be 16-byte aligned");
+  if (static_cast<int64_t>(cache->batch) * cache->n_kv_heads * cache->budget >= (int64_t(1) << 31))
+    return attend_fail(LINATTN_EUNSUPPORTED, "too many slots for 32-bit TMA coordinates");
+  return LINATTN_OK;
+}
+
+}  // namespace
+
+extern "C" int linattn_heavy_maps(const linattn_heavy_t* cache, void* maps) {
+  if (const int rc = attend_cache(cache)) return rc;
+  if (!maps) return attend_fail(LINATTN_EINVAL, "NULL pointer");
+  static_assert(2 * sizeof(CUtensorMap) == LINATTN_HEAVY_MAPS, "two tensor maps");
+  CUtensorMap m[2];
+  if (!attend_maps(cache, &m[0], &m[1])) return attend_fail(LINATTN_ECUDA, "tensor map encoding failed");
+  memcpy(maps, m, sizeof(m));
+  return LINATTN_OK;
+}
+
 extern "C" int linattn_heavy_attend(const linattn_heavy_t* cache, const void* q, int64_t Hq, const int64_t* q_strides,
                                     float scale, int32_t accumulate, void* out, const int64_t* out_strides,
                                     int32_t* ticket, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream) {
-  if (!cache || !cache->k || !cache->v || !cache->mass || !cache->seen || !q || !out || !q_strides || !out_strides || !ticket)
-    return attend_fail(LINATTN_EINVAL, "NULL pointer");
-  if (cache->dtype != LINATTN_F16 && cache->dtype != LINATTN_BF16)
-    return attend_fail(LINATTN_EUNSUPPORTED, "f16 or bf16 caches");
+  if (const int rc = attend_cache(cache)) return rc;
+  if (!q || !out || !q_strides || !out_strides || !ticket) return attend_fail(LINATTN_EINVAL, "NULL pointer");
   const int64_t D = cache->head_dim;
-  if (D != 64 && D != 128) return attend_fail(LINATTN_EUNSUPPORTED, "head_dim must be 64 or 128");
-  if (cache->batch < 1 || cache->n_kv_heads < 1 || cache->budget < 1 || cache->budget > (1 << 24))
-    return attend_fail(LINATTN_EINVAL, "batch, n_kv_heads and budget must be > 0 (budget <= 2^24)");
   if (Hq < 1 || Hq % cache->n_kv_heads) return attend_fail(LINATTN_EINVAL, "H_q must be a multiple of H_kv");
   if (!(scale > 0.f) || scale > 1e30f) return attend_fail(LINATTN_EINVAL, "scale must be positive and finite");
-  if ((reinterpret_cast<uintptr_t>(cache->k) | reinterpret_cast<uintptr_t>(cache->v)) % 16 || reinterpret_cast<uintptr_t>(q) % 4 ||
-      q_strides[0] % 2 || q_strides[1] % 2)
-    return attend_fail(LINATTN_EINVAL, "K and V must be 16-byte aligned, q rows 4-byte aligned");
-  const int64_t units = static_cast<int64_t>(cache->batch) * cache->n_kv_heads, rows = units * cache->budget;
-  if (rows >= (int64_t(1) << 31)) return attend_fail(LINATTN_EUNSUPPORTED, "too many slots for 32-bit TMA coordinates");
+  if (reinterpret_cast<uintptr_t>(q) % 4 || q_strides[0] % 2 || q_strides[1] % 2)
+    return attend_fail(LINATTN_EINVAL, "q rows must be 4-byte aligned");
+  const int64_t units = static_cast<int64_t>(cache->batch) * cache->n_kv_heads;
   if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 ||
       workspace_bytes < linattn_heavy_attend_workspace(cache->batch, Hq, cache->n_kv_heads, cache->budget))
     return attend_fail(LINATTN_EINVAL, "workspace too small or not 16-byte aligned");
-  const CUtensorMapDataType cu = cache->dtype == LINATTN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  CUtensorMap tk, tv;
-  const int64_t dims[3] = {D, rows, 1}, strides[2] = {D * 2, rows * D * 2};
-  const int box[3] = {64, AT_BOX, 1};
-  if (!tensor_map_3d(&tk, cache->k, cu, dims, strides, box) || !tensor_map_3d(&tv, cache->v, cu, dims, strides, box))
-    return attend_fail(LINATTN_ECUDA, "tensor map encoding failed");
+  CUtensorMap m[2];
+  if (cache->maps) memcpy(m, cache->maps, sizeof(m));
+  else if (!attend_maps(cache, &m[0], &m[1])) return attend_fail(LINATTN_ECUDA, "tensor map encoding failed");
+  const CUtensorMap &tk = m[0], &tv = m[1];
   HeavyAttendArgs a;
   a.mass = cache->mass;
   a.seen = cache->seen;

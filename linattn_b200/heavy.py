@@ -19,7 +19,6 @@ order of its keys), ``pos`` says which token a slot holds.
 from __future__ import annotations
 
 import ctypes
-import functools
 import math
 from typing import Optional
 
@@ -66,6 +65,11 @@ class HeavyCache:
                              self.seen.data_ptr(), L.dtype_code(self.k), batch, n_kv_heads, budget, head_dim, sinks, recent)
         # what every call passes
         self._lib, self._ref, self._ticket_ptr = L.lib(), ctypes.byref(self._desc), self._ticket.data_ptr()
+        self._maps = ctypes.create_string_buffer(L.HEAVY_MAPS)
+        L.check(self._lib.linattn_heavy_maps(self._ref, self._maps))
+        self._desc.maps = ctypes.addressof(self._maps)
+        self._index = self.device.index
+        self._plans: dict = {}  # checked arguments of append and attend, by shapes, strides and types
         self._unit_ticket_ptr = self._unit_ticket.data_ptr()
         self._status_ptr = L.status_word(self.device).data_ptr()
         self._scale = 1.0 / math.sqrt(head_dim)
@@ -105,44 +109,75 @@ class HeavyCache:
         """Take ``(B, H_kv, T_new, D)`` keys / values, one token after the other: each fills the
         next empty slot or, in a full cache, replaces the slot of least mass (lowest slot on
         ties) outside the sinks and the last ``recent`` tokens (itself among them)."""
-        shape = k.shape
-        if len(shape) != 4 or shape[0] != self.batch or shape[1] != self.n_kv_heads or shape[3] != self.head_dim or v.shape != shape:
+        key = (k.shape, k.stride(), v.shape, v.stride(), k.dtype, v.dtype, k.get_device(), v.get_device())
+        plan = self._plans.get(key)
+        if plan is None:
+            plan = self._keep(key, self._plan_append(k, v))
+        if plan[0] is None or (k.data_ptr() | v.data_ptr()) & 15:  # rows off the 16-byte grid
+            return self.append(k.clone(memory_format=torch.contiguous_format), v.clone(memory_format=torch.contiguous_format))
+        L.check(self._lib.linattn_heavy_append(self._ref, k.data_ptr(), v.data_ptr(), plan[0], plan[1], plan[2],
+                                               self._ticket_ptr, self._status_ptr, L.raw_stream(self._index)))
+        if L.strict():
+            L.check_status(self.device)
+
+    def _keep(self, key, plan):
+        if len(self._plans) >= 256:
+            self._plans.clear()
+        self._plans[key] = plan
+        return plan
+
+    def _plan_append(self, k: torch.Tensor, v: torch.Tensor):
+        """(strides of k, of v, T_new); (None,) where the rows have to be copied first."""
+        shape = tuple(k.shape)
+        if len(shape) != 4 or shape[:2] != (self.batch, self.n_kv_heads) or shape[3] != self.head_dim or v.shape != k.shape:
             raise ValueError(f"k and v must be ({self.batch}, {self.n_kv_heads}, T_new, {self.head_dim})")
         if k.dtype != self.dtype or v.dtype != self.dtype:
             raise ValueError(f"k and v must be {self.dtype} as the cache")
-        dev = L.require_cuda(k, v, self.k)
-        k, v = _rows16(k), _rows16(v)
-        L.check(self._lib.linattn_heavy_append(
-            self._ref, k.data_ptr(), v.data_ptr(), L.strides3(k), L.strides3(v), shape[2], self._ticket_ptr, self._status_ptr,
-            L.raw_stream(dev.index)))
-        if L.strict():
-            L.check_status(dev)
+        L.require_cuda(k, v, self.k)
+        if not (_on_grid(k) and _on_grid(v)):
+            return (None,)
+        return L.strides3(k), L.strides3(v), shape[2]
 
     def attend(self, q: torch.Tensor, *, scale: Optional[float] = None, accumulate: bool = True,
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """``o (B, H_q, 1, D)`` of one query token per sequence over the slots in use; with
         ``accumulate`` each slot's mass grows by its weights, summed over its group's heads."""
         shape = q.shape
-        if len(shape) != 4 or shape[0] != self.batch or shape[1] % self.n_kv_heads or shape[1] < 1 or shape[2] != 1 or shape[3] != self.head_dim:
-            raise ValueError(f"q must be ({self.batch}, a multiple of {self.n_kv_heads}, 1, {self.head_dim}), got {tuple(shape)}")
+        key = (shape, q.stride(), q.dtype, q.get_device())
+        plan = self._plans.get(key)
+        if plan is None:
+            plan = self._keep(key, self._plan_attend(q))
+        hq, strides, dense, need = plan
+        if strides is None or q.data_ptr() & 15:  # rows off the 16-byte grid
+            return self.attend(q.clone(memory_format=torch.contiguous_format), scale=scale, accumulate=accumulate, out=out)
+        if out is None:
+            out, out_strides = torch.empty(shape, dtype=self.dtype, device=self.device), dense
+        else:
+            L.require_cuda(out, self.k)
+            if out.shape != shape or out.dtype != self.dtype or out.stride(3) != 1:
+                raise ValueError("out must have q's shape and dtype with contiguous channels")
+            out_strides = L.strides2(out)
+        if self._workspace is None or self._workspace.numel() < need:
+            self._workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
+        L.check(self._lib.linattn_heavy_attend(
+            self._ref, q.data_ptr(), hq, strides, self._scale if scale is None else float(scale), 1 if accumulate else 0,
+            out.data_ptr(), out_strides, self._unit_ticket_ptr, self._workspace.data_ptr(), need, self._status_ptr,
+            L.raw_stream(self._index)))
+        if L.strict():
+            L.check_status(self.device)
+        return out
+
+    def _plan_attend(self, q: torch.Tensor):
+        """(H_q, strides of q or None where the rows have to be copied first, of a new output, workspace bytes)."""
+        shape = tuple(q.shape)
+        if (len(shape) != 4 or shape[0] != self.batch or shape[1] < 1 or shape[1] % self.n_kv_heads
+                or shape[2:] != (1, self.head_dim)):
+            raise ValueError(f"q must be ({self.batch}, a multiple of {self.n_kv_heads}, 1, {self.head_dim}), got {shape}")
         if q.dtype != self.dtype:
             raise ValueError(f"q must be {self.dtype} as the cache")
-        dev = L.require_cuda(q, self.k, out)
-        q = _rows16(q)
-        if out is None:
-            out = torch.empty(shape, dtype=q.dtype, device=dev)
-        elif out.shape != shape or out.dtype != q.dtype or out.stride(3) != 1:
-            raise ValueError("out must have q's shape and dtype with contiguous channels")
-        need = _attend_bytes(self.batch, shape[1], self.n_kv_heads, self.budget)
-        if self._workspace is None or self._workspace.numel() < need:
-            self._workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-        L.check(self._lib.linattn_heavy_attend(
-            self._ref, q.data_ptr(), shape[1], L.strides2(q), self._scale if scale is None else float(scale), int(accumulate),
-            out.data_ptr(), L.strides2(out), self._unit_ticket_ptr, self._workspace.data_ptr(), need, self._status_ptr,
-            L.raw_stream(dev.index)))
-        if L.strict():
-            L.check_status(dev)
-        return out
+        L.require_cuda(q, self.k)
+        return (shape[1], L.strides2(q) if _on_grid(q) else None, L.i64_array((shape[1] * self.head_dim, self.head_dim)),
+                self._lib.linattn_heavy_attend_workspace(self.batch, shape[1], self.n_kv_heads, self.budget))
 
     def step(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: Optional[float] = None,
              out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -151,15 +186,12 @@ class HeavyCache:
         return self.attend(q, scale=scale, out=out)
 
 
-@functools.lru_cache(maxsize=1024)
-def _attend_bytes(batch: int, hq: int, hkv: int, budget: int) -> int:
-    return L.lib().linattn_heavy_attend_workspace(batch, hq, hkv, budget)
+def _on_grid(x: torch.Tensor) -> bool:
+    """Contiguous channels and strides of whole 16-byte pieces."""
+    *outer, last = x.stride()
+    return last == 1 and all(s & 7 == 0 for s in outer)
 
 
 def _rows16(x: torch.Tensor) -> torch.Tensor:
     """x with contiguous channels and rows on 16 bytes."""
-    *outer, last = x.stride()
-    bits = x.data_ptr() >> 1
-    for s in outer:
-        bits |= s
-    return x.contiguous() if last != 1 or bits & 7 else x
+    return x if _on_grid(x) and x.data_ptr() & 15 == 0 else x.clone(memory_format=torch.contiguous_format)

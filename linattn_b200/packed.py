@@ -29,7 +29,7 @@ def _rows(name: str, x: torch.Tensor) -> torch.Tensor:
         raise ValueError(f"{name} must be (tokens, heads, head_dim), got shape {tuple(x.shape)}")
     s0, s1, s2 = x.stride()
     if s2 != 1 or (s0 | s1) & 7 or s0 < 1 or s1 < 1 or x.data_ptr() & 15:
-        x = x.contiguous()
+        x = x.clone(memory_format=torch.contiguous_format)  # (contiguous() may hand back an unaligned view)
     return x
 
 

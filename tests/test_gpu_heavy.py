@@ -38,6 +38,8 @@ LOADS = [
     ([5000, 4097], 1000, 0, 1, 2, 64, torch.float16),
     ([700], 64, 4, 60, 1, 128, torch.bfloat16),      # nothing is left to choose
     ([900, 2], 257, 3, 200, 2, 64, torch.bfloat16),
+    ([70001], 300, 2, 30, 1, 64, torch.float16),     # more tokens than a CTA's registers hold
+    ([20000], 12000, 4, 4000, 2, 64, torch.bfloat16),
 ]
 
 
@@ -210,6 +212,49 @@ def test_attend(cuda, seen, budget, hq, hkv, d, dtype, accumulate):
         cache.attend(qs, scale=scale, accumulate=accumulate, out=wide[..., d:])
     side.synchronize()
     assert torch.equal(wide[..., d:], first) and (wide[..., :d] == 0).all()
+
+
+@pytest.mark.parametrize("batch,budget", [(70, 40), (33, 400), (3, 2000)])
+def test_attend_shares(cuda, batch, budget):
+    """Many short sequences to a CTA and many CTAs to a sequence, some of them empty."""
+    from linattn_b200 import HeavyCache
+
+    hq, hkv, d, dtype = 8, 4, 64, torch.bfloat16
+    g = torch.Generator().manual_seed(batch)
+    cache = HeavyCache(batch, hkv, d, budget, dtype=dtype)
+    cache.k.copy_(torch.randn(batch, hkv, budget, d, generator=g))
+    cache.v.copy_(torch.randn(batch, hkv, budget, d, generator=g))
+    cache.seen.copy_(torch.randint(0, 2 * budget, (batch,), generator=g) * (torch.rand(batch, generator=g) < 0.8))
+    q = torch.randn(batch, hq, 1, d, generator=g).to(dtype).cuda()
+    for _ in range(2):  # the arrival counts are back at zero
+        before = cache.mass.clone()
+        o = cache.attend(q)
+        _check_attend(cache, q, o, before, cache.mass, 1 / math.sqrt(d), True)
+
+
+def test_unaligned_rows(cuda):
+    """Rows off the 16-byte grid and channels that are not next to one another are copied first."""
+    from linattn_b200 import HeavyCache
+
+    b, h, d, dtype = 2, 2, 64, torch.float16
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn(3, b, h, 1, d, generator=g).to(dtype).cuda()
+    caches = [HeavyCache(b, h, d, 16, dtype=dtype) for _ in range(3)]
+
+    def odd(t):
+        base = torch.empty(t.numel() + 1, dtype=dtype, device="cuda")
+        base[1:] = t.flatten()
+        return base[1:].view(t.shape)
+
+    def across(t):
+        return t.transpose(2, 3).contiguous().transpose(2, 3)
+
+    outs = []
+    for c, f in zip(caches, (lambda t: t, odd, across)):
+        c.append(f(x[0]), f(x[1]))
+        outs.append(c.attend(f(x[2])))
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+    assert torch.equal(caches[0].k, caches[1].k) and torch.equal(caches[0].v, caches[2].v)
 
 
 def test_attend_nan_reaches_its_head_only(cuda):

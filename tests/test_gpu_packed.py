@@ -88,6 +88,8 @@ CASES = [
     ([50, 20, 300], [17, 0, 128], 8, 2, 128, torch.bfloat16, True),          # more queries than keys: empty rows
     ([100, 31], [260, 500], 8, 8, 64, torch.bfloat16, False),
     ([1100], [1100], 8, 2, 128, torch.bfloat16, True),
+    (list(range(40)), list(range(40)), 4, 2, 64, torch.bfloat16, True),                       # two sequences to a lane
+    ([3 * i % 50 for i in range(70)], [5 * i % 90 for i in range(70)], 2, 1, 64, torch.float16, True),  # more than 64
 ]
 
 

@@ -62,7 +62,7 @@ def test_packed_plans():
 
 def _heavy(**kw):
     a = dict(k=4096, v=4096, mass=4096, pos=4096, seen=4096, dtype=L.F16, batch=2, n_kv_heads=2, budget=64, head_dim=64,
-             sinks=1, recent=8)
+             sinks=1, recent=8, maps=None)
     a.update(kw)
     return L.Heavy(*a.values())
 
@@ -79,6 +79,8 @@ def test_heavy_cache_arguments(bad, rc):
 
 def test_heavy_calls():
     lib = L.lib()
+    assert lib.linattn_heavy_maps(_heavy(dtype=L.F32), P) == 2
+    assert lib.linattn_heavy_maps(_heavy(), None) == 1
     assert lib.linattn_heavy_append(_heavy(), None, P, I3, I3, 1, P, None, None) == 1
     assert lib.linattn_heavy_append(_heavy(), P, P, (L.c_i64 * 3)(4, 64, 64), I3, 1, P, None, None) == 1
     assert lib.linattn_heavy_append(_heavy(), P, P, I3, I3, -1, P, None, None) == 1
