@@ -48,10 +48,11 @@ constexpr int MT_GROUPS = 4;  // warpgroups on scores, each with a TMEM buffer o
 constexpr int MT_THREADS = 128 * (1 + MT_GROUPS);
 constexpr int MT_KEYS = 128 * MT_GROUPS;  // keys of a CTA
 
-#ifndef MT_POLY_BITS
-#define MT_POLY_BITS 0x52
-#endif
-constexpr uint32_t MT_POLY = MT_POLY_BITS;
+// Of every 8 pairs of weights, those computed on the FMA pipe (ex2_poly2: 2.7e-6 off, as the sums
+// of thousands of them 1e-7): none / 2 / 3 / 4 of 8 took 1379 / 1237 / 1210 / about 1400 us for 16384
+// tokens, 32 / 8 heads, D = 128.
+constexpr uint32_t MT_POLY = 0x52;
+
 
 __device__ __forceinline__ uint64_t ex2_pair(uint64_t x) {
   const float2 v = unpack_f2(x);
@@ -242,7 +243,7 @@ __global__ void __launch_bounds__(MT_THREADS, 1)
       tc_fence_after();
       // columns of queries before this key, past the sequence or outside the window do not
       // count, whatever their scores are
-      const int c_lo = p.causal ? (key - pos0) * p.G : 0;
+      const int c_lo = p.causal ? max(0, key - pos0) * p.G : 0;
       uint64_t sum[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
