@@ -4,7 +4,8 @@ Operators (same names and semantics as ``linattn.kernels.triton.*``):
 ``page_bounds``, ``page_select``, ``block_sparse_attention``, ``indexer_topk``,
 ``lse_combine``.
 Plugin: ``build("cuda_quest" | "cuda_dsa" | "cuda_csa2" | "cuda_nsa", cfg)`` returns an ``AttentionVariant`` like
-``linattn.registry.build``.  Serving path: ``PagedKVCache`` + ``QuestDecoder``.
+``linattn.registry.build``.  Serving path: ``PagedKVCache`` + ``QuestDecoder``; with
+eviction, ``packed_attention`` + ``attention_mass`` for the prompts and ``HeavyCache``.
 
 Every call runs hand-written CUDA in ``_native/liblinattn_b200.so`` through the C
 ABI of ``include/linattn_b200.h``; there is no CPU fallback.
