@@ -13,12 +13,16 @@
 // half of them), so that o is not spread over warps; one barrier a tile.  P is split into
 // hi + lo 16-bit parts (to ~2^-16), so o carries its own rounding only.
 //
-// The masses need a unit's final lse: its scores go to the workspace (4 bytes a slot and head,
-// which L2 holds until they are read back), and four more warps add a finished unit's weights
-// while the others go on with the next one (done by the same warps it cost 59 of 205 us at 64
-// sequences x 8 heads x 4096 slots).  A unit that one CTA has whole is finished there; of one
-// that several CTAs share, the last to arrive merges their (o, m, l): the parts are added in
-// their order, whoever does it, so results do not depend on it.
+// The masses need a unit's final lse, so its scores are kept until then, and four more warps add
+// a finished unit's weights while the others go on with the next one (done by the same warps,
+// through global memory, it cost 59 of 205 us at 64 sequences x 8 heads x 4096 slots).  A unit
+// that one CTA has whole keeps its scores in tensor memory, which this kernel has no other use
+// for: a warp stores its accumulator fragments as they are, 4 columns a tile, and the mass warp
+// of the same 32 lanes reads them back (4096 slots a unit for up to 8 heads, twice over; through
+// the workspace in global memory the call took 168 us instead of 162).  Longer ones, and
+// units that several CTAs share, go through the workspace; the last CTA to arrive at a shared
+// unit merges its (o, m, l): the parts are added in their order, whoever does it, so results do
+// not depend on it.
 #include <cstdio>
 #include <cstring>
 #include <type_traits>
@@ -96,6 +100,11 @@ __device__ __forceinline__ bool attend_barrier_or(bool x) {
       : "memory");
   return r != 0;
 }
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, const float (&v)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(__float_as_uint(v[0])),
+               "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3]))
+               : "memory");
+}
 __device__ __forceinline__ void attend_barrier() { asm volatile("barrier.cta.sync 1, 256;" ::: "memory"); }
 
 template <typename T, int D, int NT>
@@ -114,6 +123,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
   __shared__ float fin[2][2][HN];
   __shared__ int64_t job_unit[2];
   __shared__ int job_count[2];  // slots in use, or -1: no more
+  __shared__ int job_tmem[2];   // scores in tensor memory
+  __shared__ uint32_t tmem_sh;
   __shared__ float upper[D == 64 ? 4 * 32 * 4 * NT : 1];  // D = 64: o of the tile's upper slots
   __shared__ int dead, arrived;
   __shared__ int64_t share[3];  // first tile, end, all tiles
@@ -132,6 +143,11 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     dead = 0;
     mbar_fence_init();
   }
+  if (warp == AT_WARPS + 1 && a.accumulate) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_sh)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   // this CTA's share of the tiles
@@ -170,6 +186,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     }
   }
   __syncthreads();
+  tc_fence_after();
   const int64_t t0 = share[0], t1 = share[1], total = share[2];
   const int64_t nc = lmin(gridDim.x, total);
   // sequences without slots: o = 0
@@ -179,7 +196,17 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         const int head = i / D;
         static_cast<T*>(a.out)[b * a.ob + (static_cast<int64_t>(head / a.heads) * a.G + a.h0 + head % a.heads) * a.oh + i % D] = T(0.f);
       }
-  if (t1 <= t0) return;
+  // tensor memory: two units' scores of 256 columns, of a unit 128 columns for each warp of a
+  // lane quarter, 4 NT columns a tile
+  const uint32_t tmem = a.accumulate ? tmem_sh : 0;
+  auto free_tmem = [&] {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  };
+  if (t1 <= t0) {
+    if (warp == AT_WARPS + 1 && a.accumulate) free_tmem();
+    return;
+  }
   AttendWalk w{a.seen, a.B, a.H, a.M};
   w.sequence(start[0]);
   w.h = start[1] / w.tiles;
@@ -188,9 +215,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
   if (warp == AT_WARPS) {
     if (lane == 0) {
       int j = 0;
-      int64_t t = t0;
       bool ok = true;
-      while (ok && t < t1) {
+      for (int64_t t = t0; ok && t < t1;) {
         const int end = static_cast<int>(lmin(w.tiles, first + (t1 - t)));
         const int64_t row0 = (static_cast<int64_t>(w.b) * a.H + w.h) * a.M;
         for (int i = first; ok && i < end; ++i, ++j) {
@@ -233,16 +259,70 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     const int at = tid - 32 * (AT_WARPS + 1);
     for (int job = 0;; ++job) {
       const int x = job & 1;
-      if (!__all_sync(0xffffffffu, mbar_wait_bounded(&job_full[x], static_cast<uint32_t>((job >> 1) & 1)))) {
-        if (lane == 0) report(a.status, LINATTN_DEV_TIMEOUT);
-        return;
-      }
-      const int count = job_count[x];
-      if (count < 0) return;
+      const bool there = warp_wait(&job_full[x], static_cast<uint32_t>((job >> 1) & 1));
+      if (!there && lane == 0) report(a.status, LINATTN_DEV_TIMEOUT);
+      const int count = there ? job_count[x] : -1;
+      if (count < 0) break;
       const int64_t unit = job_unit[x];
       float* mass = a.mass + unit * a.M;
       const float* sc = a.scores + unit * a.heads * a.M;
-      if ((a.M & 3) == 0) {  // rows on 16 bytes: 8 slots a thread at a time, the loads together
+      if (job_tmem[x]) {
+        // this lane's scores of a tile: slots g and g + 8 of the two warps of its quarter, heads
+        // 2 tig and 2 tig + 1 (of every 8)
+        tc_fence_after();
+        const int g = lane >> 2, tig = lane & 3, quarter = warp & 3;
+        float f0[NT][2], f1[NT][2];
+#pragma unroll
+        for (int y = 0; y < NT; ++y)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int head = y * 8 + 2 * tig + e;
+            f0[y][e] = fin[x][0][head];
+            f1[y][e] = head < a.heads ? fin[x][1][head] : 0.f;
+          }
+        constexpr int STEP = NT >= 4 ? 1 : 4 / NT;  // tiles of 16 columns
+        constexpr int BATCH = 2 * STEP;             // tiles whose masses are fetched together
+        const int tiles = (count + AT_ROWS - 1) / AT_ROWS;
+        for (int i0 = 0; i0 < tiles; i0 += BATCH) {
+          // lane tig = 0 owns slot g, tig = 1 slot g + 8
+          const int n0 = i0 * AT_ROWS + 16 * quarter + g + 8 * tig;
+          float old[2][BATCH];
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int e = 0; e < BATCH; ++e) {
+              const int n = n0 + 64 * half + e * AT_ROWS;
+              old[half][e] = tig < 2 && n < count ? mass[n] : 0.f;
+            }
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int s0 = 0; s0 < BATCH; s0 += STEP) {
+              if (i0 + s0 >= tiles) continue;
+              uint32_t sv[16];
+              tmem_ld16(tmem + (static_cast<uint32_t>(32 * quarter) << 16) + x * 256 + half * 128 + (i0 + s0) * 4 * NT, sv);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < STEP; ++e) {
+                float lo = 0.f, hi = 0.f;
+#pragma unroll
+                for (int y = 0; y < NT; ++y)
+#pragma unroll
+                  for (int z = 0; z < 2; ++z) {
+                    lo += ex2_approx(__uint_as_float(sv[((e * NT + y) * 4 + z) & 15]) - f0[y][z]) * f1[y][z];
+                    hi += ex2_approx(__uint_as_float(sv[((e * NT + y) * 4 + 2 + z) & 15]) - f0[y][z]) * f1[y][z];
+                  }
+                lo += __shfl_xor_sync(0xffffffffu, lo, 1);
+                hi += __shfl_xor_sync(0xffffffffu, hi, 1);
+                lo += __shfl_xor_sync(0xffffffffu, lo, 2);
+                hi += __shfl_xor_sync(0xffffffffu, hi, 2);
+                const int n = n0 + 64 * half + (s0 + e) * AT_ROWS;
+                if (tig < 2 && n < count) mass[n] = old[half][s0 + e] + (tig == 0 ? lo : hi);
+              }
+            }
+        }
+        tc_fence_before();
+      } else if ((a.M & 3) == 0) {  // rows on 16 bytes: 8 slots a thread at a time, the loads together
         constexpr int U = 2;
         const int quads = (count + 3) >> 2, stride = a.M >> 2;
         for (int n0 = at; n0 < quads; n0 += U * AT_MASS) {
@@ -287,6 +367,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
       }
       mbar_arrive(&job_empty[x]);
     }
+    tc_fence_before();
+    asm volatile("barrier.cta.sync 2, 128;" ::: "memory");  // the other mass warps have read theirs
+    if (warp == AT_WARPS + 1) free_tmem();
+    return;
   }
 
   const int g = lane >> 2, tig = lane & 3;
@@ -298,20 +382,22 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
   const int vrow = (lane & 7) + ((lane >> 4) & 1) * 8, vchunk = ct * 2 + ((lane >> 3) & 1);
   const uint32_t k_off = krow * 128, v_off = HALVES * SM::HALF + (vchunk >> 3) * SM::HALF;
   int j = 0, jobs = 0;
-  int64_t t = t0;
   bool ok = true;
   // room for a unit's result: the mass warps are done with the one before the last
   auto job_room = [&] {
     if (a.accumulate && jobs >= 2 && ok)
       ok = __all_sync(0xffffffffu, mbar_wait_bounded(&job_empty[jobs & 1], static_cast<uint32_t>((jobs / 2 - 1) & 1)));
+    tc_fence_after();
   };
-  auto job_send = [&](int64_t unit, int count) {  // one thread, after a barrier
+  auto job_send = [&](int64_t unit, int count, bool in_tmem) {  // one thread, after a barrier
     job_unit[jobs & 1] = unit;
     job_count[jobs & 1] = count;
+    job_tmem[jobs & 1] = in_tmem ? 1 : 0;
     mbar_arrive(&job_full[jobs & 1]);
   };
-  while (t < t1) {
+  for (int64_t t = t0; t < t1;) {
     const int end = static_cast<int>(lmin(w.tiles, first + (t1 - t)));
+    const bool whole = first == 0 && end == w.tiles;  // else several CTAs share the unit
     const int64_t unit = static_cast<int64_t>(w.b) * a.H + w.h;
     // q as the B operand: channels 16 kk + 2 tig (+ 1, + 8, + 9) of head g
     uint32_t q[NT][D / 16][2];
@@ -332,6 +418,11 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
       l[x][0] = l[x][1] = 0.f;
     }
     float* sc = a.scores + unit * a.heads * a.M;
+    const int64_t u0 = t - first, u1 = u0 + w.tiles;                       // the unit's tiles among all
+    const int64_t c0 = ((u0 + 1) * nc - 1) / total, c1 = (u1 * nc - 1) / total;  // the CTAs that share it
+    const bool in_tmem = a.accumulate && whole && w.tiles * NT <= 32 && NT <= 2;
+    if (in_tmem) job_room();
+    const uint32_t sc_tmem = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + (jobs & 1) * 256 + (warp >> 2) * 128;
     for (int i = first; i < end; ++i, ++j) {
       const int st = j % ST, valid = min(AT_ROWS, w.count - i * AT_ROWS);
       // a warp whose wait gave up goes on through the barriers
@@ -359,9 +450,13 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
           const int r = e < 2 ? r0 : r1, head = x * 8 + 2 * tig + (e & 1);
           const float v = r < valid ? (s[x][e] + s2[x][e]) * a.scale_log2 : -INFINITY;
           s[x][e] = v;
-          if (a.accumulate && r < valid && head < a.heads) sc[static_cast<int64_t>(head) * a.M + i * AT_ROWS + r] = v;
+          if (a.accumulate && !in_tmem && r < valid && head < a.heads) sc[static_cast<int64_t>(head) * a.M + i * AT_ROWS + r] = v;
           grow |= v > m[x][e & 1] + 8.f;
         }
+      if (in_tmem) {
+#pragma unroll
+        for (int x = 0; x < NT; ++x) tmem_st4(sc_tmem + (i * NT + x) * 4, s[x]);
+      }
       uint8_t* pb = pbuf + (j & 1) * (2 * HN * AT_PROW);
       float ps[NT][2];  // this lane's share of the tile's sums
       auto weights = [&] {
@@ -486,12 +581,15 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         for (int e = 0; e < 4; ++e) acc[x][e] += upper[((ct * 32 + lane) * NT + x) * 4 + e];
     }
     T* out = static_cast<T*>(a.out) + w.b * a.ob + (static_cast<int64_t>(w.h) * a.G + a.h0) * a.oh;
-    const int64_t u0 = t - first, u1 = u0 + w.tiles;                       // the unit's tiles among all
-    const int64_t c0 = ((u0 + 1) * nc - 1) / total, c1 = (u1 * nc - 1) / total;  // the CTAs that share it
     bool finish = true;
-    job_room();
+    if (in_tmem) {
+      tmem_wait_st();
+      tc_fence_before();
+    } else {
+      job_room();
+    }
     float (*result)[HN] = fin[jobs & 1];
-    if (c0 == c1) {
+    if (whole) {
       if (warp == 0 && g == 0) {
 #pragma unroll
         for (int x = 0; x < NT; ++x)
@@ -596,7 +694,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
       }
     }
     if (finish && a.accumulate) {
-      if (tid == 0) job_send(unit, w.count);
+      if (tid == 0) job_send(unit, w.count, in_tmem);
       ++jobs;
     }
     t += end - first;
@@ -605,7 +703,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
   }
   if (a.accumulate) {
     job_room();
-    if (tid == 0) job_send(0, -1);
+    if (tid == 0) job_send(0, -1, false);
   }
   if (!ok && lane == 0) {
     report(a.status, LINATTN_DEV_TIMEOUT);

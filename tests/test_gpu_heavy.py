@@ -214,18 +214,21 @@ def test_attend(cuda, seen, budget, hq, hkv, d, dtype, accumulate):
     assert torch.equal(wide[..., d:], first) and (wide[..., :d] == 0).all()
 
 
-@pytest.mark.parametrize("batch,budget", [(70, 40), (33, 400), (3, 2000)])
-def test_attend_shares(cuda, batch, budget):
-    """Many short sequences to a CTA and many CTAs to a sequence, some of them empty."""
+@pytest.mark.parametrize("batch,budget,hq", [(70, 40, 8), (33, 400, 8), (3, 2000, 8), (40, 301, 48), (45, 4000, 8), (30, 1900, 64)])
+def test_attend_shares(cuda, batch, budget, hq):
+    """Many short sequences to a CTA and many CTAs to a sequence, some of them empty; units that
+    one CTA has whole, of the sizes whose scores stay in tensor memory and of larger ones."""
     from linattn_b200 import HeavyCache
 
-    hq, hkv, d, dtype = 8, 4, 64, torch.bfloat16
-    g = torch.Generator().manual_seed(batch)
+    hkv, d, dtype = 4, 64, torch.bfloat16
+    g = torch.Generator(device="cuda").manual_seed(batch)
     cache = HeavyCache(batch, hkv, d, budget, dtype=dtype)
-    cache.k.copy_(torch.randn(batch, hkv, budget, d, generator=g))
-    cache.v.copy_(torch.randn(batch, hkv, budget, d, generator=g))
-    cache.seen.copy_(torch.randint(0, 2 * budget, (batch,), generator=g) * (torch.rand(batch, generator=g) < 0.8))
-    q = torch.randn(batch, hq, 1, d, generator=g).to(dtype).cuda()
+    cache.k.normal_(generator=g)
+    cache.v.normal_(generator=g)
+    cache.mass.uniform_(generator=g)
+    cache.seen.copy_(torch.randint(0, 2 * budget, (batch,), generator=g, device="cuda")
+                     * (torch.rand(batch, generator=g, device="cuda") < 0.8))
+    q = torch.randn(batch, hq, 1, d, generator=g, device="cuda").to(dtype)
     for _ in range(2):  # the arrival counts are back at zero
         before = cache.mass.clone()
         o = cache.attend(q)
