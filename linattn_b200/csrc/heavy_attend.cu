@@ -665,6 +665,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
           }
         }
         attend_barrier();
+        if (a.accumulate && tid == 0) job_send(unit, w.count, false);  // the masses beside the merge of o
         // groups of threads over the parts, four channels a thread
         const int quads = a.heads * (D / 4), groups = max(1, 32 * AT_WARPS / quads);
         for (int y0 = 0; y0 < quads; y0 += 32 * AT_WARPS) {
@@ -694,7 +695,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
       }
     }
     if (finish && a.accumulate) {
-      if (tid == 0) job_send(unit, w.count, in_tmem);
+      if (whole && tid == 0) job_send(unit, w.count, in_tmem);
       ++jobs;
     }
     t += end - first;
