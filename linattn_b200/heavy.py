@@ -56,10 +56,9 @@ class HeavyCache:
         self.v = torch.zeros(*shape, head_dim, dtype=dtype, device=self.device)
         self.mass = torch.zeros(shape, dtype=torch.float32, device=self.device)
         self.pos = torch.zeros(shape, dtype=torch.int32, device=self.device)
-        self.seen = torch.zeros(batch, dtype=torch.int32, device=self.device)
-        self._ticket = torch.zeros(batch, dtype=torch.int32, device=self.device)
+        ints = torch.zeros(batch * (2 + n_kv_heads), dtype=torch.int32, device=self.device)
+        self.seen, self._ticket, self._unit_ticket = ints[:batch], ints[batch:2 * batch], ints[2 * batch:]
         self.device = self.k.device
-        self._unit_ticket = torch.zeros(batch * n_kv_heads, dtype=torch.int32, device=self.device)
         self._workspace: Optional[torch.Tensor] = None  # attend()'s, by its first call
         self._desc = L.Heavy(self.k.data_ptr(), self.v.data_ptr(), self.mass.data_ptr(), self.pos.data_ptr(),
                              self.seen.data_ptr(), L.dtype_code(self.k), batch, n_kv_heads, budget, head_dim, sinks, recent)

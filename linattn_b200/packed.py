@@ -13,8 +13,7 @@ Packed layout: ``q (N_q, H_q, D)``, ``k, v (N_k, H_kv, D)``, offsets ``cu_q, cu_
 
 from __future__ import annotations
 
-import functools
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -23,14 +22,29 @@ from linattn_b200 import _lib as L
 __all__ = ["packed_attention", "attention_mass"]
 
 
-def _rows(name: str, x: torch.Tensor) -> torch.Tensor:
-    """x with contiguous channels and 16-byte rows, as the tensor maps read it."""
-    if x.dim() != 3:
-        raise ValueError(f"{name} must be (tokens, heads, head_dim), got shape {tuple(x.shape)}")
-    s0, s1, s2 = x.stride()
-    if s2 != 1 or (s0 | s1) & 7 or s0 < 1 or s1 < 1 or x.data_ptr() & 15:
-        x = x.clone(memory_format=torch.contiguous_format)  # (contiguous() may hand back an unaligned view)
-    return x
+_PLANS: dict = {}  # checked arguments by shapes, strides and types (nothing of their contents or addresses)
+
+
+class _Plan(NamedTuple):
+    s: int
+    nq: int
+    nk: int
+    hq: int
+    hkv: int
+    d: int
+    max_q: int
+    max_k: int
+    n_splits: int
+    ws_bytes: int
+    dtype: int
+    device: torch.device
+    copies: tuple      # operands whose rows have to be copied first
+    strides: tuple     # of the operands, as the library takes them
+    out_strides: object
+
+
+def _layout(x):
+    return None if x is None else (x.shape, x.stride(), x.dtype, x.get_device())
 
 
 def _offsets(name: str, cu: torch.Tensor) -> int:
@@ -39,39 +53,64 @@ def _offsets(name: str, cu: torch.Tensor) -> int:
     return cu.numel() - 1
 
 
-def _packed(q, k, cu_q, cu_k, max_q, max_k):
-    """The checked arguments that both operators share."""
+def _on_grid(x: torch.Tensor) -> bool:
+    """Contiguous channels and strides of whole 16-byte pieces, as the tensor maps read it."""
+    s0, s1, s2 = x.stride()
+    return s2 == 1 and not (s0 | s1) & 7 and s0 > 0 and s1 > 0
+
+
+def _plan(q, k, v, cu_q, cu_k, max_q, max_k, window, n_splits) -> _Plan:
+    """The checked arguments of attention (``window`` None) or mass (``v`` None)."""
+    dev = L.require_cuda(q, k, v, cu_q, cu_k)
+    operands = [("q", q), ("k", k)] + ([("v", v)] if v is not None else [])
+    for name, x in operands:
+        if x.dim() != 3:
+            raise ValueError(f"{name} must be (tokens, heads, head_dim), got shape {tuple(x.shape)}")
     if q.dtype != k.dtype:
         raise ValueError("q and k must have one dtype")
-    q, k = _rows("q", q), _rows("k", k)
     nq, hq, d = q.shape
     nk, hkv, dk = k.shape
     if d != dk:
         raise ValueError(f"head_dim of q and k differ: {d} and {dk}")
+    if v is not None and (v.dtype != k.dtype or v.shape != k.shape):
+        raise ValueError("k and v must have one dtype and shape")
     s = _offsets("cu_q", cu_q)
     if cu_k is None:
         if nq != nk:
             raise ValueError("without cu_k, q and k must hold the same tokens")
-        cu_k = cu_q
     elif _offsets("cu_k", cu_k) != s:
         raise ValueError("cu_q and cu_k must describe the same number of sequences")
-    return (q, k, cu_k, s, nq, nk, hq, hkv, d, nq if max_q is None else min(int(max_q), nq),
-            nk if max_k is None else min(int(max_k), nk))
-
-
-@functools.lru_cache(maxsize=1024)
-def _attention_plan(device: int, nq: int, hq: int, hkv: int, d: int, s: int, max_q: int, max_k: int, n_splits: int):
-    """(splits, workspace bytes); ``n_splits`` 0: the library's choice."""
+    max_q = nq if max_q is None else min(int(max_q), nq)
+    max_k = nk if max_k is None else min(int(max_k), nk)
     lib = L.lib()
-    n = n_splits or lib.linattn_packed_attention_splits(nq, hq, hkv, s, max_q, max_k)
-    return n, lib.linattn_packed_attention_workspace(nq, hq, d, n)
+    if window is None:
+        n = n_splits or lib.linattn_packed_attention_splits(nq, hq, hkv, s, max_q, max_k)
+        ws = lib.linattn_packed_attention_workspace(nq, hq, d, n)
+    else:
+        if window < 0:
+            raise ValueError("window must be >= 0")
+        n = n_splits or lib.linattn_attention_mass_splits(hq, hkv, s, max_q, max_k, window)
+        ws = lib.linattn_attention_mass_workspace(nk, hkv, n)
+    copies = tuple(not _on_grid(x) for _, x in operands)
+    # a copy is contiguous
+    strides = tuple(L.i64_array((x.shape[1] * d, d)) if c else L.strides2(x) for c, (_, x) in zip(copies, operands))
+    return _Plan(s, nq, nk, hq, hkv, d, max_q, max_k, n, ws, L.dtype_code(q), dev, copies, strides, L.i64_array((hq * d, d)))
 
 
-@functools.lru_cache(maxsize=1024)
-def _mass_plan(device: int, nk: int, hq: int, hkv: int, s: int, max_q: int, max_k: int, window: int, n_splits: int):
-    lib = L.lib()
-    n = n_splits or lib.linattn_attention_mass_splits(hq, hkv, s, max_q, max_k, window)
-    return n, lib.linattn_attention_mass_workspace(nk, hkv, n)
+def _planned(key, *args) -> _Plan:
+    plan = _PLANS.get(key)
+    if plan is None:
+        if len(_PLANS) >= 1024:
+            _PLANS.clear()
+        plan = _PLANS[key] = _plan(*args)
+    return plan
+
+
+def _aligned(x: torch.Tensor, copy: bool, strides, plan: _Plan):
+    """x on the 16-byte grid (a copy where it is not) and its strides."""
+    if not copy and x.data_ptr() & 15 == 0:
+        return x, strides
+    return x.clone(memory_format=torch.contiguous_format), L.i64_array((x.shape[1] * plan.d, plan.d))
 
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor,
@@ -90,31 +129,36 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     ``max_q`` / ``max_k``: the longest sequence's query / key rows, where the caller knows them
     (they size the grid; the default is all rows).  ``n_splits`` (default: chosen) cuts the key
     ranges when there are few rows; ``workspace``: fp32 scratch for it, allocated if None."""
-    dev = L.require_cuda(q, k, v, cu_q, cu_k, out, lse_out, workspace)
-    q, k, cu_k, s, nq, nk, hq, hkv, d, max_q, max_k = _packed(q, k, cu_q, cu_k, max_q, max_k)
-    if v.dtype != k.dtype or v.shape != k.shape:
-        raise ValueError("k and v must have one dtype and shape")
-    v = _rows("v", v)
+    p = _planned((_layout(q), _layout(k), _layout(v), _layout(cu_q), _layout(cu_k), max_q, max_k, None, n_splits),
+                 q, k, v, cu_q, cu_k, max_q, max_k, None, n_splits)
+    q, sq = _aligned(q, p.copies[0], p.strides[0], p)
+    k, sk = _aligned(k, p.copies[1], p.strides[1], p)
+    v, sv = _aligned(v, p.copies[2], p.strides[2], p)
+    out_strides = p.out_strides
     if out is None:
-        out = torch.empty((nq, hq, d), dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
-        raise ValueError("out must have q's shape and dtype with contiguous channels")
+        out = torch.empty((p.nq, p.hq, p.d), dtype=q.dtype, device=p.device)
+    else:
+        L.require_cuda(q, out)
+        if out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
+            raise ValueError("out must have q's shape and dtype with contiguous channels")
+        out_strides = L.strides2(out)
     if lse_out is None:
-        lse_out = torch.empty((nq, hq), dtype=torch.float32, device=dev)
-    elif lse_out.shape != (nq, hq) or lse_out.dtype != torch.float32 or not lse_out.is_contiguous():
-        raise ValueError("lse_out must be a contiguous fp32 (N_q, H_q) tensor")
-    n_splits, ws_bytes = _attention_plan(dev.index, nq, hq, hkv, d, s, max_q, max_k, n_splits or 0)
-    if n_splits > 1:
+        lse_out = torch.empty((p.nq, p.hq), dtype=torch.float32, device=p.device)
+    elif lse_out.shape != (p.nq, p.hq) or lse_out.dtype != torch.float32 or not lse_out.is_contiguous() or lse_out.device != p.device:
+        raise ValueError("lse_out must be a contiguous fp32 (N_q, H_q) tensor on q's device")
+    ws_bytes = p.ws_bytes
+    if p.n_splits > 1:
         if workspace is None:
-            workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+            workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=p.device)
+        L.require_cuda(q, workspace)
         ws_bytes = workspace.numel() * workspace.element_size()
     L.check(L.lib().linattn_packed_attention(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), L.dtype_code(q), nq, nk, hq, hkv, d, L.strides2(q), L.strides2(k),
-        L.strides2(v), cu_q.data_ptr(), cu_k.data_ptr(), s, max_q, max_k, int(causal),
-        d ** -0.5 if scale is None else float(scale), out.data_ptr(), L.strides2(out), lse_out.data_ptr(),
-        n_splits, L.ptr(workspace), ws_bytes, L.status_word(dev).data_ptr(), L.raw_stream(dev.index)))
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), p.dtype, p.nq, p.nk, p.hq, p.hkv, p.d, sq, sk, sv, cu_q.data_ptr(),
+        (cu_q if cu_k is None else cu_k).data_ptr(), p.s, p.max_q, p.max_k, 1 if causal else 0,
+        p.d ** -0.5 if scale is None else float(scale), out.data_ptr(), out_strides, lse_out.data_ptr(),
+        p.n_splits, L.ptr(workspace), ws_bytes, L.status_word(p.device).data_ptr(), L.raw_stream(p.device.index)))
     if L.strict():
-        L.check_status(dev)
+        L.check_status(p.device)
     return out, lse_out
 
 
@@ -127,26 +171,27 @@ def attention_mass(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, cu_q: to
     queries that read key ``j`` and the query heads of kv head ``h``.  ``lse (N_q, H_q)`` as
     :func:`packed_attention` returns it for the same ``q, k`` and offsets.  ``window > 0``:
     only each sequence's last ``window`` queries count.  The sums have a fixed order."""
-    dev = L.require_cuda(q, k, lse, cu_q, cu_k, out, workspace)
-    q, k, cu_k, s, nq, nk, hq, hkv, d, max_q, max_k = _packed(q, k, cu_q, cu_k, max_q, max_k)
-    if lse.shape != (nq, hq) or lse.dtype != torch.float32 or not lse.is_contiguous():
-        raise ValueError("lse must be a contiguous fp32 (N_q, H_q) tensor")
-    if window < 0:
-        raise ValueError("window must be >= 0")
+    p = _planned((_layout(q), _layout(k), None, _layout(cu_q), _layout(cu_k), max_q, max_k, window, n_splits),
+                 q, k, None, cu_q, cu_k, max_q, max_k, window, n_splits)
+    q, sq = _aligned(q, p.copies[0], p.strides[0], p)
+    k, sk = _aligned(k, p.copies[1], p.strides[1], p)
+    if lse.shape != (p.nq, p.hq) or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != p.device:
+        raise ValueError("lse must be a contiguous fp32 (N_q, H_q) tensor on q's device")
     if out is None:
-        out = torch.empty((hkv, nk), dtype=torch.float32, device=dev)
-    elif out.shape != (hkv, nk) or out.dtype != torch.float32 or out.stride(1) != 1:
-        raise ValueError("out must be an fp32 (H_kv, N_k) tensor with contiguous rows")
-    n_splits, ws_bytes = _mass_plan(dev.index, nk, hq, hkv, s, max_q, max_k, int(window), n_splits or 0)
-    if n_splits > 1:
+        out = torch.empty((p.hkv, p.nk), dtype=torch.float32, device=p.device)
+    elif out.shape != (p.hkv, p.nk) or out.dtype != torch.float32 or out.stride(1) != 1 or out.device != p.device:
+        raise ValueError("out must be an fp32 (H_kv, N_k) tensor with contiguous rows on q's device")
+    ws_bytes = p.ws_bytes
+    if p.n_splits > 1:
         if workspace is None:
-            workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+            workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=p.device)
+        L.require_cuda(q, workspace)
         ws_bytes = workspace.numel() * workspace.element_size()
     L.check(L.lib().linattn_attention_mass(
-        q.data_ptr(), k.data_ptr(), L.dtype_code(q), nq, nk, hq, hkv, d, L.strides2(q), L.strides2(k), lse.data_ptr(),
-        cu_q.data_ptr(), cu_k.data_ptr(), s, max_q, max_k, int(causal), int(window),
-        d ** -0.5 if scale is None else float(scale), out.data_ptr(), out.stride(0), n_splits,
-        L.ptr(workspace), ws_bytes, L.status_word(dev).data_ptr(), L.raw_stream(dev.index)))
+        q.data_ptr(), k.data_ptr(), p.dtype, p.nq, p.nk, p.hq, p.hkv, p.d, sq, sk, lse.data_ptr(), cu_q.data_ptr(),
+        (cu_q if cu_k is None else cu_k).data_ptr(), p.s, p.max_q, p.max_k, 1 if causal else 0, int(window),
+        p.d ** -0.5 if scale is None else float(scale), out.data_ptr(), out.stride(0), p.n_splits, L.ptr(workspace),
+        ws_bytes, L.status_word(p.device).data_ptr(), L.raw_stream(p.device.index)))
     if L.strict():
-        L.check_status(dev)
+        L.check_status(p.device)
     return out

@@ -234,6 +234,32 @@ def test_mass_sums_to_the_queries(cuda):
         at += n
 
 
+def test_packed_without_keys_or_queries(cuda):
+    from linattn_b200 import attention_mass, packed_attention
+
+    q, k, v = _inputs(11, [5], [7], 4, 2, 64, torch.bfloat16)
+    o, lse = packed_attention(q, k[:0], v[:0], _cu([5]), _cu([0]))
+    assert (o == 0).all() and (lse == -math.inf).all()
+    o, lse = packed_attention(q[:0], k, v, _cu([0]), _cu([7]))
+    assert o.shape == (0, 4, 64) and lse.shape == (0, 4)
+    assert (attention_mass(q[:0], k, lse, _cu([0]), _cu([7])) == 0).all()
+    assert attention_mass(q, k[:0], torch.zeros(5, 4, device="cuda"), _cu([5]), _cu([0])).shape == (2, 0)
+    none = torch.zeros(1, dtype=torch.int32, device="cuda")  # no sequence at all
+    assert packed_attention(q[:0], k[:0], v[:0], none)[0].shape == (0, 4, 64)
+
+
+def test_packed_broadcast_heads(cuda):
+    """K and V expanded over heads (stride 0) and single heads with odd strides."""
+    from linattn_b200 import packed_attention
+
+    q, k, v = _inputs(12, [50], [50], 4, 1, 64, torch.float16)
+    cu = _cu([50])
+    want = packed_attention(q, k.expand(-1, 2, -1).contiguous(), v.expand(-1, 2, -1).contiguous(), cu)[0]
+    assert torch.equal(packed_attention(q, k.expand(-1, 2, -1), v.expand(-1, 2, -1), cu)[0], want)
+    one = packed_attention(q, k, v, cu)[0]
+    assert torch.equal(packed_attention(q, k.as_strided(k.shape, (64, 3, 1)), v, cu)[0], one)
+
+
 def test_packed_refusals(cuda):
     from linattn_b200 import attention_mass, packed_attention
 
