@@ -146,11 +146,11 @@ class HeavyCache:
         plan = self._plans.get(key)
         if plan is None:
             plan = self._keep(key, self._plan_attend(q))
-        hq, strides, dense, need = plan
+        hq, strides, dense, packed, need = plan
         if strides is None or q.data_ptr() & 15:  # rows off the 16-byte grid
             return self.attend(q.clone(memory_format=torch.contiguous_format), scale=scale, accumulate=accumulate, out=out)
         if out is None:
-            out, out_strides = torch.empty(shape, dtype=self.dtype, device=self.device), dense
+            out, out_strides = (torch.empty_like(q) if dense else q.new_empty(shape)), packed
         else:
             L.require_cuda(out, self.k)
             if out.shape != shape or out.dtype != self.dtype or out.stride(3) != 1:
@@ -167,7 +167,8 @@ class HeavyCache:
         return out
 
     def _plan_attend(self, q: torch.Tensor):
-        """(H_q, strides of q or None where the rows have to be copied first, of a new output, workspace bytes)."""
+        """(H_q, strides of q or None where the rows have to be copied first, whether q is
+        contiguous, strides of a new output, workspace bytes)."""
         shape = tuple(q.shape)
         if (len(shape) != 4 or shape[0] != self.batch or shape[1] < 1 or shape[1] % self.n_kv_heads
                 or shape[2:] != (1, self.head_dim)):
@@ -175,7 +176,7 @@ class HeavyCache:
         if q.dtype != self.dtype:
             raise ValueError(f"q must be {self.dtype} as the cache")
         L.require_cuda(q, self.k)
-        return (shape[1], L.strides2(q) if _on_grid(q) else None, L.i64_array((shape[1] * self.head_dim, self.head_dim)),
+        return (shape[1], L.strides2(q) if _on_grid(q) else None, q.is_contiguous(), L.i64_array((shape[1] * self.head_dim, self.head_dim)),
                 self._lib.linattn_heavy_attend_workspace(self.batch, shape[1], self.n_kv_heads, self.budget))
 
     def step(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: Optional[float] = None,

@@ -41,6 +41,7 @@ class _Plan(NamedTuple):
     copies: tuple      # operands whose rows have to be copied first
     strides: tuple     # of the operands, as the library takes them
     out_strides: object
+    dense: bool        # q is contiguous
 
 
 def _layout(x):
@@ -94,7 +95,8 @@ def _plan(q, k, v, cu_q, cu_k, max_q, max_k, window, n_splits) -> _Plan:
     copies = tuple(not _on_grid(x) for _, x in operands)
     # a copy is contiguous
     strides = tuple(L.i64_array((x.shape[1] * d, d)) if c else L.strides2(x) for c, (_, x) in zip(copies, operands))
-    return _Plan(s, nq, nk, hq, hkv, d, max_q, max_k, n, ws, L.dtype_code(q), dev, copies, strides, L.i64_array((hq * d, d)))
+    return _Plan(s, nq, nk, hq, hkv, d, max_q, max_k, n, ws, L.dtype_code(q), dev, copies, strides, L.i64_array((hq * d, d)),
+                 q.is_contiguous())
 
 
 def _planned(key, *args) -> _Plan:
@@ -136,14 +138,14 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     v, sv = _aligned(v, p.copies[2], p.strides[2], p)
     out_strides = p.out_strides
     if out is None:
-        out = torch.empty((p.nq, p.hq, p.d), dtype=q.dtype, device=p.device)
+        out = torch.empty_like(q) if p.dense else q.new_empty((p.nq, p.hq, p.d))
     else:
         L.require_cuda(q, out)
         if out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
             raise ValueError("out must have q's shape and dtype with contiguous channels")
         out_strides = L.strides2(out)
     if lse_out is None:
-        lse_out = torch.empty((p.nq, p.hq), dtype=torch.float32, device=p.device)
+        lse_out = q.new_empty((p.nq, p.hq), dtype=torch.float32)
     elif lse_out.shape != (p.nq, p.hq) or lse_out.dtype != torch.float32 or not lse_out.is_contiguous() or lse_out.device != p.device:
         raise ValueError("lse_out must be a contiguous fp32 (N_q, H_q) tensor on q's device")
     ws_bytes = p.ws_bytes
@@ -178,7 +180,7 @@ def attention_mass(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, cu_q: to
     if lse.shape != (p.nq, p.hq) or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != p.device:
         raise ValueError("lse must be a contiguous fp32 (N_q, H_q) tensor on q's device")
     if out is None:
-        out = torch.empty((p.hkv, p.nk), dtype=torch.float32, device=p.device)
+        out = q.new_empty((p.hkv, p.nk), dtype=torch.float32)
     elif out.shape != (p.hkv, p.nk) or out.dtype != torch.float32 or out.stride(1) != 1 or out.device != p.device:
         raise ValueError("out must be an fp32 (H_kv, N_k) tensor with contiguous rows on q's device")
     ws_bytes = p.ws_bytes
