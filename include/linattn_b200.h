@@ -571,7 +571,7 @@ int64_t linattn_attention_mass_workspace(int64_t N_k, int64_t Hkv, int32_t n_spl
  * Heavy-hitter cache: `budget` slots per (sequence, kv head).  k, v (batch, n_kv_heads,
  * budget, head_dim), mass fp32 and pos int32 (batch, n_kv_heads, budget), seen int32
  * (batch): tokens taken so far, min(seen, budget) slots in use.  All contiguous, 16-byte
- * aligned.  sinks + recent <= budget, recent >= 1.  The eviction rule keeps what the
+ * aligned.  f16 or bf16, head_dim 64 or 128; sinks + recent <= budget, recent >= 1.  The eviction rule keeps what the
  * reference's eviction variants call heavy hitters (src/linattn/variants/eviction.py),
  * as a cache that holds nothing else.
  */

@@ -18,7 +18,9 @@
 // 20% slower: the schedule is then fixed, and the next keys wait for the last product.)  Keys
 // with the most queries (the first of a sequence) come first in the grid.
 // Bound: the exponentials (16 a clock and SM: 1024 clocks a tile, against 512 for its MMAs
-// at D = 128).
+// at D = 128), 3 of 8 of which go to the FMA pipe instead.  Measured (32 / 8 heads, D = 128, bf16):
+// 4096 tokens 92 us, 16384 tokens 1140 to 1290 us (850 to 960 TFLOP/s); FMA pipe 64%, exponential
+// unit 57% busy.
 #include <cstdio>
 #include <type_traits>
 

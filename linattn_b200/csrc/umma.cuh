@@ -129,16 +129,6 @@ __device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float max3_nan(float a, float b, float c) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
 // 2^x of two values x in [.., 127] on the FMA pipe, beside the exponential unit's 16 a clock:
 // x = n + f with n the nearest integer (added and taken off at 1.5 2^23, whose low bits then
 // hold n), 2^f by the degree-4 polynomial of least relative error on [-1/2, 1/2] (Remez
