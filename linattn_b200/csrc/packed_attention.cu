@@ -49,14 +49,17 @@ struct PackedArgs {
   const int32_t* cu_k;
   int64_t Nq, Nk;
   int S, Hq, Hkv, G, tokens;  // tokens of a row tile (floor(128 / G))
+  int inv_g;         // ceil(2^16 / G): (r inv_g) >> 16 = r / G for r < 128
   int causal;
   float scale_log2;
   void* out;
   int64_t ot, oh;
   float* lse;        // (N_q, H_q) or NULL
   int n_splits;
-  float* part_o;     // (n_splits, N_q, H_q, D)
-  float* part_lse;   // (n_splits, N_q, H_q)
+  // parts of a cut key range, rows next to one another as a row tile has them (row = token G + head
+  // of the group), so that a warp's rows are written and read together
+  float4* part_o;    // (n_splits, H_kv, D / 4, N_q G) four channels of a row
+  float* part_lse;   // (n_splits, H_kv, N_q G)
   int64_t items;     // at most: tiles x H_kv x n_splits
   int32_t* status;
 };
@@ -71,8 +74,9 @@ template <int D>
 struct PackedSmem {
   static constexpr int TILE = 128 * D * 2;           // Q, K or V tile
   static constexpr int KS = D == 128 ? 2 : 4;        // K ring stages
-  static constexpr int VS = D == 128 ? 3 : 4;        // V ring stages
-  static constexpr int BYTES = 1024 + TILE * (2 + KS + VS);
+  static constexpr int VS = D == 128 ? 2 : 4;        // V ring stages
+  static constexpr int OUT = 8 * 4096;               // outputs on their way: 32 rows x 64 channels a softmax warp
+  static constexpr int BYTES = 1024 + TILE * (2 + KS + VS) + OUT;
 };
 
 // One work item: two row tiles of a sequence, a kv head, a part of the keys.
@@ -460,7 +464,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     const int i = (warp >> 2) - 1, r = tid & 127;
     const uint32_t lane_addr = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
     const uint32_t s_addr = lane_addr + i * 128, o_addr = lane_addr + 256 + i * 128;
-    const int rt = r / p.G, rg = r - rt * p.G;
+    const int rt = (r * p.inv_g) >> 16, rg = r - rt * p.G;
     const float sl = p.scale_log2;
     const uint64_t sl2 = pack_f2(sl, sl);
     int sc = 0;  // score tiles so far
@@ -549,42 +553,82 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       const float inv = l != 0.f ? 1.f / l : 0.f;
       const float lse = l != 0.f ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
       const int64_t token = static_cast<int64_t>(w.q_first) + t;
-      const int head = w.kvh * p.G + rg;
       if (p.n_splits > 1) {
-        const int64_t row = w.split * (p.Nq * p.Hq) + token * p.Hq + head;
-        if (row_ok) p.part_lse[row] = lse;
+        const int64_t rows = p.Nq * p.G, at = token * p.G + rg;
+        const int64_t part = static_cast<int64_t>(w.split) * p.Hkv + w.kvh;
+        if (row_ok) p.part_lse[part * rows + at] = lse;
+        float4* dst = p.part_o + part * (D / 4) * rows + at;
 #pragma unroll 1
         for (int c = 0; c < (ni > 0 ? D / 32 : 0); ++c) {
           uint32_t ov[32];
           tmem_ld32(o_addr + c * 32, ov);
           tmem_wait_ld();
           if (row_ok) {
-            float4* dst = reinterpret_cast<float4*>(p.part_o + row * D + c * 32);
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-              dst[e] = make_float4(__uint_as_float(ov[4 * e]) * inv, __uint_as_float(ov[4 * e + 1]) * inv,
-                                   __uint_as_float(ov[4 * e + 2]) * inv, __uint_as_float(ov[4 * e + 3]) * inv);
+              dst[(c * 8 + e) * rows] =
+                  make_float4(__uint_as_float(ov[4 * e]) * inv, __uint_as_float(ov[4 * e + 1]) * inv,
+                              __uint_as_float(ov[4 * e + 2]) * inv, __uint_as_float(ov[4 * e + 3]) * inv);
           }
         }
       } else {
+        const int head = w.kvh * p.G + rg;
         if (row_ok && p.lse) p.lse[token * p.Hq + head] = lse;
-        // each thread writes its row, 64 bytes at a time
-        T* dst = static_cast<T*>(p.out) + token * p.ot + head * p.oh;
+        T* out = static_cast<T*>(p.out);
+        if (__all_sync(0xffffffffu, row_ok)) {
+          // 64 channels at a time through shared memory (16-byte pieces, swizzled by the row), then
+          // four whole rows a store; a row to a thread takes 32 lines a store (a prompt of 4096
+          // tokens 123.8 against 126.0 us, the batch of 12 sequences 116.7 against 121.3)
+          uint8_t* st = sv_ring + VS * TILE + (i * 4 + (warp & 3)) * 4096;
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t ov[32];
-          if (ni > 0) {  // warp-uniform
-            tmem_ld32(o_addr + c * 32, ov);
-            tmem_wait_ld();
-          }
-          if (row_ok) {
+          for (int c = 0; c < HALVES; ++c) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-              uint32_t y[4];
+              uint32_t ov[16];
+              if (ni > 0) {  // warp-uniform
+                tmem_ld16(o_addr + c * 64 + q * 16, ov);
+                tmem_wait_ld();
+              }
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                y[e] = l != 0.f ? M::pack(__uint_as_float(ov[q * 8 + 2 * e]) * inv, __uint_as_float(ov[q * 8 + 2 * e + 1]) * inv) : 0u;
-              *reinterpret_cast<uint4*>(dst + c * 32 + q * 8) = make_uint4(y[0], y[1], y[2], y[3]);
+              for (int h = 0; h < 2; ++h) {
+                uint32_t y[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  y[e] = l != 0.f ? M::pack(__uint_as_float(ov[h * 8 + 2 * e]) * inv, __uint_as_float(ov[h * 8 + 2 * e + 1]) * inv) : 0u;
+                *reinterpret_cast<uint4*>(st + lane * 128 + (((2 * q + h) ^ (lane & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
+              }
+            }
+            __syncwarp();
+            const int piece = lane & 7;
+#pragma unroll 4
+            for (int x = 0; x < 32; x += 4) {
+              const int rw = x + (lane >> 3), rr = 32 * (warp & 3) + rw, tt = (rr * p.inv_g) >> 16;  // rr / G
+              *reinterpret_cast<uint4*>(out + (static_cast<int64_t>(w.q_first) + w.t0 + i * p.tokens + tt) * p.ot +
+                                        (static_cast<int64_t>(w.kvh) * p.G + rr - tt * p.G) * p.oh + c * 64 + piece * 8) =
+                  *reinterpret_cast<const uint4*>(st + rw * 128 + ((piece ^ (rw & 7)) << 4));
+            }
+            __syncwarp();
+          }
+        } else if (__any_sync(0xffffffffu, row_ok)) {
+          // few rows: each thread writes its own, without the wait in between (27 rows of three
+          // sequences 9.0 us, by way of shared memory 9.5)
+          T* dst = out + token * p.ot + head * p.oh;
+#pragma unroll 1
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t ov[16];
+            if (ni > 0) {  // warp-uniform
+              tmem_ld16(o_addr + c * 16, ov);
+              tmem_wait_ld();
+            }
+            if (row_ok) {
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {
+                uint32_t y[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  y[e] = l != 0.f ? M::pack(__uint_as_float(ov[q * 8 + 2 * e]) * inv, __uint_as_float(ov[q * 8 + 2 * e + 1]) * inv) : 0u;
+                *reinterpret_cast<uint4*>(dst + c * 16 + q * 8) = make_uint4(y[0], y[1], y[2], y[3]);
+              }
             }
           }
         }
@@ -608,59 +652,58 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
-// Merge of the parts of a key range: D / 4 lanes a row, four channels a lane, every part's
-// weight 2^(lse_s - max) computed by the lanes together (at most 32 parts, one to a lane).
-// Part by part in their order.  (The row-per-CTA merge of the decode path took about half of
-// the call at thousands of rows.)
-constexpr int PM_THREADS = 256;
-
+// Merge of the parts of a key range: 32 rows to a block, a lane to a row, and 8 of their channels to
+// a warp.  A row's weights 2^(lse_s - max) are found by its lane in every warp; the parts are added
+// in their order.
 template <typename T, int D>
-__global__ void __launch_bounds__(PM_THREADS) packed_merge_kernel(const PackedArgs p) {
+__global__ void __launch_bounds__(4 * D) packed_merge_kernel(const PackedArgs p) {
   using M = MmaOp<T>;
-  constexpr int LANES = D / 4;
+  constexpr int QUADS = 2;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int64_t rows = p.Nq * p.Hq;
-  const int64_t row = (static_cast<int64_t>(blockIdx.x) * PM_THREADS + threadIdx.x) / LANES;
-  const int lane = threadIdx.x & 31, in = threadIdx.x % LANES, base = lane - in;
-  const bool there = row < rows;
-  // lanes of a row take its parts in turn: with 16 lanes to a row, two rounds
-  float mine[32 / LANES], mx = -INFINITY;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, kvh = blockIdx.y;
+  const int64_t rows = p.Nq * p.G, row = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+  if (row >= rows) return;
+  const float* lse = p.part_lse + kvh * rows + row;
+  const int64_t next = p.Hkv * rows;  // to the next part
+  float mx = -INFINITY, sum = 0.f;
+#pragma unroll 8
+  for (int s = 0; s < p.n_splits; ++s) mx = fmaxf(mx, lse[s * next]);
+  const float4* src = p.part_o + (static_cast<int64_t>(kvh) * (D / 4) + warp * QUADS) * rows + row;
+  float4 acc[QUADS];
 #pragma unroll
-  for (int e = 0; e < 32 / LANES; ++e) {
-    const int s = in + e * LANES;
-    mine[e] = there && s < p.n_splits ? p.part_lse[s * rows + row] : -INFINITY;
-    mx = fmaxf(mx, mine[e]);
-  }
+  for (int q = 0; q < QUADS; ++q) acc[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+  constexpr int STEP = 8;  // parts whose loads go out together
+  for (int s0 = 0; s0 < p.n_splits; s0 += STEP) {
+    // a part that reads nothing has no weight (its o is not written); one of NaN keeps it
+    float f[STEP];
+    float4 o[STEP][QUADS];
 #pragma unroll
-  for (int o = LANES / 2; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  float sum = 0.f;
+    for (int e = 0; e < STEP; ++e) {
+      const float part = s0 + e < p.n_splits ? lse[(s0 + e) * next] : -INFINITY;
+      f[e] = part == -INFINITY ? 0.f : ex2_approx((part - mx) * 1.4426950408889634f);
 #pragma unroll
-  for (int e = 0; e < 32 / LANES; ++e) {
-    // a part that reads nothing has no weight; one of NaN keeps it
-    mine[e] = mine[e] == -INFINITY ? 0.f : ex2_approx((mine[e] - mx) * 1.4426950408889634f);
-    sum += mine[e];
-  }
+      for (int q = 0; q < QUADS; ++q)
+        o[e][q] = part == -INFINITY ? make_float4(0.f, 0.f, 0.f, 0.f) : __ldg(src + (s0 + e) * (D / 4) * next + q * rows);
+    }
 #pragma unroll
-  for (int o = LANES / 2; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  const float4* src = reinterpret_cast<const float4*>(p.part_o) + row * LANES + in;
-#pragma unroll 4
-  for (int s = 0; s < p.n_splits; ++s) {
-    const float f = __shfl_sync(0xffffffffu, LANES == 32 || s < LANES ? mine[0] : mine[32 / LANES - 1], base + s % LANES);
-    if (there && f != 0.f) {
-      const float4 o = __ldg(src + static_cast<int64_t>(s) * rows * LANES);
-      acc.x += f * o.x;
-      acc.y += f * o.y;
-      acc.z += f * o.z;
-      acc.w += f * o.w;
+    for (int e = 0; e < STEP; ++e) {
+      sum += f[e];
+#pragma unroll
+      for (int q = 0; q < QUADS; ++q) {
+        acc[q].x += f[e] * o[e][q].x;
+        acc[q].y += f[e] * o[e][q].y;
+        acc[q].z += f[e] * o[e][q].z;
+        acc[q].w += f[e] * o[e][q].w;
+      }
     }
   }
-  if (!there) return;
   const float inv = sum != 0.f ? 1.f / sum : 0.f;
-  const int64_t token = row / p.Hq;
-  *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + token * p.ot + (row - token * p.Hq) * p.oh + in * 4) =
-      make_uint2(M::pack(acc.x * inv, acc.y * inv), M::pack(acc.z * inv, acc.w * inv));
-  if (p.lse && in == 0) p.lse[row] = sum != 0.f ? mx + logf(sum) : -INFINITY;
+  const int64_t token = row / p.G;
+  const int head = kvh * p.G + static_cast<int>(row - token * p.G);
+  T* dst = static_cast<T*>(p.out) + token * p.ot + head * p.oh + warp * QUADS * 4;
+  *reinterpret_cast<uint4*>(dst) = make_uint4(M::pack(acc[0].x * inv, acc[0].y * inv), M::pack(acc[0].z * inv, acc[0].w * inv),
+                                              M::pack(acc[1].x * inv, acc[1].y * inv), M::pack(acc[1].z * inv, acc[1].w * inv));
+  if (p.lse && warp == 0) p.lse[token * p.Hq + head] = sum != 0.f ? mx + logf(sum) : -INFINITY;
 }
 
 int packed_fail(int code, const char* what) {
@@ -681,9 +724,8 @@ cudaError_t launch_packed(const PackedArgs& p, const CUtensorMap& q, const CUten
   if (launched != cudaSuccess || p.n_splits == 1) return launched;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
-  const int64_t threads = p.Nq * p.Hq * (D / 4);
-  cfg.gridDim = dim3(static_cast<unsigned>((threads + PM_THREADS - 1) / PM_THREADS));
-  cfg.blockDim = dim3(PM_THREADS);
+  cfg.gridDim = dim3(static_cast<unsigned>((p.Nq * p.G + 31) / 32), static_cast<unsigned>(p.Hkv));
+  cfg.blockDim = dim3(4 * D);
   cfg.stream = st;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -706,9 +748,34 @@ using namespace linattn;
 extern "C" int32_t linattn_packed_attention_splits(int64_t N_q, int64_t Hq, int64_t Hkv, int64_t S, int64_t max_q,
                                                    int64_t max_k) {
   if (N_q < 1 || Hkv < 1 || Hq < Hkv || Hq / Hkv > 128 || S < 1 || max_q < 1) return 1;
-  const int64_t ctas = packed_tiles(N_q, Hq / Hkv, S, max_q) * Hkv;
-  // one wave of the GPU, with at least 4 key tiles to a part
-  return static_cast<int32_t>(lmax(1, lmin(lmin(sm_count() / lmax(1, ctas), (max_k + 127) / 128 / 4), 32)));
+  // Time of n parts to a key range, in key tiles of a work item (1.7 to 2 us): the longest item's, or
+  // what the items of a CTA come to where they are more; 1.5 for each item's start and end, and
+  // with parts 2.5 for the merge and their bytes, written and read (a tile's time moves 12
+  // MB).  The mean item reads what its sequence has before its queries and half of the rest;
+  // sequences are taken to be as unlike in keys as in queries.  Measured in us, by parts:
+  //   384 queries on 15737 keys, 2 kv heads, D = 64: 1: 197, 4: 61, 6: 47, 8: 65, 12: 52, 18: 54
+  //   1 query on 30000 keys, 8 kv heads, D = 128: 1: 437, 8: 67, 16: 44, 18: 44, 24: 57
+  //   700 queries on 3000 keys, 8 kv heads: 1: 64, 2: 72, 3: 63, 5: 71, 8: 83
+  //   prompts of 2118, 777, 283 and 315 tokens, 2 kv heads: 1: 43, 2: 35, 3: 30, 4: 30, 8: 36
+  //   a prompt of 1500 tokens, 8 kv heads: 1: 32, 2: 60
+  const double sms = sm_count(), items = static_cast<double>(packed_tiles(N_q, Hq / Hkv, S, max_q) * Hkv);
+  const double longest = (max_k + 127) / 128;
+  const double even = lmin(N_q, S * max_q) / static_cast<double>(S * max_q);
+  const double mean = even * (max_k - 0.5 * lmin(max_q, max_k)) / 128;
+  const double bytes = 1024.0 * N_q * Hq;
+  int best = 1;
+  double least = 0;
+  for (int n = 1; n <= 32 && n <= longest; ++n) {
+    const int64_t rounds = static_cast<int64_t>((items * n + sms - 1) / sms);
+    const double share = mean / n < 1 ? 1 : mean / n;
+    const double most = rounds * share > longest / n ? rounds * share : longest / n;
+    const double time = most + 1.5 * rounds + (n > 1 ? 2.5 + n * bytes / 12e6 : 0.0);
+    if (n == 1 || time < least) {
+      least = time;
+      best = n;
+    }
+  }
+  return best;
 }
 
 extern "C" int64_t linattn_packed_attention_workspace(int64_t N_q, int64_t Hq, int64_t D, int32_t n_splits) {
@@ -729,6 +796,7 @@ extern "C" int linattn_packed_attention(const void* q, const void* k, const void
   if (N_q < 0 || N_k < 0 || S < 0 || max_q < 0 || max_k < 0 || n_splits < 1)
     return packed_fail(LINATTN_EINVAL, "sizes must not be negative");
   if (N_q >= (int64_t(1) << 30) || N_k >= (int64_t(1) << 30)) return packed_fail(LINATTN_EUNSUPPORTED, "at most 2^30 rows");
+  if (n_splits > 1 && Hkv > 65535) return packed_fail(LINATTN_EUNSUPPORTED, "at most 65535 kv heads with parts");
   if (!(scale > 0.f) || scale > 1e30f) return packed_fail(LINATTN_EINVAL, "scale must be positive and finite");
   if (N_q == 0 || S == 0) return LINATTN_OK;
   if (!q || !out || (N_k > 0 && (!k || !v))) return packed_fail(LINATTN_EINVAL, "NULL pointer");
@@ -744,6 +812,7 @@ extern "C" int linattn_packed_attention(const void* q, const void* k, const void
   PackedArgs p;
   p.G = static_cast<int>(Hq / Hkv);
   p.tokens = 128 / p.G;
+  p.inv_g = (65536 + p.G - 1) / p.G;
   const CUtensorMapDataType cu = dtype == LINATTN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   CUtensorMap tq, tk, tv;
   const int64_t qd[3] = {D, Hq, N_q}, qs[2] = {q_strides[1] * 2, q_strides[0] * 2};
@@ -760,11 +829,11 @@ extern "C" int linattn_packed_attention(const void* q, const void* k, const void
   p.out = out; p.ot = out_strides[0]; p.oh = out_strides[1];
   p.lse = lse;
   p.n_splits = n_splits;
-  p.part_o = static_cast<float*>(workspace);
-  p.part_lse = n_splits > 1 ? p.part_o + n_splits * N_q * Hq * D : nullptr;
+  p.part_o = static_cast<float4*>(workspace);
+  p.part_lse = n_splits > 1 ? static_cast<float*>(workspace) + n_splits * N_q * Hq * D : nullptr;
   p.status = status;
   const int64_t tiles = packed_tiles(N_q, p.G, S, max_q);
-  if (Hkv * static_cast<int64_t>(n_splits) >= (int64_t(1) << 31) || n_splits > 32) return packed_fail(LINATTN_EUNSUPPORTED, "too many tiles, or more than 32 splits");
+  if (Hkv > 65535 || n_splits > 32) return packed_fail(LINATTN_EUNSUPPORTED, "more than 65535 kv heads, or than 32 splits");
   if (tiles == 0) return LINATTN_OK;
   p.items = tiles * Hkv * n_splits;
   const unsigned grid = static_cast<unsigned>(lmin(sm_count(), p.items));
