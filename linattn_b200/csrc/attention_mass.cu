@@ -338,14 +338,20 @@ extern "C" int32_t linattn_attention_mass_splits(int64_t Hq, int64_t Hkv, int64_
                                                  int64_t window) {
   if (Hkv < 1 || Hq < Hkv || S < 1 || max_q < 1 || max_k < 1) return 1;
   const int64_t tokens = lmax(1, 128 / (Hq / Hkv));
-  const int64_t ctas = S * ((max_k + MT_KEYS - 1) / MT_KEYS) * Hkv;
+  // all but the longest sequence are taken to be half as long
+  const int64_t ctas = (((S + 1) * ((max_k + MT_KEYS - 1) / MT_KEYS) + 1) / 2) * Hkv;
   const int64_t q_tiles = ((window > 0 ? lmin(window, max_q) : max_q) + tokens - 1) / tokens;
   const int64_t sms = sm_count();
-  // CTAs differ in length (causal), so a few rounds of the GPU (4096 tokens, D = 128: 2 / 3 / 4 /
-  // 6 rounds 91 / 92 / 96 / 103 us; 8192 tokens, D = 64: 315 / 299 / 301 / 304); at least 8
-  // query tiles to a split
+  // CTAs differ in length (causal), so a few rounds of the GPU: two where one split leaves SMs
+  // idle, else three (4096 tokens, D = 128: 2 / 3 / 4 / 6 rounds 91 / 92 / 96 / 103 us; 8192
+  // tokens, D = 64: 315 / 299 / 301 / 304).  At least 2 query tiles to a split.  Measured in us,
+  // by splits:
+  //   a prompt of 1500 tokens, 8 kv heads of 32: 1: 105, 5: 32, 8: 25, 12: 27, 16: 29
+  //   ten prompts of 5 to 923 tokens, 2 kv heads of 8: 1: 63, 3: 30, 6: 20, 8: 18, 12: 19
+  //   prompts of 385 and 232 tokens, 4 kv heads of 20: 1: 33, 4: 16, 8: 12, 16: 11
   if (ctas >= 3 * sms) return 1;
-  return static_cast<int32_t>(lmax(1, lmin(lmin((3 * sms + ctas - 1) / ctas, q_tiles / 8), 64)));
+  const int64_t rounds = ctas < sms ? 2 : 3;
+  return static_cast<int32_t>(lmax(1, lmin(lmin((rounds * sms + ctas - 1) / ctas, q_tiles / 2), 64)));
 }
 
 extern "C" int64_t linattn_attention_mass_workspace(int64_t N_k, int64_t Hkv, int32_t n_splits) {

@@ -110,6 +110,18 @@ def test_packed_attention(cuda, case, splits):
         assert torch.equal(again, o) and torch.equal(lse2, lse)
 
 
+@pytest.mark.parametrize("splits", [8, 9, 32])
+@pytest.mark.parametrize("hq,hkv,d,dtype", [(6, 2, 128, torch.float16), (5, 1, 64, torch.bfloat16)])
+def test_packed_attention_many_parts(cuda, splits, hq, hkv, d, dtype):
+    """Parts of one key tile, and parts that are left without any."""
+    from linattn_b200 import packed_attention
+
+    lq, lk = [7, 130, 0, 33], [3000, 140, 5, 20]
+    q, k, v = _inputs(splits, lq, lk, hq, hkv, d, dtype)
+    o, lse = packed_attention(q, k, v, _cu(lq), _cu(lk), n_splits=splits)
+    _check_attention(o, lse, q, k, v, lq, lk, d ** -0.5, True)
+
+
 def test_packed_attention_growing_scores(cuda):
     """Scores that keep rising move the running maximum on every key tile."""
     from linattn_b200 import packed_attention
@@ -216,6 +228,21 @@ def test_attention_mass(cuda, case, window, splits):
                            n_splits=splits if splits else 1)
     if splits:
         assert torch.equal(again, got)
+
+
+@pytest.mark.parametrize("lens,hq,hkv,d", [([600, 30, 250], 8, 2, 128), ([385, 232], 20, 4, 64), ([900], 16, 1, 128)])
+def test_mass_of_chosen_splits(cuda, lens, hq, hkv, d):
+    """The chosen number of splits, one, and as many as query tiles give the same sums."""
+    from linattn_b200 import attention_mass, packed_attention
+
+    q, k, v = _inputs(21, lens, lens, hq, hkv, d, torch.float16)
+    cu = _cu(lens)
+    _, lse = packed_attention(q, k, v, cu, max_q=max(lens), max_k=max(lens))
+    one = attention_mass(q, k, lse, cu, max_q=max(lens), max_k=max(lens), n_splits=1).double()
+    for splits in (None, 13, 64):
+        got = attention_mass(q, k, lse, cu, max_q=max(lens), max_k=max(lens), n_splits=splits).double()
+        # fp32 sums of the same positive terms in another order: each rounds at most once a term
+        assert ((got - one).abs() <= 2 * max(lens) * (hq // hkv) * 2.0 ** -24 * one).all()
 
 
 def test_mass_sums_to_the_queries(cuda):
