@@ -19,7 +19,9 @@
 // that one CTA has whole keeps its scores in tensor memory, which this kernel has no other use
 // for: a warp stores its accumulator fragments as they are, 4 columns a tile, and the mass warp
 // of the same 32 lanes reads them back (4096 slots a unit for up to 8 heads, twice over; through
-// the workspace in global memory the call took 168 us instead of 162).  Longer ones, and
+// the workspace in global memory the call took 168 us instead of 162).  When a CTA has no more
+// tiles, its other eight warps help with the masses of its last unit (7 units of 1978 slots on 8
+// heads, D = 64: 17 us; with four warps and scores that are not read as 16 bytes 23).  Longer ones, and
 // units that several CTAs share, go through the workspace; the last CTA to arrive at a shared
 // unit merges its (o, m, l): the parts are added in their order, whoever does it, so results do
 // not depend on it.
@@ -45,7 +47,8 @@ struct HeavyAttendArgs {
   int h0, heads;     // heads [h0, h0 + heads) of every group in this launch
   float scale_log2;
   int accumulate;
-  float* scores;     // (B * H, heads, M) log2-domain scores
+  int Ms;            // M up to a multiple of 4
+  float* scores;     // (B * H, heads, Ms) log2-domain scores
   float* part_o;     // (CTAs, 2, HN, D) unnormalised o of units that this CTA shares
   float* part_ml;    // (CTAs, 2, 2, HN) their maxima and sums
   int32_t* ticket;   // (B * H) zeros: arrivals at a shared unit
@@ -124,6 +127,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
   __shared__ int64_t job_unit[2];
   __shared__ int job_count[2];  // slots in use, or -1: no more
   __shared__ int job_tmem[2];   // scores in tensor memory
+  __shared__ int job_next[2];   // else: the slots / 4 that warps have taken
+  __shared__ int job_last[2];   // the CTA's last unit: the tile warps take part
   __shared__ uint32_t tmem_sh;
   __shared__ float upper[D == 64 ? 4 * 32 * 4 * NT : 1];  // D = 64: o of the tile's upper slots
   __shared__ int dead, arrived;
@@ -254,9 +259,128 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     return;
   }
 
+  // A finished unit's weights into its masses, by four warps (group) of each of the groups.
+  auto add_tmem = [&](int x, int64_t unit, int count, int group, int groups) {
+    float* mass = a.mass + unit * a.M;
+    // this lane's scores of a tile: slots g and g + 8 of the two warps of its quarter, heads
+    // 2 tig and 2 tig + 1 (of every 8)
+    const int g = lane >> 2, tig = lane & 3, quarter = warp & 3;
+    float f0[NT][2], f1[NT][2];
+#pragma unroll
+    for (int y = 0; y < NT; ++y)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int head = y * 8 + 2 * tig + e;
+        f0[y][e] = fin[x][0][head];
+        f1[y][e] = head < a.heads ? fin[x][1][head] : 0.f;
+      }
+    constexpr int STEP = NT >= 4 ? 1 : 4 / NT;  // tiles of 16 columns
+    constexpr int BATCH = 2 * STEP;             // tiles whose masses are fetched together
+    const int tiles = (count + AT_ROWS - 1) / AT_ROWS;
+    for (int i0 = group * BATCH; i0 < tiles; i0 += groups * BATCH) {
+      // lane tig = 0 owns slot g, tig = 1 slot g + 8
+      const int n0 = i0 * AT_ROWS + 16 * quarter + g + 8 * tig;
+      float old[2][BATCH];
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int e = 0; e < BATCH; ++e) {
+          const int n = n0 + 64 * half + e * AT_ROWS;
+          old[half][e] = tig < 2 && n < count ? mass[n] : 0.f;
+        }
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int s0 = 0; s0 < BATCH; s0 += STEP) {
+          if (i0 + s0 >= tiles) continue;
+          uint32_t sv[16];
+          tmem_ld16(tmem + (static_cast<uint32_t>(32 * quarter) << 16) + x * 256 + half * 128 + (i0 + s0) * 4 * NT, sv);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < STEP; ++e) {
+            float lo = 0.f, hi = 0.f;
+#pragma unroll
+            for (int y = 0; y < NT; ++y)
+#pragma unroll
+              for (int z = 0; z < 2; ++z) {
+                lo += ex2_approx(__uint_as_float(sv[((e * NT + y) * 4 + z) & 15]) - f0[y][z]) * f1[y][z];
+                hi += ex2_approx(__uint_as_float(sv[((e * NT + y) * 4 + 2 + z) & 15]) - f0[y][z]) * f1[y][z];
+              }
+            lo += __shfl_xor_sync(0xffffffffu, lo, 1);
+            hi += __shfl_xor_sync(0xffffffffu, hi, 1);
+            lo += __shfl_xor_sync(0xffffffffu, lo, 2);
+            hi += __shfl_xor_sync(0xffffffffu, hi, 2);
+            const int n = n0 + 64 * half + (s0 + e) * AT_ROWS;
+            if (tig < 2 && n < count) mass[n] = old[half][s0 + e] + (tig == 0 ? lo : hi);
+          }
+        }
+    }
+  };
+  // The same from the workspace; warps take 256 slots at a time.
+  auto add_scores = [&](int x, int64_t unit, int count) {
+    constexpr int U = 2;  // times 4 slots a thread, their loads together
+    float* mass = a.mass + unit * a.M;
+    const float4* sc = reinterpret_cast<const float4*>(a.scores + unit * a.heads * a.Ms);
+    const int quads = (count + 3) >> 2, stride = a.Ms >> 2;
+    const bool aligned = (a.M & 3) == 0;  // rows of masses on 16 bytes
+    for (;;) {
+      int n0 = 0;
+      if (lane == 0) n0 = atomicAdd(&job_next[x], 32 * U);
+      n0 = __shfl_sync(0xffffffffu, n0, 0);
+      if (n0 >= quads) break;
+      n0 += lane;
+      float v[U][4];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int n = (n0 + u * 32) * 4;
+        if (aligned) {
+          const float4 y = n < count ? *reinterpret_cast<const float4*>(mass + n) : make_float4(0.f, 0.f, 0.f, 0.f);
+          v[u][0] = y.x;
+          v[u][1] = y.y;
+          v[u][2] = y.z;
+          v[u][3] = y.w;
+        } else {
+#pragma unroll
+          for (int z = 0; z < 4; ++z) v[u][z] = n + z < count ? mass[n + z] : 0.f;
+        }
+      }
+      for (int h0 = 0; h0 < a.heads; h0 += 4) {
+        float4 y[U][4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (h0 + e < a.heads && n0 + u * 32 < quads) y[u][e] = __ldcg(sc + static_cast<int64_t>(h0 + e) * stride + n0 + u * 32);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (h0 + e < a.heads) {
+            const float f0 = fin[x][0][h0 + e], f1 = fin[x][1][h0 + e];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+              const int n = (n0 + u * 32) * 4;  // slots past the count keep what they hold
+              if (n < count) v[u][0] += ex2_approx(y[u][e].x - f0) * f1;
+              if (n + 1 < count) v[u][1] += ex2_approx(y[u][e].y - f0) * f1;
+              if (n + 2 < count) v[u][2] += ex2_approx(y[u][e].z - f0) * f1;
+              if (n + 3 < count) v[u][3] += ex2_approx(y[u][e].w - f0) * f1;
+            }
+          }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int n = (n0 + u * 32) * 4;
+        if (aligned) {
+          if (n < count) *reinterpret_cast<float4*>(mass + n) = make_float4(v[u][0], v[u][1], v[u][2], v[u][3]);
+        } else {
+#pragma unroll
+          for (int z = 0; z < 4; ++z)
+            if (n + z < count) mass[n + z] = v[u][z];
+        }
+      }
+    }
+  };
+
   if (warp > AT_WARPS) {
     if (!a.accumulate) return;
-    const int at = tid - 32 * (AT_WARPS + 1);
     for (int job = 0;; ++job) {
       const int x = job & 1;
       const bool there = warp_wait(&job_full[x], static_cast<uint32_t>((job >> 1) & 1));
@@ -264,111 +388,17 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
       const int count = there ? job_count[x] : -1;
       if (count < 0) break;
       const int64_t unit = job_unit[x];
-      float* mass = a.mass + unit * a.M;
-      const float* sc = a.scores + unit * a.heads * a.M;
       if (job_tmem[x]) {
-        // this lane's scores of a tile: slots g and g + 8 of the two warps of its quarter, heads
-        // 2 tig and 2 tig + 1 (of every 8)
         tc_fence_after();
-        const int g = lane >> 2, tig = lane & 3, quarter = warp & 3;
-        float f0[NT][2], f1[NT][2];
-#pragma unroll
-        for (int y = 0; y < NT; ++y)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int head = y * 8 + 2 * tig + e;
-            f0[y][e] = fin[x][0][head];
-            f1[y][e] = head < a.heads ? fin[x][1][head] : 0.f;
-          }
-        constexpr int STEP = NT >= 4 ? 1 : 4 / NT;  // tiles of 16 columns
-        constexpr int BATCH = 2 * STEP;             // tiles whose masses are fetched together
-        const int tiles = (count + AT_ROWS - 1) / AT_ROWS;
-        for (int i0 = 0; i0 < tiles; i0 += BATCH) {
-          // lane tig = 0 owns slot g, tig = 1 slot g + 8
-          const int n0 = i0 * AT_ROWS + 16 * quarter + g + 8 * tig;
-          float old[2][BATCH];
-#pragma unroll
-          for (int half = 0; half < 2; ++half)
-#pragma unroll
-            for (int e = 0; e < BATCH; ++e) {
-              const int n = n0 + 64 * half + e * AT_ROWS;
-              old[half][e] = tig < 2 && n < count ? mass[n] : 0.f;
-            }
-#pragma unroll
-          for (int half = 0; half < 2; ++half)
-#pragma unroll
-            for (int s0 = 0; s0 < BATCH; s0 += STEP) {
-              if (i0 + s0 >= tiles) continue;
-              uint32_t sv[16];
-              tmem_ld16(tmem + (static_cast<uint32_t>(32 * quarter) << 16) + x * 256 + half * 128 + (i0 + s0) * 4 * NT, sv);
-              tmem_wait_ld();
-#pragma unroll
-              for (int e = 0; e < STEP; ++e) {
-                float lo = 0.f, hi = 0.f;
-#pragma unroll
-                for (int y = 0; y < NT; ++y)
-#pragma unroll
-                  for (int z = 0; z < 2; ++z) {
-                    lo += ex2_approx(__uint_as_float(sv[((e * NT + y) * 4 + z) & 15]) - f0[y][z]) * f1[y][z];
-                    hi += ex2_approx(__uint_as_float(sv[((e * NT + y) * 4 + 2 + z) & 15]) - f0[y][z]) * f1[y][z];
-                  }
-                lo += __shfl_xor_sync(0xffffffffu, lo, 1);
-                hi += __shfl_xor_sync(0xffffffffu, hi, 1);
-                lo += __shfl_xor_sync(0xffffffffu, lo, 2);
-                hi += __shfl_xor_sync(0xffffffffu, hi, 2);
-                const int n = n0 + 64 * half + (s0 + e) * AT_ROWS;
-                if (tig < 2 && n < count) mass[n] = old[half][s0 + e] + (tig == 0 ? lo : hi);
-              }
-            }
-        }
+        add_tmem(x, unit, count, 0, job_last[x] ? 3 : 1);
         tc_fence_before();
-      } else if ((a.M & 3) == 0) {  // rows on 16 bytes: 8 slots a thread at a time, the loads together
-        constexpr int U = 2;
-        const int quads = (count + 3) >> 2, stride = a.M >> 2;
-        for (int n0 = at; n0 < quads; n0 += U * AT_MASS) {
-          float4 v[U];
-#pragma unroll
-          for (int u = 0; u < U; ++u)
-            v[u] = n0 + u * AT_MASS < quads ? reinterpret_cast<const float4*>(mass)[n0 + u * AT_MASS] : make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int h0 = 0; h0 < a.heads; h0 += 4) {
-            float4 y[U][4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-              for (int u = 0; u < U; ++u)
-                if (h0 + e < a.heads && n0 + u * AT_MASS < quads)
-                  y[u][e] = __ldcg(reinterpret_cast<const float4*>(sc) + static_cast<int64_t>(h0 + e) * stride + n0 + u * AT_MASS);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (h0 + e < a.heads) {
-                const float f0 = fin[x][0][h0 + e], f1 = fin[x][1][h0 + e];
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                  const int n = (n0 + u * AT_MASS) * 4;  // slots past the count keep what they hold
-                  if (n < count) v[u].x += ex2_approx(y[u][e].x - f0) * f1;
-                  if (n + 1 < count) v[u].y += ex2_approx(y[u][e].y - f0) * f1;
-                  if (n + 2 < count) v[u].z += ex2_approx(y[u][e].z - f0) * f1;
-                  if (n + 3 < count) v[u].w += ex2_approx(y[u][e].w - f0) * f1;
-                }
-              }
-          }
-#pragma unroll
-          for (int u = 0; u < U; ++u)
-            if (n0 + u * AT_MASS < quads) reinterpret_cast<float4*>(mass)[n0 + u * AT_MASS] = v[u];
-        }
       } else {
-        for (int n = at; n < count; n += AT_MASS) {
-          float v = mass[n];
-#pragma unroll 4
-          for (int head = 0; head < a.heads; ++head)
-            v += ex2_approx(__ldcg(sc + static_cast<int64_t>(head) * a.M + n) - fin[x][0][head]) * fin[x][1][head];
-          mass[n] = v;
-        }
+        add_scores(x, unit, count);
       }
       mbar_arrive(&job_empty[x]);
     }
     tc_fence_before();
-    asm volatile("barrier.cta.sync 2, 128;" ::: "memory");  // the other mass warps have read theirs
+    asm volatile("barrier.cta.sync 2, 384;" ::: "memory");  // the other warps have read theirs
     if (warp == AT_WARPS + 1) free_tmem();
     return;
   }
@@ -382,22 +412,25 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
   const int vrow = (lane & 7) + ((lane >> 4) & 1) * 8, vchunk = ct * 2 + ((lane >> 3) & 1);
   const uint32_t k_off = krow * 128, v_off = HALVES * SM::HALF + (vchunk >> 3) * SM::HALF;
   int j = 0, jobs = 0;
-  bool ok = true;
+  bool ok = true, help = false;
   // room for a unit's result: the mass warps are done with the one before the last
   auto job_room = [&] {
     if (a.accumulate && jobs >= 2 && ok)
       ok = __all_sync(0xffffffffu, mbar_wait_bounded(&job_empty[jobs & 1], static_cast<uint32_t>((jobs / 2 - 1) & 1)));
     tc_fence_after();
   };
-  auto job_send = [&](int64_t unit, int count, bool in_tmem) {  // one thread, after a barrier
+  auto job_send = [&](int64_t unit, int count, bool in_tmem, bool last) {  // one thread, after a barrier
     job_unit[jobs & 1] = unit;
     job_count[jobs & 1] = count;
     job_tmem[jobs & 1] = in_tmem ? 1 : 0;
+    job_next[jobs & 1] = 0;
+    job_last[jobs & 1] = last ? 1 : 0;
     mbar_arrive(&job_full[jobs & 1]);
   };
   for (int64_t t = t0; t < t1;) {
     const int end = static_cast<int>(lmin(w.tiles, first + (t1 - t)));
     const bool whole = first == 0 && end == w.tiles;  // else several CTAs share the unit
+    const bool last = t + (end - first) >= t1;        // of this CTA
     const int64_t unit = static_cast<int64_t>(w.b) * a.H + w.h;
     // q as the B operand: channels 16 kk + 2 tig (+ 1, + 8, + 9) of head g
     uint32_t q[NT][D / 16][2];
@@ -417,7 +450,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
       m[x][0] = m[x][1] = -INFINITY;
       l[x][0] = l[x][1] = 0.f;
     }
-    float* sc = a.scores + unit * a.heads * a.M;
+    float* sc = a.scores + unit * a.heads * a.Ms;
     const int64_t u0 = t - first, u1 = u0 + w.tiles;                       // the unit's tiles among all
     const int64_t c0 = ((u0 + 1) * nc - 1) / total, c1 = (u1 * nc - 1) / total;  // the CTAs that share it
     const bool in_tmem = a.accumulate && whole && w.tiles * NT <= 32 && NT <= 2;
@@ -450,7 +483,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
           const int r = e < 2 ? r0 : r1, head = x * 8 + 2 * tig + (e & 1);
           const float v = r < valid ? (s[x][e] + s2[x][e]) * a.scale_log2 : -INFINITY;
           s[x][e] = v;
-          if (a.accumulate && !in_tmem && r < valid && head < a.heads) sc[static_cast<int64_t>(head) * a.M + i * AT_ROWS + r] = v;
+          if (a.accumulate && !in_tmem && r < valid && head < a.heads) sc[static_cast<int64_t>(head) * a.Ms + i * AT_ROWS + r] = v;
           grow |= v > m[x][e & 1] + 8.f;
         }
       if (in_tmem) {
@@ -665,7 +698,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
           }
         }
         attend_barrier();
-        if (a.accumulate && tid == 0) job_send(unit, w.count, false);  // the masses beside the merge of o
+        if (a.accumulate && tid == 0) job_send(unit, w.count, false, last);  // the masses beside the merge of o
         // groups of threads over the parts, four channels a thread
         const int quads = a.heads * (D / 4), groups = max(1, 32 * AT_WARPS / quads);
         for (int y0 = 0; y0 < quads; y0 += 32 * AT_WARPS) {
@@ -695,7 +728,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
       }
     }
     if (finish && a.accumulate) {
-      if (whole && tid == 0) job_send(unit, w.count, in_tmem);
+      if (whole && tid == 0) job_send(unit, w.count, in_tmem, last);
+      help = last;
       ++jobs;
     }
     t += end - first;
@@ -704,7 +738,16 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
   }
   if (a.accumulate) {
     job_room();
-    if (tid == 0) job_send(0, -1, false);
+    if (tid == 0) job_send(0, -1, false, false);
+    attend_barrier();
+    if (help) {  // with the masses of the last unit
+      const int x = (jobs - 1) & 1;
+      tc_fence_after();
+      if (job_tmem[x]) add_tmem(x, job_unit[x], job_count[x], 1 + (warp >> 2), 3);
+      else add_scores(x, job_unit[x], job_count[x]);
+      tc_fence_before();
+    }
+    asm volatile("barrier.cta.sync 2, 384;" ::: "memory");
   }
   if (!ok && lane == 0) {
     report(a.status, LINATTN_DEV_TIMEOUT);
@@ -763,7 +806,7 @@ int64_t attend_ctas(int64_t units, int64_t budget) { return lmin(lmin(sm_count()
 extern "C" int64_t linattn_heavy_attend_workspace(int64_t batch, int64_t Hq, int64_t Hkv, int64_t budget) {
   if (batch < 1 || Hkv < 1 || Hq < Hkv || budget < 1) return 0;
   const int64_t heads = lmin(Hq / Hkv, AT_HEADS), hn = 8 * attend_nt(heads);
-  return batch * Hkv * heads * budget * 4 + sm_count() * 2 * hn * (128 + 2) * 4 + 64;
+  return batch * Hkv * heads * ((budget + 3) / 4 * 4) * 4 + sm_count() * 2 * hn * (128 + 2) * 4 + 64;
 }
 
 namespace {
@@ -833,6 +876,7 @@ extern "C" int linattn_heavy_attend(const linattn_heavy_t* cache, const void* q,
   a.B = cache->batch;
   a.H = cache->n_kv_heads;
   a.M = cache->budget;
+  a.Ms = (cache->budget + 3) / 4 * 4;
   a.G = static_cast<int>(Hq / cache->n_kv_heads);
   a.scale_log2 = scale * 1.4426950408889634f;
   a.accumulate = accumulate ? 1 : 0;

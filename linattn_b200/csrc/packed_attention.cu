@@ -578,7 +578,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         if (__all_sync(0xffffffffu, row_ok)) {
           // 64 channels at a time through shared memory (16-byte pieces, swizzled by the row), then
           // four whole rows a store; a row to a thread takes 32 lines a store (a prompt of 4096
-          // tokens 123.8 against 126.0 us, the batch of 12 sequences 116.7 against 121.3)
+          // tokens 123.8 against 126.0 us, a batch of 9 sequences 116.7 against 121.3)
           uint8_t* st = sv_ring + VS * TILE + (i * 4 + (warp & 3)) * 4096;
 #pragma unroll 1
           for (int c = 0; c < HALVES; ++c) {

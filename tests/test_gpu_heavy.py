@@ -235,6 +235,27 @@ def test_attend_shares(cuda, batch, budget, hq):
         _check_attend(cache, q, o, before, cache.mass, 1 / math.sqrt(d), True)
 
 
+@pytest.mark.parametrize("budget,hq,dtype", [(1024, 4, torch.bfloat16), (1023, 16, torch.float16), (4222, 4, torch.float16),
+                                             (301, 32, torch.bfloat16), (2050, 64, torch.bfloat16)])
+def test_attend_whole_units(cuda, budget, hq, dtype):
+    """As many full units as the GPU has SMs, twice: every CTA has whole ones, its last among them."""
+    from linattn_b200 import HeavyCache
+
+    hkv, d = 4, 128
+    batch = max(1, torch.cuda.get_device_properties(0).multi_processor_count * 2 // hkv)
+    g = torch.Generator(device="cuda").manual_seed(budget)
+    cache = HeavyCache(batch, hkv, d, budget, dtype=dtype)
+    cache.k.normal_(generator=g)
+    cache.v.normal_(generator=g)
+    cache.mass.uniform_(generator=g)
+    cache.seen.fill_(budget)
+    q = torch.randn(batch, hq, 1, d, generator=g, device="cuda").to(dtype)
+    for _ in range(2):
+        before = cache.mass.clone()
+        o = cache.attend(q)
+        _check_attend(cache, q, o, before, cache.mass, 1 / math.sqrt(d), True)
+
+
 def test_unaligned_rows(cuda):
     """Rows off the 16-byte grid and channels that are not next to one another are copied first."""
     from linattn_b200 import HeavyCache
