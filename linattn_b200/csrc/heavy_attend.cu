@@ -13,18 +13,21 @@
 // half of them), so that o is not spread over warps; one barrier a tile.  P is split into
 // hi + lo 16-bit parts (to ~2^-16), so o carries its own rounding only.
 //
-// The masses need a unit's final lse, so its scores are kept until then, and four more warps add
-// a finished unit's weights while the others go on with the next one (done by the same warps,
-// through global memory, it cost 59 of 205 us at 64 sequences x 8 heads x 4096 slots).  A unit
-// that one CTA has whole keeps its scores in tensor memory, which this kernel has no other use
-// for: a warp stores its accumulator fragments as they are, 4 columns a tile, and the mass warp
-// of the same 32 lanes reads them back (4096 slots a unit for up to 8 heads, twice over; through
-// the workspace in global memory the call took 168 us instead of 162).  When a CTA has no more
-// tiles, its other eight warps help with the masses of its last unit (7 units of 1978 slots on 8
-// heads, D = 64: 17 us; with four warps and scores that are not read as 16 bytes 23).  Longer ones, and
-// units that several CTAs share, go through the workspace; the last CTA to arrive at a shared
-// unit merges its (o, m, l): the parts are added in their order, whoever does it, so results do
-// not depend on it.
+// The masses need a unit's final lse, so its scores are kept until then, and four more warps
+// finish a unit while the others go on with the next one (done by the same warps, through global
+// memory, the masses cost 59 of 205 us at 64 sequences x 8 heads x 4096 slots).  A unit that one
+// CTA has whole keeps its scores in tensor memory, which this kernel has no other use for: a warp
+// stores its accumulator fragments as they are, 4 columns a tile, and the finishing warp of the
+// same 32 lanes reads them back (4096 slots a unit for up to 8 heads, twice over; through the
+// workspace in global memory the call took 168 us instead of 162).  Longer ones, and units that
+// several CTAs share, go through the workspace.  A shared unit's (o, m, l) are merged by the
+// finishing warps of the last CTA to arrive at it: the parts are added in their order, whoever
+// does it, so results do not depend on it.  When a CTA has no more tiles, its other eight warps
+// help with its last unit.  Sequences x heads x slots in us, with the merge done by the warps that
+// have the tiles / by the finishing warps (bf16, 4 query heads to a kv head):
+//   1 x 8 x 2048, D = 128: 11.8 / 10.7     2 x 8 x 2048: 14.7 / 12.7     8 x 8 x 2048: 20.0 / 18.4
+//   64 x 8 x 512: 37.8 / 33.9              12 x 8 x 4096: 44.8 / 47.0    64 x 8 x 4096: 157 / 156
+//   24 x 8 x 1978, D = 64: 31.6 / 29.0     64 x 8 x 1978: 60.8 / 55.7
 #include <cstdio>
 #include <cstring>
 #include <type_traits>
@@ -55,13 +58,13 @@ struct HeavyAttendArgs {
   int32_t* status;
 };
 
-constexpr int AT_WARPS = 8;                     // on tiles; then one that loads, and the mass warps
-constexpr int AT_MASS = 128;                    // threads that add the masses
-constexpr int AT_THREADS = 32 * (AT_WARPS + 1) + AT_MASS;
+constexpr int AT_WARPS = 8;                     // on tiles; then one that loads, and the finishing warps
+constexpr int AT_FINISH = 128;                  // threads that finish units
+constexpr int AT_THREADS = 32 * (AT_WARPS + 1) + AT_FINISH;
 constexpr int AT_ROWS = 128;                    // slots of a tile
 constexpr int AT_BOX = 128;                     // slots of one tensor-map box
 constexpr int AT_PROW = AT_ROWS * 2 + 16;       // bytes of a row of P: banks apart
-constexpr int AT_PARTS = 192;                   // CTAs that may share a unit: more than the GPU has SMs
+constexpr int AT_PARTS = 160;                   // CTAs that may share a unit: more than the GPU has SMs
 
 template <int D, int NT>
 struct AttendSmem {
@@ -70,9 +73,8 @@ struct AttendSmem {
   static constexpr int STAGE = 2 * (D / 64) * HALF;       // K then V
   static constexpr int STAGES = D == 64 ? (NT == 4 ? 4 : 6) : NT == 4 ? 2 : 3;
   static constexpr int P = 2 * 2 * HN * AT_PROW;          // [buffer][hi, lo][head][slot]
-  // merge of a shared unit: weights of its parts, sums of its thread groups
-  static constexpr int MERGE = (AT_PARTS * HN + (HN * D > 1024 ? HN * D : 1024)) * 4;
-  static constexpr int BYTES = 1024 + STAGES * STAGE + (P > MERGE ? P : MERGE);
+  static constexpr int WEIGHTS = AT_PARTS * HN * 4;       // of the parts of a shared unit
+  static constexpr int BYTES = 1024 + STAGES * STAGE + P + WEIGHTS;
 };
 
 // The units of one CTA's share of the tiles, in order.
@@ -108,6 +110,18 @@ __device__ __forceinline__ void tmem_st4(uint32_t taddr, const float (&v)[4]) {
                "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3]))
                : "memory");
 }
+// The finishing warps'.
+__device__ __forceinline__ void finish_barrier() { asm volatile("barrier.cta.sync 3, 128;" ::: "memory"); }
+__device__ __forceinline__ bool finish_barrier_and(bool x) {
+  int r = x ? 1 : 0;
+  asm volatile(
+      "{\n\t.reg .pred a, b;\n\tsetp.ne.s32 a, %0, 0;\n\t"
+      "barrier.cta.red.and.pred b, 3, 128, a;\n\tselp.s32 %0, 1, 0, b;\n\t}"
+      : "+r"(r)
+      :
+      : "memory");
+  return r != 0;
+}
 __device__ __forceinline__ void attend_barrier() { asm volatile("barrier.cta.sync 1, 256;" ::: "memory"); }
 
 template <typename T, int D, int NT>
@@ -120,18 +134,21 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
   extern __shared__ __align__(128) uint8_t atsmem_raw[];
   uint8_t* ring = atsmem_raw + ((1024 - (smem_u32(atsmem_raw) & 1023)) & 1023);
   uint8_t* pbuf = ring + ST * SM::STAGE;
+  float* weights_sh = reinterpret_cast<float*>(pbuf + SM::P);  // [part][head]
   __shared__ __align__(8) uint64_t full[ST], empty[ST], job_full[2], job_empty[2];
   __shared__ float mx_w[AT_WARPS][HN], l_w[AT_WARPS][HN];
-  // finished units on their way to the mass warps: maxima and reciprocal sums of the heads
+  // units on their way to the finishing warps: maxima and reciprocal sums of the heads
   __shared__ float fin[2][2][HN];
   __shared__ int64_t job_unit[2];
-  __shared__ int job_count[2];  // slots in use, or -1: no more
+  __shared__ int64_t job_out[2];  // of its outputs
+  __shared__ int job_count[2];  // slots in use
+  __shared__ int job_c0[2], job_parts[2];  // the CTAs that share it; 1: none, fin is set
   __shared__ int job_tmem[2];   // scores in tensor memory
   __shared__ int job_next[2];   // else: the slots / 4 that warps have taken
   __shared__ int job_last[2];   // the CTA's last unit: the tile warps take part
   __shared__ uint32_t tmem_sh;
   __shared__ float upper[D == 64 ? 4 * 32 * 4 * NT : 1];  // D = 64: o of the tile's upper slots
-  __shared__ int dead, arrived;
+  __shared__ int dead, arrived, help;
   __shared__ int64_t share[3];  // first tile, end, all tiles
   __shared__ int start[2];      // first tile's sequence, and its tile among the sequence's
 
@@ -143,7 +160,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&job_full[s], 1);
-      mbar_init(&job_empty[s], AT_MASS);
+      mbar_init(&job_empty[s], AT_FINISH);
     }
     dead = 0;
     mbar_fence_init();
@@ -379,27 +396,110 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     }
   };
 
+  // part of CTA c0 + c of a shared unit: its second slot where the unit begins, else its first
+  auto part_slot = [&](int c0, int c) { return static_cast<int64_t>(c0 + c) * 2 + (c == 0 ? 1 : 0); };
+  // o of a shared unit: four channels a thread, the parts in their order
+  auto merge_o = [&](int x, int at, int threads) {
+    T* out = static_cast<T*>(a.out) + job_out[x];
+    const int c0 = job_c0[x], parts = job_parts[x];
+    for (int y = at; y < a.heads * (D / 4); y += threads) {
+      const int head = y / (D / 4);
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+      for (int c = 0; c < parts; ++c) {
+        const float4 po = __ldcg(reinterpret_cast<const float4*>(a.part_o + part_slot(c0, c) * HN * D) + y);
+        const float f = weights_sh[c * HN + head];
+        o.x += f * po.x;
+        o.y += f * po.y;
+        o.z += f * po.z;
+        o.w += f * po.w;
+      }
+      const float inv = fin[x][1][head];
+      T* dst = out + head * a.oh + (y % (D / 4)) * 4;
+      dst[0] = T(o.x * inv);
+      dst[1] = T(o.y * inv);
+      dst[2] = T(o.z * inv);
+      dst[3] = T(o.w * inv);
+    }
+  };
+
   if (warp > AT_WARPS) {
-    if (!a.accumulate) return;
+    const int at = tid - 32 * (AT_WARPS + 1);
+    bool told = false;  // the tile warps, whether the last unit is done
     for (int job = 0;; ++job) {
       const int x = job & 1;
-      const bool there = warp_wait(&job_full[x], static_cast<uint32_t>((job >> 1) & 1));
-      if (!there && lane == 0) report(a.status, LINATTN_DEV_TIMEOUT);
-      const int count = there ? job_count[x] : -1;
-      if (count < 0) break;
+      // of one mind: a warp that gave up takes the others along
+      if (!finish_barrier_and(warp_wait(&job_full[x], static_cast<uint32_t>((job >> 1) & 1)))) {
+        if (lane == 0) report(a.status, LINATTN_DEV_TIMEOUT);
+        break;
+      }
       const int64_t unit = job_unit[x];
-      if (job_tmem[x]) {
-        tc_fence_after();
-        add_tmem(x, unit, count, 0, job_last[x] ? 3 : 1);
-        tc_fence_before();
-      } else {
-        add_scores(x, unit, count);
+      const int count = job_count[x], c0 = job_c0[x], parts = job_parts[x];
+      const bool last = job_last[x] != 0;
+      auto slot = [&](int c) { return part_slot(c0, c); };
+      bool finish = true;
+      if (parts > 1) {
+        if (at == 0) {
+          __threadfence();  // the tile warps' part before the arrival
+          const int n = atomicAdd(a.ticket + unit, 1);
+          if (n == parts - 1) a.ticket[unit] = 0;
+          __threadfence();
+          arrived = n;
+        }
+        finish_barrier();
+        finish = arrived == parts - 1;
+        if (finish)
+          for (int head = warp - (AT_WARPS + 1); head < a.heads; head += AT_FINISH / 32) {  // lanes over the parts
+            float mc[AT_PARTS / 32], lc[AT_PARTS / 32], mx = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int y = 0; y < AT_PARTS / 32; ++y) {
+              const int c = lane + 32 * y;
+              mc[y] = c < parts ? __ldcg(a.part_ml + slot(c) * 2 * HN + head) : -INFINITY;
+              lc[y] = c < parts ? __ldcg(a.part_ml + slot(c) * 2 * HN + HN + head) : 0.f;
+              mx = fmaxf(mx, mc[y]);
+            }
+#pragma unroll
+            for (int o = 16; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+#pragma unroll
+            for (int y = 0; y < AT_PARTS / 32; ++y) {
+              const float f = mc[y] == -INFINITY ? 1.f : ex2_approx(mc[y] - mx);  // scores of NaN only: m = -inf, l = NaN
+              sum += f * lc[y];
+              if (lane + 32 * y < parts) weights_sh[(lane + 32 * y) * HN + head] = f;
+            }
+#pragma unroll
+            for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (lane == 0) {
+              fin[x][0][head] = mx == -INFINITY ? 0.f : mx;
+              fin[x][1][head] = sum != 0.f ? 1.f / sum : 0.f;
+            }
+          }
+        finish_barrier();
+      }
+      if (last) {
+        if (at == 0) help = finish ? 1 : 0;
+        asm volatile("barrier.cta.sync 2, 384;" ::: "memory");
+        told = true;
+      }
+      if (finish && parts > 1) merge_o(x, at, last ? AT_THREADS - 32 : AT_FINISH);
+      if (finish && a.accumulate) {
+        if (job_tmem[x]) {
+          tc_fence_after();
+          add_tmem(x, unit, count, 0, last ? 3 : 1);
+          tc_fence_before();
+        } else {
+          add_scores(x, unit, count);
+        }
       }
       mbar_arrive(&job_empty[x]);
+      if (last) break;
+    }
+    if (!told) {
+      if (at == 0) help = 0;
+      asm volatile("barrier.cta.sync 2, 384;" ::: "memory");
     }
     tc_fence_before();
-    asm volatile("barrier.cta.sync 2, 384;" ::: "memory");  // the other warps have read theirs
-    if (warp == AT_WARPS + 1) free_tmem();
+    asm volatile("barrier.cta.sync 2, 384;" ::: "memory");  // the other warps have read their scores
+    if (warp == AT_WARPS + 1 && a.accumulate) free_tmem();
     return;
   }
 
@@ -412,28 +512,16 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
   const int vrow = (lane & 7) + ((lane >> 4) & 1) * 8, vchunk = ct * 2 + ((lane >> 3) & 1);
   const uint32_t k_off = krow * 128, v_off = HALVES * SM::HALF + (vchunk >> 3) * SM::HALF;
   int j = 0, jobs = 0;
-  bool ok = true, help = false;
-  // room for a unit's result: the mass warps are done with the one before the last
+  bool ok = true;
+  // room for a unit's result: the finishing warps are done with the one before the last
   auto job_room = [&] {
-    if (a.accumulate && jobs >= 2 && ok)
+    if (jobs >= 2 && ok)
       ok = __all_sync(0xffffffffu, mbar_wait_bounded(&job_empty[jobs & 1], static_cast<uint32_t>((jobs / 2 - 1) & 1)));
     tc_fence_after();
   };
-  auto job_send = [&](int64_t unit, int count, bool in_tmem, bool last) {  // one thread, after a barrier
-    job_unit[jobs & 1] = unit;
-    job_count[jobs & 1] = count;
-    job_tmem[jobs & 1] = in_tmem ? 1 : 0;
-    job_next[jobs & 1] = 0;
-    job_last[jobs & 1] = last ? 1 : 0;
-    mbar_arrive(&job_full[jobs & 1]);
-  };
-  for (int64_t t = t0; t < t1;) {
-    const int end = static_cast<int>(lmin(w.tiles, first + (t1 - t)));
-    const bool whole = first == 0 && end == w.tiles;  // else several CTAs share the unit
-    const bool last = t + (end - first) >= t1;        // of this CTA
-    const int64_t unit = static_cast<int64_t>(w.b) * a.H + w.h;
-    // q as the B operand: channels 16 kk + 2 tig (+ 1, + 8, + 9) of head g
-    uint32_t q[NT][D / 16][2];
+  // q as the B operand: channels 16 kk + 2 tig (+ 1, + 8, + 9) of head g
+  uint32_t q[NT][D / 16][2];
+  auto load_q = [&] {
 #pragma unroll
     for (int x = 0; x < NT; ++x) {
       const int head = x * 8 + g;
@@ -443,6 +531,15 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
 #pragma unroll
         for (int e = 0; e < 2; ++e) q[x][kk][e] = head < a.heads ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + e * 8) : 0u;
     }
+  };
+  load_q();
+  for (int64_t t = t0; t < t1;) {
+    const int end = static_cast<int>(lmin(w.tiles, first + (t1 - t))), count = w.count;
+    const bool whole = first == 0 && end == w.tiles;  // else several CTAs share the unit
+    const bool begins = first == 0;
+    const bool last = t + (end - first) >= t1;        // of this CTA
+    const int64_t unit = static_cast<int64_t>(w.b) * a.H + w.h;
+    const int64_t out_at = w.b * a.ob + (static_cast<int64_t>(w.h) * a.G + a.h0) * a.oh;
     float acc[NT][4], m[NT][2], l[NT][2];
 #pragma unroll
     for (int x = 0; x < NT; ++x) {
@@ -457,7 +554,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     if (in_tmem) job_room();
     const uint32_t sc_tmem = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + (jobs & 1) * 256 + (warp >> 2) * 128;
     for (int i = first; i < end; ++i, ++j) {
-      const int st = j % ST, valid = min(AT_ROWS, w.count - i * AT_ROWS);
+      const int st = j % ST, valid = min(AT_ROWS, count - i * AT_ROWS);
       // a warp whose wait gave up goes on through the barriers
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full[st], static_cast<uint32_t>((j / ST) & 1)));
       const uint32_t stage = ring_a + st * SM::STAGE;
@@ -480,15 +577,24 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
       for (int x = 0; x < NT; ++x)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int r = e < 2 ? r0 : r1, head = x * 8 + 2 * tig + (e & 1);
+          const int r = e < 2 ? r0 : r1;
           const float v = r < valid ? (s[x][e] + s2[x][e]) * a.scale_log2 : -INFINITY;
           s[x][e] = v;
-          if (a.accumulate && !in_tmem && r < valid && head < a.heads) sc[static_cast<int64_t>(head) * a.Ms + i * AT_ROWS + r] = v;
           grow |= v > m[x][e & 1] + 8.f;
         }
       if (in_tmem) {
 #pragma unroll
         for (int x = 0; x < NT; ++x) tmem_st4(sc_tmem + (i * NT + x) * 4, s[x]);
+      } else if (a.accumulate) {
+        float* row = sc + 2 * tig * a.Ms + i * AT_ROWS + r0;
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+            if (x * 8 + 2 * tig + c < a.heads) {
+              if (r0 < valid) row[(x * 8 + c) * a.Ms] = s[x][c];
+              if (r1 < valid) row[(x * 8 + c) * a.Ms + 8] = s[x][c + 2];
+            }
       }
       uint8_t* pb = pbuf + (j & 1) * (2 * HN * AT_PROW);
       float ps[NT][2];  // this lane's share of the tile's sums
@@ -582,7 +688,11 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[st]);
     }
-    // ---- the unit's part is done: sums over the warps
+    // ---- the unit's part is done: the next one's q on its way, sums over the warps
+    t += end - first;
+    first = 0;
+    w.next();
+    if (!last) load_q();
 #pragma unroll
     for (int x = 0; x < NT; ++x)
 #pragma unroll
@@ -613,17 +723,15 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[x][e] += upper[((ct * 32 + lane) * NT + x) * 4 + e];
     }
-    T* out = static_cast<T*>(a.out) + w.b * a.ob + (static_cast<int64_t>(w.h) * a.G + a.h0) * a.oh;
-    bool finish = true;
     if (in_tmem) {
       tmem_wait_st();
       tc_fence_before();
     } else {
       job_room();
     }
-    float (*result)[HN] = fin[jobs & 1];
     if (whole) {
       if (warp == 0 && g == 0) {
+        float (*result)[HN] = fin[jobs & 1];
 #pragma unroll
         for (int x = 0; x < NT; ++x)
 #pragma unroll
@@ -633,6 +741,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
           }
       }
       if (th == 0) {
+        T* out = static_cast<T*>(a.out) + out_at;
 #pragma unroll
         for (int x = 0; x < NT; ++x)
 #pragma unroll
@@ -642,10 +751,9 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
             if (head < a.heads) out[head * a.oh + ct * 16 + g + (e >> 1) * 8] = T(acc[x][e] * inv);
           }
       }
-      attend_barrier();
     } else {
       // slot 0: the unit began in an earlier CTA's share
-      const int64_t at = static_cast<int64_t>(blockIdx.x) * 2 + (first > 0 ? 0 : 1);
+      const int64_t at = static_cast<int64_t>(blockIdx.x) * 2 + (begins ? 1 : 0);
       float* po = a.part_o + at * HN * D;
       float* pml = a.part_ml + at * 2 * HN;
       if (th == 0) {
@@ -663,92 +771,44 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
             pml[HN + x * 8 + 2 * tig + c] = l[x][c];
           }
       }
-      __threadfence();
-      attend_barrier();
-      if (tid == 0) {
-        const int n = atomicAdd(a.ticket + unit, 1);
-        arrived = n;
-        if (n == static_cast<int>(c1 - c0)) a.ticket[unit] = 0;
-      }
-      attend_barrier();
-      finish = arrived == static_cast<int>(c1 - c0);
-      if (finish) {
-        __threadfence();
-        // part of CTA c: its second slot where the unit begins, else its first
-        auto slot = [&](int c) { return (c0 + c) * 2 + (c == 0 ? 1 : 0); };
-        const int parts = static_cast<int>(c1 - c0) + 1;
-        float* weight = reinterpret_cast<float*>(pbuf);  // [parts][HN]; P is not read any more
-        float* sums = weight + AT_PARTS * HN;            // [groups][heads * D]
-        for (int head = warp; head < a.heads; head += AT_WARPS) {  // lanes over the parts
-          float mx = -INFINITY, sum = 0.f;
-          for (int c = lane; c < parts; c += 32) mx = fmaxf(mx, __ldcg(a.part_ml + slot(c) * 2 * HN + head));
-#pragma unroll
-          for (int o = 16; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-          for (int c = lane; c < parts; c += 32) {
-            const float mc = __ldcg(a.part_ml + slot(c) * 2 * HN + head);
-            const float f = mc == -INFINITY ? 1.f : ex2_approx(mc - mx);  // scores of NaN only: m = -inf, l = NaN
-            weight[c * HN + head] = f;
-            sum += f * __ldcg(a.part_ml + slot(c) * 2 * HN + HN + head);
-          }
-#pragma unroll
-          for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-          if (lane == 0) {
-            result[0][head] = mx == -INFINITY ? 0.f : mx;
-            result[1][head] = sum != 0.f ? 1.f / sum : 0.f;
-          }
-        }
-        attend_barrier();
-        if (a.accumulate && tid == 0) job_send(unit, w.count, false, last);  // the masses beside the merge of o
-        // groups of threads over the parts, four channels a thread
-        const int quads = a.heads * (D / 4), groups = max(1, 32 * AT_WARPS / quads);
-        for (int y0 = 0; y0 < quads; y0 += 32 * AT_WARPS) {
-          const int y = y0 + tid % min(quads, 32 * AT_WARPS), grp = tid / min(quads, 32 * AT_WARPS);
-          if (y < quads && grp < groups) {
-            const int head = y / (D / 4);
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-            for (int c = grp; c < parts; c += groups) {
-              const float4 p = __ldcg(reinterpret_cast<const float4*>(a.part_o + slot(c) * HN * D) + y);
-              const float f = weight[c * HN + head];
-              o.x += f * p.x;
-              o.y += f * p.y;
-              o.z += f * p.z;
-              o.w += f * p.w;
-            }
-            reinterpret_cast<float4*>(sums)[grp * quads + y] = o;
-          }
-        }
-        attend_barrier();
-        for (int y = tid; y < a.heads * D; y += 32 * AT_WARPS) {
-          float o = 0.f;
-          for (int x = 0; x < groups; ++x) o += sums[x * quads * 4 + y];
-          out[(y / D) * a.oh + y % D] = T(o * result[1][y / D]);
-        }
-        attend_barrier();  // P is written again
-      }
     }
-    if (finish && a.accumulate) {
-      if (whole && tid == 0) job_send(unit, w.count, in_tmem, last);
-      help = last;
-      ++jobs;
-    }
-    t += end - first;
-    first = 0;
-    w.next();
-  }
-  if (a.accumulate) {
-    job_room();
-    if (tid == 0) job_send(0, -1, false, false);
     attend_barrier();
-    if (help) {  // with the masses of the last unit
-      const int x = (jobs - 1) & 1;
+    if (tid == 0) {
+      const int x = jobs & 1;
+      job_unit[x] = unit;
+      job_out[x] = out_at;
+      job_count[x] = count;
+      job_c0[x] = static_cast<int>(c0);
+      job_parts[x] = whole ? 1 : static_cast<int>(c1 - c0) + 1;
+      job_tmem[x] = in_tmem ? 1 : 0;
+      job_next[x] = 0;
+      job_last[x] = last ? 1 : 0;
+      mbar_arrive(&job_full[x]);
+    }
+    if (last && a.accumulate && t1 - t0 > 8) {
+      // meanwhile what the masses need comes to L2, from where longer shares of tiles have pushed it
+      // (12 sequences x 8 heads x 4096 slots 47.0 us, without 49.5; shorter ones lose 0.4)
+      const int lines = (count + 31) >> 5, rows = in_tmem ? 1 : 1 + a.heads;
+      for (int y = tid; y < rows * lines; y += 32 * AT_WARPS) {
+        const int head = y / lines, n = (y - head * lines) * 32;
+        const float* at = head == 0 ? a.mass + unit * a.M + n : sc + static_cast<int64_t>(head - 1) * a.Ms + n;
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
+      }
+    }
+    ++jobs;
+  }
+  asm volatile("barrier.cta.sync 2, 384;" ::: "memory");
+  if (help) {  // with the last unit
+    const int x = (jobs - 1) & 1;
+    if (job_parts[x] > 1) merge_o(x, AT_FINISH + tid, AT_THREADS - 32);
+    if (a.accumulate) {
       tc_fence_after();
       if (job_tmem[x]) add_tmem(x, job_unit[x], job_count[x], 1 + (warp >> 2), 3);
       else add_scores(x, job_unit[x], job_count[x]);
       tc_fence_before();
     }
-    asm volatile("barrier.cta.sync 2, 384;" ::: "memory");
   }
+  asm volatile("barrier.cta.sync 2, 384;" ::: "memory");
   if (!ok && lane == 0) {
     report(a.status, LINATTN_DEV_TIMEOUT);
     dead = 1;
