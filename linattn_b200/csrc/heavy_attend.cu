@@ -19,7 +19,7 @@
 // CTA has whole keeps its scores in tensor memory, which this kernel has no other use for: a warp
 // stores its accumulator fragments as they are, 4 columns a tile, and the finishing warp of the
 // same 32 lanes reads them back (4096 slots a unit for up to 8 heads, twice over; through the
-// workspace in global memory the call took 168 us instead of 162).  Longer ones, and units that
+// workspace in global memory the call took 6 us more).  Longer ones, and units that
 // several CTAs share, go through the workspace.  A shared unit's (o, m, l) are merged by the
 // finishing warps of the last CTA to arrive at it: the parts are added in their order, whoever
 // does it, so results do not depend on it.  When a CTA has no more tiles, its other eight warps

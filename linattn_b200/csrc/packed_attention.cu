@@ -26,8 +26,8 @@
 // the exponential unit (16 a clock), which the two row tiles overlap.  Taking 2 of 8 weights
 // from a polynomial on the FMA pipe instead was slower (2161 against 1798 us for 16384
 // tokens, 32 / 8 heads): the added instructions cost more issue slots and power than they save.
-// Measured (32 / 8 heads, D = 128, bf16): 4096 tokens 126 us (1090 TFLOP/s of causal work), 16384
-// tokens 1770 to 2000 us (1100 to 1250, by the box's power); both units are active 59% of the
+// Measured (32 / 8 heads, D = 128, bf16): 4096 tokens 124 us (1110 TFLOP/s of causal work), 16384
+// tokens 1770 to 2000 us (1100 to 1250, by the box's power: at 985 W the SMs run at 1.58 GHz); both units are active 59% of the
 // time.  What is in the way is TMEM, which loads of scores share with running products, and the
 // wait of a row tile for its own P V and next scores.
 // Few rows: the key range is cut into n_splits parts, whose normalised outputs and lse a second
