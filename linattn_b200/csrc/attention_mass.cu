@@ -349,7 +349,9 @@ extern "C" int32_t linattn_attention_mass_splits(int64_t Hq, int64_t Hkv, int64_
   //   a prompt of 1500 tokens, 8 kv heads of 32: 1: 105, 5: 32, 8: 25, 12: 27, 16: 29
   //   ten prompts of 5 to 923 tokens, 2 kv heads of 8: 1: 63, 3: 30, 6: 20, 8: 18, 12: 19
   //   prompts of 385 and 232 tokens, 4 kv heads of 20: 1: 33, 4: 16, 8: 12, 16: 11
-  if (ctas >= 3 * sms) return 1;
+  // Few query tiles do not pay for the second launch (8 prompts of up to 128 tokens, 4 tiles: 10.9
+  // us and 10.5 with 2 splits, 18.5 and 26.9 with the host's call; 8 tiles: 16.9 and 10.8 with 4).
+  if (ctas >= 3 * sms || q_tiles < 6) return 1;
   const int64_t rounds = ctas < sms ? 2 : 3;
   return static_cast<int32_t>(lmax(1, lmin(lmin((rounds * sms + ctas - 1) / ctas, q_tiles / 2), 64)));
 }
