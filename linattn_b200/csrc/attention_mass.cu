@@ -304,10 +304,12 @@ __global__ void __launch_bounds__(MT_THREADS, 1)
 __global__ void __launch_bounds__(256) mass_sum_kernel(const float* __restrict__ parts, int n_splits, int64_t split_stride,
                                                        int64_t Nk, const int32_t* cu, int S, float* __restrict__ mass,
                                                        int64_t mass_stride) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int64_t j = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (j >= Nk || j < cu[0] || j >= cu[S]) return;
   const float* p = parts + blockIdx.y * Nk + j;
   float s = 0.f;
+#pragma unroll 8
   for (int i = 0; i < n_splits; ++i) s += p[i * split_stride];
   mass[blockIdx.y * mass_stride + j] = s;
 }
@@ -412,9 +414,17 @@ extern "C" int linattn_attention_mass(const void* q, const void* k, int32_t dtyp
   if (dtype == LINATTN_BF16) e = D == 128 ? launch_mass<__nv_bfloat16, 128>(p, tq, tk, grid, st) : launch_mass<__nv_bfloat16, 64>(p, tq, tk, grid, st);
   else e = D == 128 ? launch_mass<__half, 128>(p, tq, tk, grid, st) : launch_mass<__half, 64>(p, tq, tk, grid, st);
   if (e == cudaSuccess && n_splits > 1) {
-    mass_sum_kernel<<<dim3(static_cast<unsigned>((N_k + 255) / 256), static_cast<unsigned>(Hkv)), 256, 0, st>>>(
-        static_cast<const float*>(workspace), n_splits, p.split_stride, N_k, cu_k, p.S, mass, mass_stride);
-    e = cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    cfg.gridDim = dim3(static_cast<unsigned>((N_k + 255) / 256), static_cast<unsigned>(Hkv));
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, mass_sum_kernel, static_cast<const float*>(workspace), static_cast<int>(n_splits),
+                           static_cast<int64_t>(p.split_stride), N_k, cu_k, p.S, mass, mass_stride);
   }
   return e == cudaSuccess ? LINATTN_OK : mass_fail(LINATTN_ECUDA, cudaGetErrorString(e));
 }
