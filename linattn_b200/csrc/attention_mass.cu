@@ -88,6 +88,7 @@ __global__ void __launch_bounds__(MT_THREADS, 1)
   // the parts of the keys with the most queries come first
   const int split = blockIdx.x % p.n_splits, kvh = blockIdx.x / p.n_splits % p.Hkv;
   PackedTile tl;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (!packed_tile(p.cu_k, p.cu_q, p.S, p.Nk, p.Nq, MT_KEYS, blockIdx.x / p.n_splits / p.Hkv, &tl)) return;
   if (!tl.sound && tid == 0) report(p.status, LINATTN_DEV_BAD_ID);
   const int k_first = tl.first, lk = tl.n, q_first = tl.other_first, lq = tl.other_n;
@@ -326,8 +327,7 @@ cudaError_t launch_mass(const MassArgs& p, const CUtensorMap& q, const CUtensorM
   static int allowed[64] = {};
   const cudaError_t e = allow_smem(kern, MassSmem<D>::BYTES, allowed);
   if (e != cudaSuccess) return e;
-  kern<<<grid, MT_THREADS, MassSmem<D>::BYTES, st>>>(p, q, k);
-  return cudaGetLastError();
+  return launch_ahead(kern, dim3(grid), MT_THREADS, MassSmem<D>::BYTES, st, p, q, k);
 }
 
 }  // namespace
@@ -414,17 +414,9 @@ extern "C" int linattn_attention_mass(const void* q, const void* k, int32_t dtyp
   if (dtype == LINATTN_BF16) e = D == 128 ? launch_mass<__nv_bfloat16, 128>(p, tq, tk, grid, st) : launch_mass<__nv_bfloat16, 64>(p, tq, tk, grid, st);
   else e = D == 128 ? launch_mass<__half, 128>(p, tq, tk, grid, st) : launch_mass<__half, 64>(p, tq, tk, grid, st);
   if (e == cudaSuccess && n_splits > 1) {
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
-    cfg.gridDim = dim3(static_cast<unsigned>((N_k + 255) / 256), static_cast<unsigned>(Hkv));
-    cfg.blockDim = dim3(256);
-    cfg.stream = st;
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, mass_sum_kernel, static_cast<const float*>(workspace), static_cast<int>(n_splits),
-                           static_cast<int64_t>(p.split_stride), N_k, cu_k, p.S, mass, mass_stride);
+    e = launch_ahead(mass_sum_kernel, dim3(static_cast<unsigned>((N_k + 255) / 256), static_cast<unsigned>(Hkv)), 256, 0, st,
+                     static_cast<const float*>(workspace), static_cast<int>(n_splits), static_cast<int64_t>(p.split_stride), N_k, cu_k,
+                     p.S, mass, mass_stride);
   }
   return e == cudaSuccess ? LINATTN_OK : mass_fail(LINATTN_ECUDA, cudaGetErrorString(e));
 }

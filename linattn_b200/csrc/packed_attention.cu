@@ -221,6 +221,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
   PackedItem ahead;
   PackedOrder order;
   if (warp == 3) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the offsets may be the previous kernel's
     if (p.S <= 64) order.load(p);
     ahead.more = packed_item(p, order, 0, &ahead) ? 1 : 0;
   }
@@ -255,6 +256,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   tc_fence_before();
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // so may q, k and v, and out may be in use
   __syncthreads();
   tc_fence_after();
   // the item of a turn, and its slot's return
@@ -719,19 +721,10 @@ cudaError_t launch_packed(const PackedArgs& p, const CUtensorMap& q, const CUten
   static int allowed[64] = {};
   const cudaError_t e = allow_smem(kern, PackedSmem<D>::BYTES, allowed);
   if (e != cudaSuccess) return e;
-  kern<<<grid, PA_THREADS, PackedSmem<D>::BYTES, st>>>(p, q, k, v);
-  const cudaError_t launched = cudaGetLastError();
+  const cudaError_t launched = launch_ahead(kern, dim3(grid), PA_THREADS, PackedSmem<D>::BYTES, st, p, q, k, v);
   if (launched != cudaSuccess || p.n_splits == 1) return launched;
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  cfg.gridDim = dim3(static_cast<unsigned>((p.Nq * p.G + 31) / 32), static_cast<unsigned>(p.Hkv));
-  cfg.blockDim = dim3(4 * D);
-  cfg.stream = st;
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, packed_merge_kernel<T, D>, p);
+  return launch_ahead(packed_merge_kernel<T, D>, dim3(static_cast<unsigned>((p.Nq * p.G + 31) / 32), static_cast<unsigned>(p.Hkv)),
+                      4 * D, 0, st, p);
 }
 
 int64_t packed_tiles(int64_t N_q, int64_t G, int64_t S, int64_t max_q) {

@@ -58,4 +58,21 @@ __device__ __forceinline__ bool packed_tile(const int32_t* cu, const int32_t* ot
   return false;
 }
 
+// Launch that does not wait for the end of the stream's previous kernel: the kernel starts with
+// what needs nothing of others and waits (griddepcontrol.wait) before it reads or writes.
+template <typename K, typename... A>
+cudaError_t launch_ahead(K kern, dim3 grid, unsigned threads, size_t smem, cudaStream_t st, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
 }  // namespace linattn

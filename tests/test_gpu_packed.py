@@ -122,6 +122,32 @@ def test_packed_attention_many_parts(cuda, splits, hq, hkv, d, dtype):
     _check_attention(o, lse, q, k, v, lq, lk, d ** -0.5, True)
 
 
+def test_packed_after_its_producers(cuda):
+    """Offsets and rows that the kernels right before write, calls whose inputs are the last one's outputs."""
+    from linattn_b200 import attention_mass, packed_attention
+
+    d = 64
+    for round_ in range(20):
+        lens = [1 + (7 * round_ + 13 * i) % 90 for i in range(9)]
+        n = torch.tensor([0] + lens, device="cuda")
+        g = torch.Generator(device="cuda").manual_seed(round_)
+        x = torch.randn(sum(lens), 4, d, generator=g, device="cuda")
+        busy = torch.randn(1 << 20, device="cuda")
+        for _ in range(3):
+            busy = busy.sin()
+        cu = n.cumsum(0, dtype=torch.int32)
+        q = x.to(torch.float16)
+        o, lse = packed_attention(q, q, q, cu)
+        o2, lse2 = packed_attention(o, o, q, cu, n_splits=2)
+        mass = attention_mass(o, o, lse2, cu, n_splits=3)
+        o3, _ = packed_attention(o2, o, o2, cu)
+        _check_attention(o, lse, q, q, q, lens, lens, d ** -0.5, True)
+        _check_attention(o2, lse2, o, o, q, lens, lens, d ** -0.5, True)
+        assert abs(float(mass.double().sum()) - sum(lens) * 4) <= 1e-4 * sum(lens) * 4
+        again, _ = packed_attention(o2, o, o2, cu)
+        assert torch.equal(o3, again)
+
+
 def test_packed_attention_growing_scores(cuda):
     """Scores that keep rising move the running maximum on every key tile."""
     from linattn_b200 import packed_attention
