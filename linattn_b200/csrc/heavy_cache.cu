@@ -186,6 +186,7 @@ __global__ void __launch_bounds__(SEL_THREADS, 2) heavy_select_kernel(const Heav
   __shared__ uint32_t above[2];             // this CTA's candidates over the threshold / equal to it
   const int tid = threadIdx.x, lane = tid & 31, cl = static_cast<int>(cluster.num_blocks()),
             rank = static_cast<int>(cluster.block_rank());
+  asm volatile("griddepcontrol.wait;" ::: "memory");               // started ahead of the previous kernel's end
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the row copies wait for this kernel's end
   const int unit_in = blockIdx.x / cl;
   const int h = unit_in % c.H, s = unit_in / c.H;
@@ -581,7 +582,7 @@ extern "C" int linattn_heavy_load(const linattn_heavy_t* cache, const void* k, c
   a.N = N;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   // CTAs for the whole GPU where the units alone are too few, each with 1024 tokens or more.
   // (The cluster that selects moving the rows too: 19.9 against 17.5 us for 32768 tokens and 8
   // heads, whose 64 CTAs are too few for the copies.)
@@ -595,8 +596,10 @@ extern "C" int linattn_heavy_load(const linattn_heavy_t* cache, const void* k, c
   attr[0].val.clusterDim.x = cl;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   cudaError_t e = cudaLaunchKernelEx(&cfg, heavy_select_kernel, c, a);
   if (e != cudaSuccess) return cuda_result(e);
   const int per = GATHER_THREADS / c.pieces * GATHER_ROWS;

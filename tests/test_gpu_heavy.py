@@ -379,3 +379,43 @@ def test_prompt_to_decode(cuda):
     for name in ("k", "v", "mass", "pos", "seen"):
         assert torch.equal(getattr(eager, name), getattr(graphed, name)), name
     assert eager.seen.tolist() == [m + 60 for m in lens]
+
+
+def test_steps_right_after_one_another(cuda):
+    """Prompt, masses, load and decode steps without a pause give what they give one at a time."""
+    from linattn_b200 import HeavyCache, attention_mass, packed_attention
+
+    hq, hkv, d, budget = 8, 2, 128, 96
+    lens = [300, 40, 777]
+    n = sum(lens)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.randn(12, n, hq, d, generator=g, device="cuda").to(torch.bfloat16)
+    new = torch.randn(6, 2, len(lens), hkv, 1, d, generator=g, device="cuda").to(torch.bfloat16)
+    ends = torch.tensor([0] + lens, device="cuda")
+
+    def chain(pause):
+        cache = HeavyCache(len(lens), hkv, d, budget, dtype=torch.bfloat16, sinks=4, recent=16)
+        outs = []
+        for r in range(3):  # the cache is loaded again, over what the steps before made of it
+            cu = ends.cumsum(0, dtype=torch.int32)
+            pause()
+            q, k, v = x[4 * r], x[4 * r + 1][:, :hkv], x[4 * r + 2][:, :hkv]
+            o, lse = packed_attention(q, k, v, cu)
+            pause()
+            mass = attention_mass(q, k, lse, cu, window=200)
+            pause()
+            cache.load(k, v, mass, cu)
+            pause()
+            outs += [o, mass]
+            for s in range(2):
+                cache.append(new[2 * r + s, 0], new[2 * r + s, 1])
+                pause()
+                outs.append(cache.attend(o[:len(lens)].unsqueeze(2).contiguous()))
+                pause()
+            outs += [cache.k.clone(), cache.v.clone(), cache.mass.clone(), cache.pos.clone(), cache.seen.clone()]
+        return outs
+
+    want = chain(torch.cuda.synchronize)
+    for _ in range(5):
+        got = chain(lambda: None)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
