@@ -13,6 +13,7 @@
 #include <cstdio>
 
 #include "launchers.cuh"
+#include "packed_tiles.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -550,10 +551,9 @@ extern "C" int linattn_heavy_append(const linattn_heavy_t* cache, const void* k_
   }
   if ((reinterpret_cast<uintptr_t>(k_new) | reinterpret_cast<uintptr_t>(v_new)) % 16)
     return heavy_fail(LINATTN_EINVAL, "append: rows must be 16-byte aligned");
-  heavy_append_kernel<<<dim3(c.H, c.B), APPEND_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(
-      c, static_cast<const uint4*>(k_new), static_cast<const uint4*>(v_new), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
-      static_cast<int>(T_new), ticket);
-  return cuda_result(cudaGetLastError());
+  return cuda_result(launch_ahead(heavy_append_kernel, dim3(c.H, c.B), APPEND_THREADS, 0, static_cast<cudaStream_t>(stream), c,
+                                  static_cast<const uint4*>(k_new), static_cast<const uint4*>(v_new), ks[0], ks[1], ks[2], vs[0],
+                                  vs[1], vs[2], static_cast<int>(T_new), ticket));
 }
 
 extern "C" int linattn_heavy_load(const linattn_heavy_t* cache, const void* k, const void* v, const int64_t* k_strides,
@@ -606,14 +606,6 @@ extern "C" int linattn_heavy_load(const linattn_heavy_t* cache, const void* k, c
   const unsigned gx = static_cast<unsigned>((lmin(c.M, N) + per - 1) / per);
   if (gx == 0) return LINATTN_OK;
   // set up while the selection runs; the positions are read after its end
-  cudaLaunchConfig_t next = {};
-  next.gridDim = dim3(gx, c.H, static_cast<unsigned>(S));
-  next.blockDim = dim3(GATHER_THREADS);
-  next.stream = st;
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  next.attrs = attr;
-  next.numAttrs = 1;
-  return cuda_result(cudaLaunchKernelEx(&next, heavy_gather_kernel, c, a, static_cast<const uint4*>(k), ks[0], ks[1],
-                                        static_cast<const uint4*>(v), vs[0], vs[1]));
+  return cuda_result(launch_ahead(heavy_gather_kernel, dim3(gx, c.H, static_cast<unsigned>(S)), GATHER_THREADS, 0, st, c, a,
+                                  static_cast<const uint4*>(k), ks[0], ks[1], static_cast<const uint4*>(v), vs[0], vs[1]));
 }
