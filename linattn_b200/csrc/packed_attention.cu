@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
   uint8_t* sq = asmem_raw + ((1024 - (smem_u32(asmem_raw) & 1023)) & 1023);  // two row tiles
   uint8_t* sk = sq + 2 * TILE;
   uint8_t* sv_ring = sk + KS * TILE;
-  __shared__ __align__(8) uint64_t q_full[2], q_empty[2], k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], v_ragged,
+  __shared__ __align__(8) uint64_t q_full[2], q_empty[2], k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], v_ragged[VS],
       s_full[2], p_full[2][2], pv_done[2], i_full[PA_ITEMS], i_empty[PA_ITEMS], last;
   __shared__ PackedItem items[PA_ITEMS];
   __shared__ uint32_t tmem_sh;
@@ -233,6 +233,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     for (int s = 0; s < VS; ++s) {
       mbar_init(&v_full[s], 1);
       mbar_init(&v_empty[s], 1);
+      mbar_init(&v_ragged[s], 1);
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&q_full[s], 1);
@@ -246,7 +247,6 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       mbar_init(&i_full[s], 1);
       mbar_init(&i_empty[s], PA_THREADS / 32 - 1);
     }
-    mbar_init(&v_ragged, 1);
     mbar_init(&last, 1);
     dead = 0;
     mbar_fence_init();
@@ -275,8 +275,10 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
   if (warp < 4) {
     regs_dec<PA_REGS_LOW>();
     if (warp == 0) {
-      int kc = 0, vc = 0, rc = 0, qc[2] = {0, 0};  // loads so far: K, V and ragged V tiles, Q of each row tile
-      bool ok = true, ragged_last = false;
+      int kc = 0, vc = 0, qc[2] = {0, 0};  // loads so far: K and V tiles, Q of each row tile
+      // a bit for each V stage: whether its last load was a ragged tile, and the parity of its ragged loads
+      uint32_t ragged = 0, ragged_par = 0;
+      bool ok = true;
       for (int turn = 0;; ++turn) {
         const PackedItem* item = take(turn, &ok);
         if (!item) break;
@@ -303,10 +305,13 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             const int st = vc % VS;
             if (vc >= VS) ok = ok && mbar_wait_bounded(&v_empty[st], static_cast<uint32_t>((vc / VS - 1) & 1));
             if (!ok || dead) return;
-            // a ragged V tile goes to warp 2 first, which passes it on
-            ragged_last = j == w.ragged;
-            if (ragged_last) ++rc;
-            uint64_t* bar = ragged_last ? &v_ragged : &v_full[st];
+            // A ragged V tile goes to warp 2 first, which passes it on.  Each stage has its barrier for
+            // that: v_empty orders a stage's loads, while ragged tiles of short items next to one
+            // another are in flight together.
+            const bool to_clear = j == w.ragged;
+            ragged = (ragged & ~(1u << st)) | (static_cast<uint32_t>(to_clear) << st);
+            ragged_par ^= static_cast<uint32_t>(to_clear) << st;
+            uint64_t* bar = to_clear ? &v_ragged[st] : &v_full[st];
             mbar_arrive_expect_tx(bar, TILE);
             for (int c = 0; c < HALVES; ++c)
               tma_load_3d(sv_ring + st * TILE + c * 16384, &tmv, 64 * c, w.kvh, w.k_first + (w.j0 + j) * 128, bar);
@@ -333,10 +338,11 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           if (qc[i] > 0) (void)mbar_wait_bounded(&q_full[i], static_cast<uint32_t>((qc[i] - 1) & 1), 200000000ull);
         for (int j = kc > KS ? kc - KS : 0; j < kc; ++j)
           (void)mbar_wait_bounded(&k_full[j % KS], static_cast<uint32_t>((j / KS) & 1), 200000000ull);
-        for (int j = vc > VS ? vc - VS : 0; j < vc; ++j)
-          if (!(ragged_last && j == vc - 1))
-            (void)mbar_wait_bounded(&v_full[j % VS], static_cast<uint32_t>((j / VS) & 1), 200000000ull);
-        if (rc > 0) (void)mbar_wait_bounded(&v_ragged, static_cast<uint32_t>((rc - 1) & 1), 200000000ull);
+        for (int j = vc > VS ? vc - VS : 0; j < vc; ++j) {
+          const int st = j % VS;
+          if ((ragged >> st) & 1u) (void)mbar_wait_bounded(&v_ragged[st], ((ragged_par >> st) & 1u) ^ 1u, 200000000ull);
+          else (void)mbar_wait_bounded(&v_full[st], static_cast<uint32_t>((j / VS) & 1), 200000000ull);
+        }
       }
     } else if (warp == 1) {
       int kc = 0, vc = 0, qc0 = 0, qc1 = 0, pc0 = 0, pc1 = 0;  // tiles so far: K, V, Q and P of each row tile
@@ -421,16 +427,18 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         }
       }
     } else if (warp == 2) {
-      int vc = 0, rc = 0;
+      int vc = 0;
+      uint32_t par = 0;  // a bit for each V stage: of its ragged tiles
       bool ok = true;
       for (int turn = 0;; ++turn) {
         const PackedItem* item = take(turn, &ok);
         if (!item) break;
         const PackedItem& w = *item;
         if (w.ragged >= 0) {
-          ok = __all_sync(0xffffffffu, mbar_wait_bounded(&v_ragged, static_cast<uint32_t>(rc++ & 1)));
+          const int st = (vc + w.ragged) % VS;
+          ok = warp_wait(&v_ragged[st], (par >> st) & 1u);
+          par ^= 1u << st;
           if (ok) {
-            const int st = (vc + w.ragged) % VS;
             const int from = (w.lk & 127) * 8;  // 16-byte pieces of the 128-byte rows of one channel half
             uint8_t* t = sv_ring + st * TILE;
             for (int c = 0; c < HALVES; ++c)

@@ -343,3 +343,37 @@ def test_packed_refusals(cuda):
         attention_mass(q, k, lse, cu, out=torch.empty(2, 9, device="cuda"))
     with pytest.raises(ValueError, match="CUDA"):
         packed_attention(q.cpu(), k.cpu(), v.cpu(), cu.cpu())
+
+
+@pytest.mark.parametrize("kind,hq,hkv,d,dtype", [
+    ("below a tile", 16, 8, 128, torch.bfloat16), ("below a tile", 8, 8, 64, torch.float16),
+    ("more than 64", 16, 8, 128, torch.float16), ("more than 64", 8, 8, 64, torch.bfloat16),
+    ("row tiles in turn", 8, 8, 128, torch.bfloat16), ("row tiles in turn", 8, 8, 64, torch.float16),
+])
+def test_packed_many_ragged_items(cuda, kind, hq, hkv, d, dtype):
+    """Several work items of one key tile to a CTA, whose V rows past the sequence (here the
+    next one's NaN and Inf) are cleared while the next items' tiles are already loaded."""
+    from linattn_b200 import packed_attention
+
+    if kind == "row tiles in turn":  # items whose second row tile is empty, then ones whose first reads nothing
+        lq = [100 if i % 2 else 2 * (128 * hkv // hq) - i for i in range(60)]
+        lk = [100 if i % 2 else 100 - i for i in range(60)]
+    else:
+        n = 64 if kind == "below a tile" else 110
+        lq = lk = [1 + (37 * i) % 127 for i in range(n)]
+    q, k, v = _inputs(31, lq, lk, hq, hkv, d, dtype)
+    cu_q, cu_k = _cu(lq), _cu(lk)
+    clean = [packed_attention(q, k, v, cu_q, cu_k, max_q=max(lq), max_k=max(lk), n_splits=n) for n in (1, None)]
+    for o, lse in clean:
+        _check_attention(o, lse, q, k, v, lq, lk, d ** -0.5, True)
+    rest = torch.zeros(sum(lq), dtype=torch.bool, device="cuda")
+    for s in range(0, len(lq), 3):  # every third sequence is sound, its neighbours are not
+        rest[int(cu_q[s]):int(cu_q[s + 1])] = True
+    for s in range(len(lq)):
+        if s % 3:
+            k[int(cu_k[s]):int(cu_k[s + 1])] = math.nan
+            v[int(cu_k[s]):int(cu_k[s + 1])] = math.nan if s % 2 else math.inf
+    o, lse = clean[0]
+    for _ in range(3):
+        o2, lse2 = packed_attention(q, k, v, cu_q, cu_k, max_q=max(lq), max_k=max(lk), n_splits=1)
+        assert torch.equal(o2[rest], o[rest]) and torch.equal(lse2[rest], lse[rest])
