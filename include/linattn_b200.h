@@ -534,8 +534,8 @@ int linattn_shard_merge(const float* scores, const int32_t* ids, int64_t R, int6
  * o = 0 and lse = -inf.  bf16 or f16 (one type), D 64 or 128, at most 128 query heads to
  * a kv head.  Strides in elements {token, head}, channels contiguous, rows and strides
  * multiples of 16 bytes.  lse (N_q, H_q) contiguous, or NULL.  max_q / max_k: at least the
- * longest sequence's query / key rows (they size the grid; rows beyond them are not
- * written).  n_splits > 1 (at most 32) cuts every key range and merges the parts through
+ * longest sequence's query / key rows (they size the grid).  Rows of no sequence, and rows of
+ * one beyond its first max_q, are not written.  n_splits > 1 (at most 32) cuts every key range and merges the parts through
  * `workspace` (linattn_packed_attention_workspace bytes, 16-byte aligned);
  * linattn_packed_attention_splits proposes a number.  Offsets that are not ascending or
  * leave the buffers are clamped and reported (LINATTN_DEV_BAD_ID).  No reference

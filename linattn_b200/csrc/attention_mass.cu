@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(MT_THREADS, 1)
   const int split = blockIdx.x % p.n_splits, kvh = blockIdx.x / p.n_splits % p.Hkv;
   PackedTile tl;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (!packed_tile(p.cu_k, p.cu_q, p.S, p.Nk, p.Nq, MT_KEYS, blockIdx.x / p.n_splits / p.Hkv, &tl)) return;
+  if (!packed_tile(p.cu_k, p.cu_q, p.S, p.Nk, p.Nq, MT_KEYS, static_cast<int>(p.Nk), blockIdx.x / p.n_splits / p.Hkv, &tl)) return;
   if (!tl.sound && tid == 0) report(p.status, LINATTN_DEV_BAD_ID);
   const int k_first = tl.first, lk = tl.n, q_first = tl.other_first, lq = tl.other_n;
   const int key0 = tl.tile * MT_KEYS, shift = lk - lq;  // query i stands at position i + shift

@@ -48,6 +48,7 @@ struct PackedArgs {
   const int32_t* cu_q;
   const int32_t* cu_k;
   int64_t Nq, Nk;
+  int max_q;         // rows of a sequence at most: later ones are not written
   int S, Hq, Hkv, G, tokens;  // tokens of a row tile (floor(128 / G))
   int inv_g;         // ceil(2^16 / G): (r inv_g) >> 16 = r / G for r < 128
   int causal;
@@ -107,7 +108,7 @@ struct PackedOrder {
         sound[e] = packed_range(p.cu_q, s, p.Nq, &first[e], &n[e]);
         sound[e] &= packed_range(p.cu_k, s, p.Nk, &other_first[e], &other_n[e]);
       }
-      pairs[e] = (n[e] + 2 * p.tokens - 1) / (2 * p.tokens);
+      pairs[e] = (min(n[e], p.max_q) + 2 * p.tokens - 1) / (2 * p.tokens);
       base[e] = max(0, other_n[e] - n[e]) / (2 * p.tokens);
       levels = max(levels, base[e] + pairs[e]);
     }
@@ -165,16 +166,16 @@ __device__ __forceinline__ bool packed_item(const PackedArgs& p, const PackedOrd
   if (p.S <= 64) {
     if (!order.find(at, &t)) return false;
   } else {  // sequence after sequence, each from its end
-    if (!packed_tile(p.cu_q, p.cu_k, p.S, p.Nq, p.Nk, 2 * p.tokens, at, &t)) return false;
-    t.tile = (t.n + 2 * p.tokens - 1) / (2 * p.tokens) - 1 - t.tile;
+    if (!packed_tile(p.cu_q, p.cu_k, p.S, p.Nq, p.Nk, 2 * p.tokens, p.max_q, at, &t)) return false;
+    t.tile = (min(t.n, p.max_q) + 2 * p.tokens - 1) / (2 * p.tokens) - 1 - t.tile;
   }
   if (!t.sound && (threadIdx.x & 31) == 0) report(p.status, LINATTN_DEV_BAD_ID);
   w->q_first = t.first;
-  w->lq = t.n;
+  w->lq = min(t.n, p.max_q);
   w->k_first = t.other_first;
   w->lk = t.other_n;
   w->t0 = t.tile * 2 * p.tokens;
-  w->shift = w->lk - w->lq;  // token t reads keys up to t + shift
+  w->shift = w->lk - t.n;  // token t reads keys up to t + shift
   int nt[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -664,15 +665,16 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
 
 // Merge of the parts of a key range: 32 rows to a block, a lane to a row, and 8 of their channels to
 // a warp.  A row's weights 2^(lse_s - max) are found by its lane in every warp; the parts are added
-// in their order.
+// in their order.  Rows that the parts do not cover (no sequence's) are left alone.
 template <typename T, int D>
 __global__ void __launch_bounds__(4 * D) packed_merge_kernel(const PackedArgs p) {
   using M = MmaOp<T>;
   constexpr int QUADS = 2;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, kvh = blockIdx.y;
-  const int64_t rows = p.Nq * p.G, row = static_cast<int64_t>(blockIdx.x) * 32 + lane;
-  if (row >= rows) return;
+  const int64_t rows = p.Nq * p.G, row0 = static_cast<int64_t>(blockIdx.x) * 32 + lane, row = lmin(row0, rows - 1);
+  PackedOwner owner;
+  owner.load(p.cu_q, p.S, p.Nq, p.max_q);
   const float* lse = p.part_lse + kvh * rows + row;
   const int64_t next = p.Hkv * rows;  // to the next part
   float mx = -INFINITY, sum = 0.f;
@@ -709,6 +711,7 @@ __global__ void __launch_bounds__(4 * D) packed_merge_kernel(const PackedArgs p)
   }
   const float inv = sum != 0.f ? 1.f / sum : 0.f;
   const int64_t token = row / p.G;
+  if (!owner.has(token) || row0 >= rows) return;
   const int head = kvh * p.G + static_cast<int>(row - token * p.G);
   T* dst = static_cast<T*>(p.out) + token * p.ot + head * p.oh + warp * QUADS * 4;
   *reinterpret_cast<uint4*>(dst) = make_uint4(M::pack(acc[0].x * inv, acc[0].y * inv), M::pack(acc[0].z * inv, acc[0].w * inv),
@@ -823,7 +826,7 @@ extern "C" int linattn_packed_attention(const void* q, const void* k, const void
   if (!tensor_map_3d(&tq, q, cu, qd, qs, qbox) || !tensor_map_3d(&tk, keys ? k : q, cu, kd, ks, kbox) ||
       !tensor_map_3d(&tv, keys ? v : q, cu, kd, vs, kbox))
     return packed_fail(LINATTN_ECUDA, "tensor map encoding failed");
-  p.cu_q = cu_q; p.cu_k = cu_k; p.Nq = N_q; p.Nk = N_k;
+  p.cu_q = cu_q; p.cu_k = cu_k; p.Nq = N_q; p.Nk = N_k; p.max_q = static_cast<int>(lmin(max_q, N_q));
   p.S = static_cast<int>(S); p.Hq = static_cast<int>(Hq); p.Hkv = static_cast<int>(Hkv);
   p.causal = causal ? 1 : 0;
   p.scale_log2 = scale * 1.4426950408889634f;

@@ -16,15 +16,68 @@ __device__ __forceinline__ bool packed_range(const int32_t* cu, int s, int64_t N
   return a == lo && b == hi;
 }
 
-// The sequence of the `idx`-th tile of `rows` rows of `cu`'s sequences, one after the other:
-// the tile among its sequence's, and the sequence's range in both `cu` and `other`.  All lanes
-// of a warp call it and get the same answer.  False past the last tile.
+// Which rows are some sequence's, among its first `most`: the others (padding before the first
+// sequence or past the last, holes between clamped offsets, rows beyond the longest sequence that
+// the caller named) are never written.  A warp asks for 32 rows in ascending order: `load`
+// fetches the offsets of up to 32 sequences, so that it can go out with other loads, and `has`
+// answers; of more sequences `has` finds the ones that matter by a search, 32 ways a step.
+struct PackedOwner {
+  const int32_t* cu;
+  int64_t N;
+  int S, most, first, n;  // the last two: of this lane's sequence
+  __device__ __forceinline__ void fetch(int s) {
+    first = n = 0;
+    if (s < S) packed_range(cu, s, N, &first, &n);
+    n = min(n, most);
+  }
+  __device__ __forceinline__ void load(const int32_t* offsets, int sequences, int64_t rows, int longest) {
+    cu = offsets;
+    S = sequences;
+    N = rows;
+    most = longest;
+    fetch(S <= 32 ? threadIdx.x & 31 : S);
+  }
+  __device__ __forceinline__ bool has(int64_t row) {
+    const int lane = threadIdx.x & 31;
+    const int64_t lo = __shfl_sync(0xffffffffu, row, 0), hi = __shfl_sync(0xffffffffu, row, 31);
+    bool owned = false;
+    auto look = [&] {
+      unsigned near = __ballot_sync(0xffffffffu, n > 0 && first <= hi && first + n > lo);
+      for (; near; near &= near - 1) {
+        const int l = __ffs(near) - 1, f = __shfl_sync(0xffffffffu, first, l), c = __shfl_sync(0xffffffffu, n, l);
+        owned |= row >= f && row < f + c;
+      }
+    };
+    if (S <= 32) {
+      look();
+      return owned;
+    }
+    int s0 = 0;  // the last sequence that begins at or before `lo` is in [s0, s0 + span)
+    for (int span = S; span > 32;) {
+      const int step = (span + 31) / 32, s = s0 + lane * step;
+      const unsigned before = __ballot_sync(0xffffffffu, lane * step < span && cu[min(s, S)] <= lo);
+      const int l = before ? 31 - __clz(before) : 0;
+      s0 += l * step;
+      span = min(step, span - l * step);
+    }
+    for (; s0 < S; s0 += 32) {
+      fetch(s0 + lane);
+      look();
+      if (__shfl_sync(0xffffffffu, s0 + 32 < S ? first : 0, 31) > hi) break;
+    }
+    return owned;
+  }
+};
+
+// The sequence of the `idx`-th tile of `rows` rows of `cu`'s sequences (`most` rows of one at
+// most), one after the other: the tile among its sequence's, and the sequence's range in both `cu`
+// and `other`.  All lanes of a warp call it and get the same answer.  False past the last tile.
 struct PackedTile {
   int tile, first, n, other_first, other_n;
   bool sound;  // no offset had to be clamped
 };
 __device__ __forceinline__ bool packed_tile(const int32_t* cu, const int32_t* other, int S, int64_t N, int64_t N_other,
-                                            int rows, int64_t idx, PackedTile* t) {
+                                            int rows, int most, int64_t idx, PackedTile* t) {
   const int lane = threadIdx.x & 31;
   int64_t base = 0;
   for (int s0 = 0; s0 < S; s0 += 32) {
@@ -34,7 +87,7 @@ __device__ __forceinline__ bool packed_tile(const int32_t* cu, const int32_t* ot
       sound = packed_range(cu, s0 + lane, N, &first, &n);
       sound &= packed_range(other, s0 + lane, N_other, &other_first, &other_n);
     }
-    const int mine = (n + rows - 1) / rows;
+    const int mine = (min(n, most) + rows - 1) / rows;
     int incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {

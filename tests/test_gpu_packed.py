@@ -377,3 +377,44 @@ def test_packed_many_ragged_items(cuda, kind, hq, hkv, d, dtype):
     for _ in range(3):
         o2, lse2 = packed_attention(q, k, v, cu_q, cu_k, max_q=max(lq), max_k=max(lk), n_splits=1)
         assert torch.equal(o2[rest], o[rest]) and torch.equal(lse2[rest], lse[rest])
+
+
+@pytest.mark.parametrize("splits", [None, 1, 3])
+@pytest.mark.parametrize("lq,lk,before,after,hq,hkv,d,dtype,max_q", [
+    ([1] * 8, [4000] * 8, 0, 56, 8, 2, 128, torch.bfloat16, None),               # single tokens in a fixed buffer
+    ([200], [8000], 0, 1500, 8, 8, 64, torch.float16, None),                     # a chunk
+    ([0, 33, 1, 150], [0, 900, 300, 150], 7, 3, 6, 2, 128, torch.float16, None), # G = 3, rows before the first one
+    ([3, 0, 5] * 30, [500, 9, 0] * 30, 5, 40, 4, 2, 64, torch.bfloat16, None),   # more sequences than a search step
+    ([2] * 1100, [300] * 1100, 33, 70, 2, 1, 64, torch.float16, None),           # than two
+    ([40, 300, 90], [600, 700, 90], 2, 9, 8, 2, 128, torch.bfloat16, 77),        # longer than the caller says
+    ([10, 90] * 40, [600, 90] * 40, 0, 0, 8, 2, 64, torch.bfloat16, 21),
+])
+def test_packed_rows_of_no_sequence_are_left_alone(cuda, splits, lq, lk, before, after, hq, hkv, d, dtype, max_q):
+    """Padding of a fixed buffer, and rows beyond the longest sequence that the caller names,
+    keep what `out` and `lse_out` hold, whatever the number of parts."""
+    from linattn_b200 import packed_attention
+
+    n = before + sum(lq) + after
+    q, k, v = _inputs(41, [n], lk, hq, hkv, d, dtype)
+    cu_q = _cu(lq) + before
+    out = torch.full_like(q, 7.0)
+    lse = torch.full((n, hq), 5.0, device="cuda")
+    scratch = torch.full((32 * n * hq * (d + 1),), math.nan, device="cuda")  # what no part writes shows
+    packed_attention(q, k, v, cu_q, _cu(lk), max_q=max_q or max(lq), max_k=max(lk), out=out, lse_out=lse, n_splits=splits,
+                     workspace=scratch)
+    inside = torch.zeros(n, dtype=torch.bool, device="cuda")
+    at = before
+    for m in lq:
+        inside[at:at + min(m, max_q or m)] = True
+        at += m
+    assert (out[~inside] == 7).all() and (lse[~inside] == 5).all()
+    want, want_lse = packed_attention(q[before:n - after].contiguous(), k, v, _cu(lq), _cu(lk), n_splits=1)
+    ours = inside[before:n - after]
+    # either side rounds its weights and its outputs once (2 u max |v|), and has a score's error e
+    # (scale sum |q k| is below 1.5 sqrt(d) here)
+    e = d * 2.0 ** -24 * 1.5 * d ** 0.5 + 2.0 ** -20
+    got, ref = out[before:n - after][ours].double(), want[ours].double()
+    assert ((got - ref).abs() <= (4.1 * U[dtype] + 4 * e) * v.abs().max().double()).all()
+    got, ref = lse[before:n - after][ours].double(), want_lse[ours].double()
+    assert torch.equal(got == -math.inf, ref == -math.inf)
+    assert ((got - ref).nan_to_num(0).abs() <= 4 * e).all()
