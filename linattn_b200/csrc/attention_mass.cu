@@ -37,6 +37,7 @@ struct MassArgs {
   const int32_t* cu_q;
   const int32_t* cu_k;
   int64_t Nq, Nk;
+  int max_k;                  // keys of a sequence at most: later ones are not written
   int S, Hq, Hkv, G, tokens;  // tokens of a 128-row query tile (floor(128 / G))
   int causal;
   int64_t window;
@@ -89,11 +90,12 @@ __global__ void __launch_bounds__(MT_THREADS, 1)
   const int split = blockIdx.x % p.n_splits, kvh = blockIdx.x / p.n_splits % p.Hkv;
   PackedTile tl;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (!packed_tile(p.cu_k, p.cu_q, p.S, p.Nk, p.Nq, MT_KEYS, static_cast<int>(p.Nk), blockIdx.x / p.n_splits / p.Hkv, &tl)) return;
+  if (!packed_tile(p.cu_k, p.cu_q, p.S, p.Nk, p.Nq, MT_KEYS, p.max_k, blockIdx.x / p.n_splits / p.Hkv, &tl)) return;
   if (!tl.sound && tid == 0) report(p.status, LINATTN_DEV_BAD_ID);
   const int k_first = tl.first, lk = tl.n, q_first = tl.other_first, lq = tl.other_n;
   const int key0 = tl.tile * MT_KEYS, shift = lk - lq;  // query i stands at position i + shift
-  const int key_tiles = min(MT_GROUPS, (lk - key0 + 127) >> 7);
+  const int keys = min(lk, p.max_k);
+  const int key_tiles = min(MT_GROUPS, (keys - key0 + 127) >> 7);
   // query tiles that read these keys, and this split's share of them
   const int w_lo = p.window > 0 && p.window < lq ? lq - static_cast<int>(p.window) : 0;
   const int q_lo = max(w_lo, p.causal ? key0 - shift : 0);
@@ -287,7 +289,7 @@ __global__ void __launch_bounds__(MT_THREADS, 1)
       report(p.status, LINATTN_DEV_TIMEOUT);
       dead = 1;
     }
-    if (key < lk) p.mass[split * p.split_stride + kvh * p.mass_stride + k_first + key] = total;
+    if (key < keys) p.mass[split * p.split_stride + kvh * p.mass_stride + k_first + key] = total;
   }
   tc_fence_before();
   __syncthreads();
@@ -300,19 +302,20 @@ __global__ void __launch_bounds__(MT_THREADS, 1)
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
-// mass = sum of the splits' parts, in their order (keys of no sequence are left alone by the
-// parts, so only keys that some sequence owns are summed)
+// mass = sum of the splits' parts, in their order.  Keys that the parts do not cover (no
+// sequence's) are left alone.
 __global__ void __launch_bounds__(256) mass_sum_kernel(const float* __restrict__ parts, int n_splits, int64_t split_stride,
-                                                       int64_t Nk, const int32_t* cu, int S, float* __restrict__ mass,
-                                                       int64_t mass_stride) {
+                                                       int64_t Nk, const int32_t* cu, int S, int max_k,
+                                                       float* __restrict__ mass, int64_t mass_stride) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int64_t j = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (j >= Nk || j < cu[0] || j >= cu[S]) return;
-  const float* p = parts + blockIdx.y * Nk + j;
+  PackedOwner owner;
+  owner.load(cu, S, Nk, max_k);
+  const float* p = parts + blockIdx.y * Nk + lmin(j, Nk - 1);
   float s = 0.f;
 #pragma unroll 8
   for (int i = 0; i < n_splits; ++i) s += p[i * split_stride];
-  mass[blockIdx.y * mass_stride + j] = s;
+  if (owner.has(j) && j < Nk) mass[blockIdx.y * mass_stride + j] = s;
 }
 
 int mass_fail(int code, const char* what) {
@@ -396,6 +399,7 @@ extern "C" int linattn_attention_mass(const void* q, const void* k, int32_t dtyp
   if (!tensor_map_3d(&tk, k, cu, kd, ks, kbox) || !tensor_map_3d(&tq, N_q > 0 ? q : k, cu, qd, qs, qbox))
     return mass_fail(LINATTN_ECUDA, "tensor map encoding failed");
   p.lse = lse; p.cu_q = cu_q; p.cu_k = cu_k; p.Nq = N_q; p.Nk = N_k;
+  p.max_k = static_cast<int>(lmin(max_k, N_k));
   p.S = static_cast<int>(S); p.Hq = static_cast<int>(Hq); p.Hkv = static_cast<int>(Hkv);
   p.causal = causal ? 1 : 0;
   p.window = window;
@@ -416,7 +420,7 @@ extern "C" int linattn_attention_mass(const void* q, const void* k, int32_t dtyp
   if (e == cudaSuccess && n_splits > 1) {
     e = launch_ahead(mass_sum_kernel, dim3(static_cast<unsigned>((N_k + 255) / 256), static_cast<unsigned>(Hkv)), 256, 0, st,
                      static_cast<const float*>(workspace), static_cast<int>(n_splits), static_cast<int64_t>(p.split_stride), N_k, cu_k,
-                     p.S, mass, mass_stride);
+                     p.S, p.max_k, mass, mass_stride);
   }
   return e == cudaSuccess ? LINATTN_OK : mass_fail(LINATTN_ECUDA, cudaGetErrorString(e));
 }

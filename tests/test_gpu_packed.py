@@ -418,3 +418,34 @@ def test_packed_rows_of_no_sequence_are_left_alone(cuda, splits, lq, lk, before,
     got, ref = lse[before:n - after][ours].double(), want_lse[ours].double()
     assert torch.equal(got == -math.inf, ref == -math.inf)
     assert ((got - ref).nan_to_num(0).abs() <= 4 * e).all()
+
+
+@pytest.mark.parametrize("splits", [None, 1, 3])
+@pytest.mark.parametrize("lens,before,after,hq,hkv,d,max_k", [
+    ([200, 0, 513, 1], 9, 300, 8, 2, 128, None),
+    ([900, 700, 40], 0, 5, 4, 2, 64, 300),        # longer than the caller says, inside a tile
+    ([900, 700, 40], 3, 0, 4, 2, 64, 512),        # and at its end
+    ([7, 0, 30] * 40, 1, 1, 6, 2, 64, None),
+    ([80, 3] * 600, 0, 33, 2, 1, 64, 50),
+])
+def test_mass_of_no_sequence_is_left_alone(cuda, splits, lens, before, after, hq, hkv, d, max_k):
+    """Keys of no sequence, and keys beyond the longest sequence that the caller names, keep
+    what `out` holds, whatever the number of splits."""
+    from linattn_b200 import attention_mass, packed_attention
+
+    n = before + sum(lens) + after
+    q, k, v = _inputs(43, [n], [n], hq, hkv, d, torch.bfloat16)
+    cu = _cu(lens) + before
+    _, lse = packed_attention(q, k, v, cu)
+    want = attention_mass(q, k, lse, cu, n_splits=1).double()
+    out = torch.full((hkv, n), 7.0, device="cuda")
+    attention_mass(q, k, lse, cu, max_q=max(lens), max_k=max_k or max(lens), out=out, n_splits=splits,
+                   workspace=torch.full((64 * hkv * n,), math.nan, device="cuda"))
+    inside = torch.zeros(n, dtype=torch.bool, device="cuda")
+    at = before
+    for m in lens:
+        inside[at:at + min(m, max_k or m)] = True
+        at += m
+    assert (out[:, ~inside] == 7).all()
+    # fp32 sums of the same positive terms in another order: each rounds at most once a term
+    assert ((out.double() - want).abs() <= 2 * max(lens) * (hq // hkv) * 2.0 ** -24 * want)[:, inside].all()
