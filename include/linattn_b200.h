@@ -555,7 +555,7 @@ int64_t linattn_packed_attention_workspace(int64_t N_q, int64_t Hq, int64_t D, i
  * Attention weight that each key has received: mass[h, j] = sum over the queries i of
  * j's sequence (its last `window` ones; 0 = all) that read key j, and over the query heads
  * of kv head h, of exp(scale * q_i . k_j - lse[i, head]).  Arguments as
- * linattn_packed_attention, lse as it writes it (a row with lse = -inf adds nothing);
+ * linattn_packed_attention, lse as it writes it (a row with lse = -inf or +inf adds nothing);
  * mass (H_kv, N_k) fp32 with row stride mass_stride.  Every key of a sequence is written, up to
  * its first max_k; keys of no sequence are not.
  * n_splits > 1 cuts the queries and sums the parts in a fixed order through `workspace`.

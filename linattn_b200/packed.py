@@ -174,7 +174,8 @@ def attention_mass(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, cu_q: to
     queries that read key ``j`` and the query heads of kv head ``h``.  ``lse (N_q, H_q)`` as
     :func:`packed_attention` returns it for the same ``q, k`` and offsets.  ``window > 0``:
     only each sequence's last ``window`` queries count.  The sums have a fixed order.
-    Keys of no sequence, and keys of one beyond its first ``max_k``, are not written."""
+    Keys of no sequence, and keys of one beyond its first ``max_k``, are not written.  A row
+    whose lse is -inf (it read nothing) or +inf adds nothing."""
     p = _planned((_layout(q), _layout(k), None, _layout(cu_q), _layout(cu_k), max_q, max_k, window, n_splits),
                  q, k, None, cu_q, cu_k, max_q, max_k, window, n_splits)
     q, sq = _aligned(q, p.copies[0], p.strides[0], p)

@@ -449,3 +449,19 @@ def test_mass_of_no_sequence_is_left_alone(cuda, splits, lens, before, after, hq
     assert (out[:, ~inside] == 7).all()
     # fp32 sums of the same positive terms in another order: each rounds at most once a term
     assert ((out.double() - want).abs() <= 2 * max(lens) * (hq // hkv) * 2.0 ** -24 * want)[:, inside].all()
+
+
+def test_mass_of_rows_without_a_finite_lse(cuda):
+    """A row whose lse is infinite adds nothing."""
+    from linattn_b200 import attention_mass, packed_attention
+
+    q, k, v = _inputs(44, [300], [300], 4, 2, 64, torch.float16)
+    cu = _cu([300])
+    _, lse = packed_attention(q, k, v, cu)
+    for n in (1, 3):
+        some = lse.clone()
+        some[::3, 1], some[1::3, 2] = math.inf, -math.inf
+        got = attention_mass(q, k, some, cu, n_splits=n)
+        some[::3, 1] = -math.inf
+        assert torch.equal(got, attention_mass(q, k, some, cu, n_splits=n))
+        assert not torch.equal(got, attention_mass(q, k, lse, cu, n_splits=n))
