@@ -540,9 +540,9 @@ extern "C" int linattn_heavy_append(const linattn_heavy_t* cache, const void* k_
                                     int32_t* status, void* stream) {
   HeavyCacheArgs c;
   if (const int rc = check_heavy(cache, &c, status)) return rc;
-  if (!k_new || !v_new || !k_strides || !v_strides || !ticket) return heavy_fail(LINATTN_EINVAL, "append: NULL pointer");
   if (T_new < 0 || T_new > (1 << 20)) return heavy_fail(LINATTN_EINVAL, "append: 0 .. 2^20 new tokens");
-  if (T_new == 0) return LINATTN_OK;
+  if (T_new == 0) return LINATTN_OK;  // a tensor of no elements has no address
+  if (!k_new || !v_new || !k_strides || !v_strides || !ticket) return heavy_fail(LINATTN_EINVAL, "append: NULL pointer");
   int64_t ks[3], vs[3];
   for (int i = 0; i < 3; ++i) {
     ks[i] = pieces_of(k_strides[i]);

@@ -419,3 +419,14 @@ def test_steps_right_after_one_another(cuda):
     for _ in range(5):
         got = chain(lambda: None)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_append_of_no_tokens(cuda):
+    from linattn_b200 import HeavyCache
+
+    cache = HeavyCache(2, 2, 64, 8, dtype=torch.float16)
+    x = torch.ones(2, 2, 3, 64, dtype=torch.float16, device="cuda")
+    cache.append(x, x)
+    cache.append(x[:, :, :0], x[:, :, :0])
+    cache.append(torch.empty(2, 2, 0, 64, dtype=torch.float16, device="cuda"), torch.empty(2, 2, 0, 64, dtype=torch.float16, device="cuda"))
+    assert cache.seen.tolist() == [3, 3]

@@ -107,3 +107,10 @@ def test_operators_refuse_cpu_tensors():
         attention_mass(q, q, torch.zeros(4, 2), cu)
     with pytest.raises(ValueError, match="cuda"):
         HeavyCache(1, 1, 64, 8, device="cpu")
+
+
+def test_heavy_append_of_no_tokens():
+    """An empty tensor's address is NULL: nothing to do, not an error."""
+    lib = L.lib()
+    assert lib.linattn_heavy_append(_heavy(), None, None, I3, I3, 0, P, None, None) == 0
+    assert lib.linattn_heavy_append(_heavy(budget=0), None, None, I3, I3, 0, P, None, None) == 1
