@@ -59,7 +59,7 @@ class HeavyCache:
         ints = torch.zeros(batch * (2 + n_kv_heads), dtype=torch.int32, device=self.device)
         self.seen, self._ticket, self._unit_ticket = ints[:batch], ints[batch:2 * batch], ints[2 * batch:]
         self.device = self.k.device
-        self._workspace: Optional[torch.Tensor] = None  # attend()'s, by its first call
+        self._scratch: dict = {}  # attend()'s workspaces by size, kept: a captured graph may hold one
         self._desc = L.Heavy(self.k.data_ptr(), self.v.data_ptr(), self.mass.data_ptr(), self.pos.data_ptr(),
                              self.seen.data_ptr(), L.dtype_code(self.k), batch, n_kv_heads, budget, head_dim, sinks, recent)
         # what every call passes
@@ -156,15 +156,19 @@ class HeavyCache:
             if out.shape != shape or out.dtype != self.dtype or out.stride(3) != 1:
                 raise ValueError("out must have q's shape and dtype with contiguous channels")
             out_strides = L.strides2(out)
-        if self._workspace is None or self._workspace.numel() < need:
-            self._workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
+        scratch = self._scratch.get(need) or self._new_scratch(need)
         L.check(self._lib.linattn_heavy_attend(
             self._ref, q.data_ptr(), hq, strides, self._scale if scale is None else float(scale), 1 if accumulate else 0,
-            out.data_ptr(), out_strides, self._unit_ticket_ptr, self._workspace.data_ptr(), need, self._status_ptr,
+            out.data_ptr(), out_strides, self._unit_ticket_ptr, scratch[0], need, self._status_ptr,
             L.raw_stream(self._index)))
         if L.strict():
             L.check_status(self.device)
         return out
+
+    def _new_scratch(self, need: int):
+        workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
+        scratch = self._scratch[need] = (workspace.data_ptr(), workspace)
+        return scratch
 
     def _plan_attend(self, q: torch.Tensor):
         """(H_q, strides of q or None where the rows have to be copied first, whether q is

@@ -430,3 +430,48 @@ def test_append_of_no_tokens(cuda):
     cache.append(x[:, :, :0], x[:, :, :0])
     cache.append(torch.empty(2, 2, 0, 64, dtype=torch.float16, device="cuda"), torch.empty(2, 2, 0, 64, dtype=torch.float16, device="cuda"))
     assert cache.seen.tolist() == [3, 3]
+
+
+def _filled(batch, hkv, d, budget, dtype, seed):
+    from linattn_b200 import HeavyCache
+
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    cache = HeavyCache(batch, hkv, d, budget, dtype=dtype)
+    cache.k.normal_(generator=g)
+    cache.v.normal_(generator=g)
+    cache.mass.uniform_(generator=g)
+    cache.pos.copy_(torch.arange(budget, device="cuda"))
+    cache.seen.fill_(budget)
+    return cache, g
+
+
+def test_captured_attend_outlives_larger_calls(cuda, monkeypatch):
+    """A graph's scratch stays its own when later calls need more, and other tensors are made."""
+    monkeypatch.setenv("LINATTN_B200_STRICT", "0")
+    cache, g = _filled(2, 2, 128, 9000, torch.bfloat16, 3)
+    q = torch.randn(2, 8, 1, 128, generator=g, device="cuda").to(torch.bfloat16)
+    many = torch.randn(2, 64, 1, 128, generator=g, device="cuda").to(torch.bfloat16)
+    before = cache.mass.clone()
+    want, want_mass = cache.attend(q), cache.mass.clone()
+    out = torch.empty_like(q)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        cache.attend(q, out=out)  # set up outside the capture
+        with torch.cuda.graph(graph, stream=side):
+            cache.attend(q, out=out)
+        cache.attend(many)
+    torch.cuda.current_stream().wait_stream(side)
+    cache.attend(many)
+    sizes = sorted({s[-1].numel() for s in cache._scratch.values()})
+    others = [torch.full((n // 4,), 7.0, device="cuda") for n in sizes for _ in range(4)]
+    with torch.cuda.stream(side):
+        others += [torch.full((n // 4,), 7.0, device="cuda") for n in sizes for _ in range(4)]
+    torch.cuda.synchronize()
+    cache.mass.copy_(before)
+    out.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(bool((x == 7).all()) for x in others)
+    assert torch.equal(out, want) and torch.equal(cache.mass, want_mass)
