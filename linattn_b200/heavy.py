@@ -29,12 +29,21 @@ from linattn_b200 import _lib as L
 __all__ = ["HeavyCache"]
 
 
+_STREAMS = 8  # streams whose arrival counts are there from the start
+
+
 class HeavyCache:
     """``budget`` slots per (sequence, kv head) with accumulated attention weights.
 
     Every update runs on the device and on the current stream: no host copy of the lengths,
     no allocation after the first step, so a decode step can be captured in a CUDA graph.  ``seen (B,)`` counts
-    the tokens of each sequence; ``min(seen, budget)`` slots are in use."""
+    the tokens of each sequence; ``min(seen, budget)`` slots are in use.
+
+    Calls that change the cache follow one another like any writes to a tensor: on one stream,
+    or on streams that wait for each other.  ``attend(accumulate=False)`` only reads, and may run
+    on several streams at once: each has scratch of its own, which stays for the cache's life
+    (a captured graph holds its address).  Graphs captured on one stream share that stream's
+    scratch, so of these only one runs at a time."""
 
     def __init__(self, batch: int, n_kv_heads: int, head_dim: int, budget: int, *, sinks: int = 0, recent: int = 1,
                  dtype: torch.dtype = torch.bfloat16, device="cuda"):
@@ -56,10 +65,12 @@ class HeavyCache:
         self.v = torch.zeros(*shape, head_dim, dtype=dtype, device=self.device)
         self.mass = torch.zeros(shape, dtype=torch.float32, device=self.device)
         self.pos = torch.zeros(shape, dtype=torch.int32, device=self.device)
-        ints = torch.zeros(batch * (2 + n_kv_heads), dtype=torch.int32, device=self.device)
-        self.seen, self._ticket, self._unit_ticket = ints[:batch], ints[batch:2 * batch], ints[2 * batch:]
+        ints = torch.zeros(batch * (2 + _STREAMS * n_kv_heads), dtype=torch.int32, device=self.device)
+        self.seen, self._ticket = ints[:batch], ints[batch:2 * batch]
+        self._unit_tickets = list(ints[2 * batch:].view(_STREAMS, -1))  # attend()'s, one a stream
         self.device = self.k.device
-        self._scratch: dict = {}  # attend()'s workspaces by size, kept: a captured graph may hold one
+        self._stream_tickets: dict = {}  # stream -> arrival counts
+        self._scratch: dict = {}         # (stream, bytes) -> their address, the workspace's, the workspace
         self._desc = L.Heavy(self.k.data_ptr(), self.v.data_ptr(), self.mass.data_ptr(), self.pos.data_ptr(),
                              self.seen.data_ptr(), L.dtype_code(self.k), batch, n_kv_heads, budget, head_dim, sinks, recent)
         # what every call passes
@@ -69,7 +80,6 @@ class HeavyCache:
         self._desc.maps = ctypes.addressof(self._maps)
         self._index = self.device.index
         self._plans: dict = {}  # checked arguments of append and attend, by shapes, strides and types
-        self._unit_ticket_ptr = self._unit_ticket.data_ptr()
         self._status_ptr = L.status_word(self.device).data_ptr()
         self._scale = 1.0 / math.sqrt(head_dim)
 
@@ -156,18 +166,30 @@ class HeavyCache:
             if out.shape != shape or out.dtype != self.dtype or out.stride(3) != 1:
                 raise ValueError("out must have q's shape and dtype with contiguous channels")
             out_strides = L.strides2(out)
-        scratch = self._scratch.get(need) or self._new_scratch(need)
+        stream = L.raw_stream(self._index)
+        scratch = self._scratch.get((stream, need)) or self._new_scratch(stream, need)
         L.check(self._lib.linattn_heavy_attend(
             self._ref, q.data_ptr(), hq, strides, self._scale if scale is None else float(scale), 1 if accumulate else 0,
-            out.data_ptr(), out_strides, self._unit_ticket_ptr, scratch[0], need, self._status_ptr,
-            L.raw_stream(self._index)))
+            out.data_ptr(), out_strides, scratch[0], scratch[1], need, self._status_ptr, stream))
         if L.strict():
             L.check_status(self.device)
         return out
 
-    def _new_scratch(self, need: int):
+    def _new_scratch(self, stream: int, need: int):
+        """Workspace and arrival counts of attend() on a stream, kept: a graph may hold them."""
+        tickets = self._stream_tickets.get(stream)
+        if tickets is None:
+            taken = len(self._stream_tickets)
+            if taken < _STREAMS:
+                tickets = self._unit_tickets[taken]
+            elif torch.cuda.is_current_stream_capturing():  # zeros would be there after a replay only
+                raise RuntimeError(f"attend() has run on {taken} streams: call it once on this one before capturing it")
+            else:
+                tickets = torch.zeros_like(self._unit_tickets[0])
+                self._unit_tickets.append(tickets)
+            self._stream_tickets[stream] = tickets
         workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
-        scratch = self._scratch[need] = (workspace.data_ptr(), workspace)
+        scratch = self._scratch[stream, need] = (tickets.data_ptr(), workspace.data_ptr(), workspace)
         return scratch
 
     def _plan_attend(self, q: torch.Tensor):

@@ -475,3 +475,33 @@ def test_captured_attend_outlives_larger_calls(cuda, monkeypatch):
     torch.cuda.synchronize()
     assert all(bool((x == 7).all()) for x in others)
     assert torch.equal(out, want) and torch.equal(cache.mass, want_mass)
+
+
+def test_attend_without_weights_on_streams_at_once(cuda, monkeypatch):
+    """Calls that only read the cache do not meet, on more streams than have counts from the start."""
+    from linattn_b200 import heavy
+
+    monkeypatch.setenv("LINATTN_B200_STRICT", "0")
+    cache, g = _filled(1, 2, 128, 2500, torch.float16, 4)
+    n = heavy._STREAMS + 2
+    q = [torch.randn(1, 16, 1, 128, generator=g, device="cuda").to(torch.float16) for _ in range(n)]
+    mass = cache.mass.clone()
+    want = [cache.attend(x, accumulate=False) for x in q]
+    outs = [[torch.empty_like(x) for _ in range(20)] for x in q]
+    streams = [torch.cuda.Stream() for _ in range(n)]
+    torch.cuda.synchronize()
+    for r in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                cache.attend(q[i], accumulate=False, out=outs[i][r])
+    torch.cuda.synchronize()
+    for i in range(n):
+        assert all(torch.equal(o, want[i]) for o in outs[i])
+    assert torch.equal(cache.mass, mass)
+    assert all(bool((t == 0).all()) for t in cache._unit_tickets)
+    # the counts of a further stream would be zero after a replay only: refused, not wrong
+    late = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="before capturing"):
+        with torch.cuda.graph(graph, stream=late):
+            cache.attend(q[0], accumulate=False, out=outs[0][0])
