@@ -623,7 +623,8 @@ int linattn_heavy_append(const linattn_heavy_t* cache, const void* k_new, const 
  * heads.  q, out (batch, H_q, head_dim) in the cache's dtype, strides {sequence, head} in
  * elements.  f16 / bf16, head_dim 64 or 128.  A sequence without slots gets o = 0.
  * ticket: batch * n_kv_heads int32 of scratch that holds zeros before and after every
- * call.  workspace: linattn_heavy_attend_workspace bytes, 16-byte aligned.
+ * call (one that reports LINATTN_DEV_TIMEOUT may leave others: zero it again).  Calls that
+ * overlap on the GPU need a ticket and a workspace each.  workspace: linattn_heavy_attend_workspace bytes, 16-byte aligned.
  */
 int linattn_heavy_attend(const linattn_heavy_t* cache, const void* q, int64_t Hq, const int64_t* q_strides /*[2]*/,
                          float scale, int32_t accumulate, void* out, const int64_t* out_strides /*[2]*/,

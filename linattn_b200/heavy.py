@@ -84,8 +84,12 @@ class HeavyCache:
         self._scale = 1.0 / math.sqrt(head_dim)
 
     def reset(self) -> None:
-        """Forget every token."""
+        """Forget every token.  A cache whose call reported a wait that gave up needs this
+        before its next call: the arrival counts may have stayed where that call left them."""
         self.seen.zero_()
+        self._ticket.zero_()
+        for tickets in self._unit_tickets:
+            tickets.zero_()
 
     def load(self, k: torch.Tensor, v: torch.Tensor, mass: torch.Tensor, cu: torch.Tensor,
              rows: Optional[torch.Tensor] = None) -> None:

@@ -505,3 +505,28 @@ def test_attend_without_weights_on_streams_at_once(cuda, monkeypatch):
     with pytest.raises(RuntimeError, match="before capturing"):
         with torch.cuda.graph(graph, stream=late):
             cache.attend(q[0], accumulate=False, out=outs[0][0])
+
+
+def test_reset_after_a_call_that_gave_up(cuda):
+    """Arrival counts that an abandoned call has left are gone after reset()."""
+    from linattn_b200 import HeavyCache
+
+    b, h, d, budget, dtype = 2, 2, 64, 700, torch.float16
+    g = torch.Generator(device="cuda").manual_seed(6)
+    n = 2000
+    k, v = (torch.randn(n, h, d, generator=g, device="cuda").to(dtype) for _ in range(2))
+    mass, q = torch.rand(h, n, generator=g, device="cuda"), torch.randn(b, 8, 1, d, generator=g, device="cuda").to(dtype)
+    new = torch.randn(2, b, h, 1, d, generator=g, device="cuda").to(dtype)
+    results = []
+    for left in (0, 1, 40):
+        cache = HeavyCache(b, h, d, budget, dtype=dtype)
+        cache._ticket.fill_(left)
+        for t in cache._unit_tickets:
+            t.fill_(left)
+        cache.reset()
+        cache.load(k, v, mass, _cu([900, 1100]))
+        outs = [cache.step(q, new[i], new[1 - i], out=torch.full_like(q, math.nan)) for i in range(2)]
+        results.append(outs + [cache.mass.clone(), cache.pos.clone(), cache.seen.clone()])
+    for other in results[1:]:
+        assert all(torch.equal(x, y) for x, y in zip(results[0], other))
+    assert results[0][-1].tolist() == [902, 1102]
