@@ -237,6 +237,11 @@ def raw_stream(device_index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(device_index)
 
 
+def current_device() -> int:
+    """Index of the device that launches go to."""
+    return torch._C._cuda_getDevice()
+
+
 def stream_of(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
 

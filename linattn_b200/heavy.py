@@ -97,6 +97,9 @@ class HeavyCache:
         ``(H_kv, N)`` fp32: prompt ``s`` replaces row ``rows[s]`` (int32; default ``s``) of the
         cache.  One of at most ``budget`` tokens is kept whole; of a longer one the sinks, the
         recent tokens and those of most mass (lowest position on ties), by ascending position."""
+        if L.current_device() != self._index:
+            with torch.cuda.device(self._index):
+                return self.load(k, v, mass, cu, rows)
         dev = L.require_cuda(k, v, mass, cu, rows, self.k)
         if k.dim() != 3 or k.shape[1:] != (self.n_kv_heads, self.head_dim) or v.shape != k.shape:
             raise ValueError(f"k and v must be (N, {self.n_kv_heads}, {self.head_dim})")
@@ -122,6 +125,9 @@ class HeavyCache:
         """Take ``(B, H_kv, T_new, D)`` keys / values, one token after the other: each fills the
         next empty slot or, in a full cache, replaces the slot of least mass (lowest slot on
         ties) outside the sinks and the last ``recent`` tokens (itself among them)."""
+        if L.current_device() != self._index:
+            with torch.cuda.device(self._index):
+                return self.append(k, v)
         key = (k.shape, k.stride(), v.shape, v.stride(), k.dtype, v.dtype, k.get_device(), v.get_device())
         plan = self._plans.get(key)
         if plan is None:
@@ -155,6 +161,9 @@ class HeavyCache:
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """``o (B, H_q, 1, D)`` of one query token per sequence over the slots in use; with
         ``accumulate`` each slot's mass grows by its weights, summed over its group's heads."""
+        if L.current_device() != self._index:
+            with torch.cuda.device(self._index):
+                return self.attend(q, scale=scale, accumulate=accumulate, out=out)
         shape = q.shape
         key = (shape, q.stride(), q.dtype, q.get_device())
         plan = self._plans.get(key)

@@ -134,6 +134,10 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     ranges when there are few rows; ``workspace``: fp32 scratch for it, allocated if None."""
     p = _planned((_layout(q), _layout(k), _layout(v), _layout(cu_q), _layout(cu_k), max_q, max_k, None, n_splits),
                  q, k, v, cu_q, cu_k, max_q, max_k, None, n_splits)
+    if L.current_device() != p.device.index:
+        with torch.cuda.device(p.device):
+            return packed_attention(q, k, v, cu_q, cu_k, max_q=max_q, max_k=max_k, causal=causal, scale=scale, out=out,
+                                    lse_out=lse_out, n_splits=n_splits, workspace=workspace)
     q, sq = _aligned(q, p.copies[0], p.strides[0], p)
     k, sk = _aligned(k, p.copies[1], p.strides[1], p)
     v, sv = _aligned(v, p.copies[2], p.strides[2], p)
@@ -178,6 +182,10 @@ def attention_mass(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, cu_q: to
     whose lse is -inf (it read nothing) or +inf adds nothing."""
     p = _planned((_layout(q), _layout(k), None, _layout(cu_q), _layout(cu_k), max_q, max_k, window, n_splits),
                  q, k, None, cu_q, cu_k, max_q, max_k, window, n_splits)
+    if L.current_device() != p.device.index:
+        with torch.cuda.device(p.device):
+            return attention_mass(q, k, lse, cu_q, cu_k, max_q=max_q, max_k=max_k, causal=causal, window=window, scale=scale,
+                                  out=out, n_splits=n_splits, workspace=workspace)
     q, sq = _aligned(q, p.copies[0], p.strides[0], p)
     k, sk = _aligned(k, p.copies[1], p.strides[1], p)
     if lse.shape != (p.nq, p.hq) or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != p.device:
