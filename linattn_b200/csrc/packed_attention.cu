@@ -62,6 +62,7 @@ struct PackedArgs {
   float4* part_o;    // (n_splits, H_kv, D / 4, N_q G) four channels of a row
   float* part_lse;   // (n_splits, H_kv, N_q G)
   int64_t items;     // at most: tiles x H_kv x n_splits
+  uint64_t item_ns;  // limit of a wait for an item's end
   int32_t* status;
 };
 
@@ -260,10 +261,14 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
   asm volatile("griddepcontrol.wait;" ::: "memory");  // so may q, k and v, and out may be in use
   __syncthreads();
   tc_fence_after();
+  // A wait for another warp's end of an item, not of a tile: a part of 2^27 keys takes seconds.
+  auto item_wait = [&](uint64_t* bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, p.item_ns)) != 0;
+  };
   // the item of a turn, and its slot's return
   auto take = [&](int turn, bool* ok) -> const PackedItem* {
     const int slot = turn % PA_ITEMS;
-    *ok = *ok && warp_wait(&i_full[slot], static_cast<uint32_t>((turn / PA_ITEMS) & 1));
+    *ok = *ok && item_wait(&i_full[slot], static_cast<uint32_t>((turn / PA_ITEMS) & 1));
     return *ok && items[slot].more ? &items[slot] : nullptr;
   };
   auto give_back = [&](int turn) {
@@ -437,7 +442,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         const PackedItem& w = *item;
         if (w.ragged >= 0) {
           const int st = (vc + w.ragged) % VS;
-          ok = warp_wait(&v_ragged[st], (par >> st) & 1u);
+          ok = item_wait(&v_ragged[st], (par >> st) & 1u);
           par ^= 1u << st;
           if (ok) {
             const int from = (w.lk & 127) * 8;  // 16-byte pieces of the 128-byte rows of one channel half
@@ -456,7 +461,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     } else {
       for (int turn = 0;; ++turn) {
         if (turn > 0) ahead.more = packed_item(p, order, turn, &ahead) ? 1 : 0;
-        if (turn >= PA_ITEMS && !warp_wait(&i_empty[turn % PA_ITEMS], static_cast<uint32_t>((turn / PA_ITEMS - 1) & 1))) {
+        if (turn >= PA_ITEMS && !item_wait(&i_empty[turn % PA_ITEMS], static_cast<uint32_t>((turn / PA_ITEMS - 1) & 1))) {
           if (lane == 0) {
             report(p.status, LINATTN_DEV_TIMEOUT);
             dead = 1;
@@ -840,6 +845,8 @@ extern "C" int linattn_packed_attention(const void* q, const void* k, const void
   if (Hkv > 65535 || n_splits > 32) return packed_fail(LINATTN_EUNSUPPORTED, "more than 65535 kv heads, or than 32 splits");
   if (tiles == 0) return LINATTN_OK;
   p.items = tiles * Hkv * n_splits;
+  // 2 s as every wait; a key tile of an item takes about 2 us, and two items may lie ahead
+  p.item_ns = 2000000000ull + static_cast<uint64_t>(N_k / 128 / n_splits) * 8000ull;
   const unsigned grid = static_cast<unsigned>(lmin(sm_count(), p.items));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;

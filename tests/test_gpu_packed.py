@@ -465,3 +465,22 @@ def test_mass_of_rows_without_a_finite_lse(cuda):
         some[::3, 1] = -math.inf
         assert torch.equal(got, attention_mass(q, k, some, cu, n_splits=n))
         assert not torch.equal(got, attention_mass(q, k, lse, cu, n_splits=n))
+
+
+def test_packed_part_that_outlasts_a_wait(cuda):
+    """One part of 2.4e8 keys runs for longer than a bounded wait: no warp takes that for a fault.
+    Scores of 0: lse = log(keys), whose fp32 sum of whole numbers below 2^28 is exact."""
+    from linattn_b200 import _lib as L
+    from linattn_b200 import packed_attention
+
+    n, d = 240_000_005, 64
+    if torch.cuda.mem_get_info()[0] < 3 * n * d:
+        pytest.skip("needs 46 GB")
+    q = torch.ones(1, 1, d, dtype=torch.bfloat16, device="cuda")
+    k = torch.zeros(n, 1, d, dtype=torch.bfloat16, device="cuda")
+    o, lse = packed_attention(q, k, k, _cu([1]), _cu([n]), n_splits=1)
+    assert L.read_status(cuda) == 0
+    assert (o == 0).all()
+    assert abs(float(lse) - math.log(n)) <= 2.0 ** -19 * math.log(n)
+    del k
+    torch.cuda.empty_cache()
