@@ -237,9 +237,7 @@ def raw_stream(device_index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(device_index)
 
 
-def current_device() -> int:
-    """Index of the device that launches go to."""
-    return torch._C._cuda_getDevice()
+current_device = torch._C._cuda_getDevice  # index of the device that launches go to
 
 
 def stream_of(t: torch.Tensor) -> int:

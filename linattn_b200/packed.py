@@ -38,6 +38,7 @@ class _Plan(NamedTuple):
     ws_bytes: int
     dtype: int
     device: torch.device
+    index: int         # of the device
     copies: tuple      # operands whose rows have to be copied first
     strides: tuple     # of the operands, as the library takes them
     out_strides: object
@@ -95,8 +96,8 @@ def _plan(q, k, v, cu_q, cu_k, max_q, max_k, window, n_splits) -> _Plan:
     copies = tuple(not _on_grid(x) for _, x in operands)
     # a copy is contiguous
     strides = tuple(L.i64_array((x.shape[1] * d, d)) if c else L.strides2(x) for c, (_, x) in zip(copies, operands))
-    return _Plan(s, nq, nk, hq, hkv, d, max_q, max_k, n, ws, L.dtype_code(q), dev, copies, strides, L.i64_array((hq * d, d)),
-                 q.is_contiguous())
+    return _Plan(s, nq, nk, hq, hkv, d, max_q, max_k, n, ws, L.dtype_code(q), dev, dev.index, copies, strides,
+                 L.i64_array((hq * d, d)), q.is_contiguous())
 
 
 def _planned(key, *args) -> _Plan:
@@ -134,8 +135,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     ranges when there are few rows; ``workspace``: fp32 scratch for it, allocated if None."""
     p = _planned((_layout(q), _layout(k), _layout(v), _layout(cu_q), _layout(cu_k), max_q, max_k, None, n_splits),
                  q, k, v, cu_q, cu_k, max_q, max_k, None, n_splits)
-    if L.current_device() != p.device.index:
-        with torch.cuda.device(p.device):
+    if L.current_device() != p.index:
+        with torch.cuda.device(p.index):
             return packed_attention(q, k, v, cu_q, cu_k, max_q=max_q, max_k=max_k, causal=causal, scale=scale, out=out,
                                     lse_out=lse_out, n_splits=n_splits, workspace=workspace)
     q, sq = _aligned(q, p.copies[0], p.strides[0], p)
@@ -163,7 +164,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
         q.data_ptr(), k.data_ptr(), v.data_ptr(), p.dtype, p.nq, p.nk, p.hq, p.hkv, p.d, sq, sk, sv, cu_q.data_ptr(),
         (cu_q if cu_k is None else cu_k).data_ptr(), p.s, p.max_q, p.max_k, 1 if causal else 0,
         p.d ** -0.5 if scale is None else float(scale), out.data_ptr(), out_strides, lse_out.data_ptr(),
-        p.n_splits, L.ptr(workspace), ws_bytes, L.status_word(p.device).data_ptr(), L.raw_stream(p.device.index)))
+        p.n_splits, L.ptr(workspace), ws_bytes, L.status_word(p.device).data_ptr(), L.raw_stream(p.index)))
     if L.strict():
         L.check_status(p.device)
     return out, lse_out
@@ -182,8 +183,8 @@ def attention_mass(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, cu_q: to
     whose lse is -inf (it read nothing) or +inf adds nothing."""
     p = _planned((_layout(q), _layout(k), None, _layout(cu_q), _layout(cu_k), max_q, max_k, window, n_splits),
                  q, k, None, cu_q, cu_k, max_q, max_k, window, n_splits)
-    if L.current_device() != p.device.index:
-        with torch.cuda.device(p.device):
+    if L.current_device() != p.index:
+        with torch.cuda.device(p.index):
             return attention_mass(q, k, lse, cu_q, cu_k, max_q=max_q, max_k=max_k, causal=causal, window=window, scale=scale,
                                   out=out, n_splits=n_splits, workspace=workspace)
     q, sq = _aligned(q, p.copies[0], p.strides[0], p)
@@ -204,7 +205,7 @@ def attention_mass(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, cu_q: to
         q.data_ptr(), k.data_ptr(), p.dtype, p.nq, p.nk, p.hq, p.hkv, p.d, sq, sk, lse.data_ptr(), cu_q.data_ptr(),
         (cu_q if cu_k is None else cu_k).data_ptr(), p.s, p.max_q, p.max_k, 1 if causal else 0, int(window),
         p.d ** -0.5 if scale is None else float(scale), out.data_ptr(), out.stride(0), p.n_splits, L.ptr(workspace),
-        ws_bytes, L.status_word(p.device).data_ptr(), L.raw_stream(p.device.index)))
+        ws_bytes, L.status_word(p.device).data_ptr(), L.raw_stream(p.index)))
     if L.strict():
         L.check_status(p.device)
     return out
