@@ -535,10 +535,11 @@ int linattn_shard_merge(const float* scores, const int32_t* ids, int64_t R, int6
  * a kv head.  Strides in elements {token, head}, channels contiguous, rows and strides
  * multiples of 16 bytes.  lse (N_q, H_q) contiguous, or NULL.  max_q / max_k: at least the
  * longest sequence's query / key rows (they size the grid).  Rows of no sequence, and rows of
- * one beyond its first max_q, are not written.  n_splits > 1 (at most 32) cuts every key range and merges the parts through
- * `workspace` (linattn_packed_attention_workspace bytes, 16-byte aligned);
- * linattn_packed_attention_splits proposes a number.  Offsets that are not ascending or
- * leave the buffers are clamped and reported (LINATTN_DEV_BAD_ID).  No reference
+ * one beyond its first max_q, are not written.  n_splits > 1 (at most 32) cuts every key
+ * range and merges the parts through `workspace` (linattn_packed_attention_workspace bytes,
+ * 16-byte aligned); linattn_packed_attention_splits proposes a number.  A part of very many
+ * keys of like weight loses precision in its fp32 sums (2.6e-3 of o at 2^20 keys, in
+ * proportion to them): cut such ranges.  Offsets that are not ascending or leave the buffers are clamped and reported (LINATTN_DEV_BAD_ID).  No reference
  * counterpart in one operator: dense_attention over each sequence
  * (src/linattn/core.py:148-181).
  */
@@ -596,8 +597,8 @@ int linattn_heavy_maps(const linattn_heavy_t* cache, void* maps);
 
 /*
  * Packed prompts into the cache: sequence s of k, v (N, H_kv, head_dim) (strides {token,
- * head} in elements) fills cache row rows[s] (rows NULL: row s).  A sequence of at most
- * `budget` tokens is kept whole; of a longer one the first `sinks`, the last `recent` and
+ * head} in elements) fills cache row rows[s] (rows NULL: row s), each row at most once: the
+ * sequences are taken at the same time.  A sequence of at most `budget` tokens is kept whole; of a longer one the first `sinks`, the last `recent` and
  * those of most mass among the rest (lowest position on ties, NaN above all), in ascending
  * position.  mass (H_kv, N), row stride mass_stride.  The row's masses, positions and
  * `seen` are replaced.

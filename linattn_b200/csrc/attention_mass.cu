@@ -52,8 +52,9 @@ constexpr int MT_GROUPS = 4;  // warpgroups on scores, each with a TMEM buffer o
 constexpr int MT_THREADS = 128 * (1 + MT_GROUPS);
 constexpr int MT_KEYS = 128 * MT_GROUPS;  // keys of a CTA
 
-// Of every 8 pairs of weights, those computed on the FMA pipe (ex2_poly2: 2.7e-6 off, as the sums
-// of thousands of them 1e-7): none / 2 / 3 / 4 of 8 took 1379 / 1237 / 1210 / about 1400 us for 16384
+// Of every 8 pairs of weights, those computed on the FMA pipe (ex2_poly2: up to 2.7e-6 off each, which
+// a key that few queries read keeps; sums of thousands of them are 2.3e-7 off, 4.4e-8 with every
+// weight and sum in fp32): none / 2 / 3 / 4 of 8 took 1379 / 1237 / 1210 / about 1400 us for 16384
 // tokens, 32 / 8 heads, D = 128.
 constexpr uint32_t MT_POLY = 0x52;
 

@@ -41,8 +41,8 @@ __device__ __forceinline__ uint32_t mass_key(float f) { return f != f ? 0xffffff
 // slot) gives the least (key, slot) by one 64-bit minimum; the row is then written by the
 // first threads.  Several new tokens are taken one after the other.  The last CTA of a
 // sequence (a ticket) moves `seen`, which every CTA of the sequence has read before its
-// ticket was drawn.  Bound by a launch's latency for few units (8 heads of 512 slots: 3.5 us)
-// and by HBM and L2 for many (64 x 8 x 4096 slots, 17 MB: 6.2 us).
+// ticket was drawn.  Bound by a launch's latency for few units (8 heads of 512 slots: 3.2 us)
+// and by HBM and L2 for many (64 x 8 x 4096 slots, 17 MB: 5.7 us; both in a graph).
 constexpr int APPEND_THREADS = 256;
 
 __global__ void __launch_bounds__(APPEND_THREADS) heavy_append_kernel(const HeavyCacheArgs c,
@@ -134,8 +134,9 @@ __global__ void __launch_bounds__(APPEND_THREADS) heavy_append_kernel(const Heav
 // another instead.  Then every CTA knows how many kept tokens lie before its part and writes
 // the positions and masses of its own in order.  The rows are moved by a second kernel, spread
 // evenly over the GPU: what is kept is not spread evenly over the prompt (`recent` tokens all
-// lie at its end).  Measured, both kernels: 32768 tokens to 2048 slots, 8 heads, D = 128 17.2 us,
-// most of it barriers and remote reads of the selection.
+// lie at its end).  Measured, both kernels in a graph: 32768 tokens to 2048 slots, 8 heads,
+// D = 128 15.1 us, 16 ragged prompts to 1024 slots, D = 64 21.1 us, most of it barriers and remote
+// reads of the selection.
 constexpr int SEL_THREADS = 512;
 constexpr int SEL_PER = 16;                        // tokens of a thread in one round
 constexpr int SEL_ROUND = SEL_THREADS * SEL_PER;   // tokens of a CTA in one round

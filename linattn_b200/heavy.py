@@ -35,9 +35,10 @@ _STREAMS = 8  # streams whose arrival counts are there from the start
 class HeavyCache:
     """``budget`` slots per (sequence, kv head) with accumulated attention weights.
 
-    Every update runs on the device and on the current stream: no host copy of the lengths,
-    no allocation after the first step, so a decode step can be captured in a CUDA graph.  ``seen (B,)`` counts
-    the tokens of each sequence; ``min(seen, budget)`` slots are in use.
+    Every update runs on the device and on the current stream: no host copy of the lengths, and
+    no allocation after the first step on a stream but for an output that is not given (``out``),
+    so a decode step can be captured in a CUDA graph.  ``seen (B,)`` counts the tokens of each
+    sequence; ``min(seen, budget)`` slots are in use.
 
     Calls that change the cache follow one another like any writes to a tensor: on one stream,
     or on streams that wait for each other.  ``attend(accumulate=False)`` only reads, and may run
@@ -95,7 +96,7 @@ class HeavyCache:
              rows: Optional[torch.Tensor] = None) -> None:
         """Take packed prompts ``k, v (N, H_kv, D)`` with offsets ``cu (S + 1,)`` and masses
         ``(H_kv, N)`` fp32: prompt ``s`` replaces row ``rows[s]`` (int32; default ``s``) of the
-        cache.  One of at most ``budget`` tokens is kept whole; of a longer one the sinks, the
+        cache; a row that is named twice ends up with a mixture.  One of at most ``budget`` tokens is kept whole; of a longer one the sinks, the
         recent tokens and those of most mass (lowest position on ties), by ascending position."""
         if L.current_device() != self._index:
             with torch.cuda.device(self._index):
