@@ -53,13 +53,14 @@ __global__ void __launch_bounds__(256) lse_combine_kernel(const float* __restric
 
 // Clears the tensor-core attention's work counter (the workspace header) in place of a
 // memset node, as a kernel that can itself start early behind the previous
-// kernel (programmatic dependent launch) and lets the attention launch behind it: it
-// clears, allows its dependents, then waits for its own prerequisite so that it ends
-// only after the previous kernel (whose results the attention reads) has ended.
+// kernel (programmatic dependent launch) and lets the attention launch behind it.  It
+// clears only after the previous kernel's end: that one may use the same memory, as an
+// attention on the same workspace does, or a kernel whose inputs the allocator has
+// handed out again.
 __global__ void __launch_bounds__(256) attn_counters_clear_kernel(int4* __restrict__ words, int n16) {
-  for (int i = threadIdx.x; i < n16; i += blockDim.x) words[i] = make_int4(0, 0, 0, 0);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  for (int i = threadIdx.x; i < n16; i += blockDim.x) words[i] = make_int4(0, 0, 0, 0);
 }
 
 cudaError_t launch_attn_counters_clear(void* words, int64_t bytes, cudaStream_t stream) {
